@@ -199,6 +199,109 @@ int nsq_fp8_quantize(const void* w, int w_dtype, int64_t N, int64_t K, uint8_t* 
 int nsq_fp8_quantize_noalloc(const void* w, int w_dtype, int64_t N, int64_t K, uint8_t* weight_fp8,
                              float* weight_scale, void* stream);
 
+/*
+ * int8 linear (W8A8). No counterpart in the reference (its formats are AWQ and
+ * FP8 weights with 16-bit activations); it stands beside them.
+ *
+ * nsq_int8_quantize: rows of x [M, K] (F16, BF16 or F32) to int8 codes and one
+ * fp32 scale per row, for weights (per output channel) and activations (per
+ * token) alike:
+ *   scale[m] = max_k |x[m, k]| / 127 (1 where that is 0)
+ *   codes[m, k] = rint(x[m, k] / scale[m]), nearest-even, in [-127, 127].
+ * A row with a NaN or an infinity gets that as its scale.
+ *
+ * nsq_int8_linear: y = (codes(x) . weight_int8^T) * scale(x) * weight_scale
+ * + bias, summed in int32 (exact), scaled in fp32 and rounded once; x_dtype is
+ * F16 or BF16, y has the same. It launches the row quantiser into the
+ * workspace (nsq_int8_linear_workspace_size(M, K) bytes, 16-byte aligned,
+ * stream-ordered like y), then the product. A token with a NaN or an infinity
+ * gives a row of NaN.
+ *
+ * nsq_int8_linear_quantized: the product alone, of codes the caller keeps
+ * (quantised once, used by several layers); y_dtype is F16 or BF16.
+ *
+ * Requires K % 16 == 0, K <= 131072 (int32 sums), codes, weight, x and y
+ * 16-byte aligned.
+ */
+int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* codes, float* scale, void* stream);
+size_t nsq_int8_linear_workspace_size(int64_t M, int64_t K);
+int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N, const int8_t* weight_int8,
+                    const float* weight_scale, const void* bias, int bias_dtype, void* y, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int nsq_int8_linear_quantized(const int8_t* codes, const float* scale, int64_t M, int64_t K, int64_t N,
+                              const int8_t* weight_int8, const float* weight_scale, const void* bias, int bias_dtype,
+                              void* y, int y_dtype, void* stream);
+
+/*
+ * 8-bit key/value cache: a pool of pages, as the reference's paged cache
+ * (nano_sglang/engine/paged_kv_cache.py:62-69), whose rows (one token, one kv
+ * head) are head_dim codes and one fp32 scale:
+ *   scale = max|row| / 127 (NSQ_KV_INT8) or max|row| / 448 (NSQ_KV_FP8), 1
+ *           where that is 0
+ *   code  = rint(row / scale) or e4m3(row / scale), nearest-even
+ *   value = code * scale
+ * (scales are >= 0; a row with a NaN or an infinity reads back as NaN).
+ * Strides are in elements, in the order page, token, head; head_dim is
+ * contiguous, so token-major and head-major pools both fit. Code strides are
+ * multiples of 16, code pointers 16-byte aligned, head_dim a multiple of 16 up
+ * to 256, num_pages * page_size < 2^31.
+ *
+ * Values on the device that a call cannot check before its launch -- a slot
+ * or page outside the pool, a length outside the page table -- are skipped and
+ * recorded as NSQ_EINVAL in the status word (tags 200 slot written, 201 slot
+ * read, 202 page, 203 length); nothing outside the buffers is touched.
+ */
+#define NSQ_KV_INT8 0
+#define NSQ_KV_FP8 1
+typedef struct nsq_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_pages, page_size, kv_heads, head_dim;
+  int64_t k_stride[3], v_stride[3];             /* codes: page, token, head */
+  int64_t k_scale_stride[3], v_scale_stride[3]; /* scales: page, token, head */
+  int codes;                                    /* NSQ_KV_INT8 or NSQ_KV_FP8 */
+} nsq_kv_cache;
+
+/*
+ * Quantise k and v [T, kv_heads, head_dim] (x_dtype F16 or BF16; token and
+ * head strides in elements, multiples of 8, pointers 16-byte aligned) into the
+ * places slots[t] = page * page_size + offset; a negative slot is a padded
+ * token and is skipped. Places that no slot names stay as they were. Slots are
+ * distinct: of two tokens with the same slot the stored row is unspecified.
+ */
+int nsq_kv_cache_write(const nsq_kv_cache* cache, const void* k, const void* v, int x_dtype, const int64_t* k_stride,
+                       const int64_t* v_stride, int64_t T, const int64_t* slots, void* stream);
+
+/* Read rows back as F16 or BF16: k, v [T, kv_heads, head_dim] contiguous,
+ * code * scale rounded once; zeros where a slot is negative. */
+int nsq_kv_cache_read(const nsq_kv_cache* cache, const int64_t* slots, int64_t T, void* k, void* v, int out_dtype,
+                      void* stream);
+
+/*
+ * Decode attention: one query token per sequence over its cached keys and
+ * values (causal_lm.py:340, decode batches).
+ *   out[b, h] = sum_t softmax_t(softmax_scale * q[b, h] . k[t]) v[t],
+ *   lse[b, h] = log sum_t exp(softmax_scale * q[b, h] . k[t])   (lse may be NULL)
+ * over the first seq_lens[b] tokens of sequence b, token t in page
+ * page_table[b, t / page_size]; query head h reads kv head h / (H / kv_heads).
+ * A sequence of length 0 gives 0 and -inf. q [B, H, head_dim] (F16 or BF16;
+ * sequence and head strides in elements, multiples of 8, 16-byte aligned); out
+ * [B, H, head_dim] in q's dtype, contiguous; page_table int32 [B, table_width]
+ * with a row stride. Table entries past a sequence's last page are not read.
+ * Scores, maxima and sums are fp32; the weights of v are fp16, relative to
+ * their maximum. The workspace (nsq_kv_attention_workspace_size bytes, 16-byte
+ * aligned, stream-ordered like out, any contents) holds partial results; its
+ * size depends on the arguments and the device alone, never on seq_lens.
+ */
+size_t nsq_kv_attention_workspace_size(int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                       int64_t table_width);
+int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, const int64_t* q_stride, int64_t B,
+                            int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                            const int32_t* seq_lens, float softmax_scale, void* out, float* lse, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* Limit, in nanoseconds, of every bounded device-side wait that reports to the
  * status word (0 restores the default of 2 s; nsq_device_status_reset also
  * restores it). The wind-down waits that let in-flight copies land after a

@@ -33,6 +33,22 @@ c_int = ctypes.c_int
 c_int64 = ctypes.c_int64
 c_size_t = ctypes.c_size_t
 
+# code types of the 8-bit key/value cache
+KV_INT8 = 0
+KV_FP8 = 1
+
+
+class KvCacheDesc(ctypes.Structure):
+    """struct nsq_kv_cache of include/nsq.h."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("num_pages", c_int64), ("page_size", c_int64), ("kv_heads", c_int64), ("head_dim", c_int64),
+                ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3),
+                ("k_scale_stride", c_int64 * 3), ("v_scale_stride", c_int64 * 3), ("codes", c_int)]
+
+
+_KV = ctypes.POINTER(KvCacheDesc)
+_I64S = ctypes.POINTER(c_int64)
+
 # name -> (restype, argtypes); the complete exported surface of include/nsq.h
 SIGNATURES = {
     "nsq_strerror": (ctypes.c_char_p, [c_int]),
@@ -62,6 +78,17 @@ SIGNATURES = {
     "nsq_fp8_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_size_t,
                                  c_void_p]),
     "nsq_fp8_quantize_noalloc": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "nsq_int8_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "nsq_int8_linear_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "nsq_int8_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                                c_void_p, c_void_p, c_size_t, c_void_p]),
+    "nsq_int8_linear_quantized": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                          c_int, c_void_p, c_int, c_void_p]),
+    "nsq_kv_cache_write": (c_int, [_KV, c_void_p, c_void_p, c_int, _I64S, _I64S, c_int64, c_void_p, c_void_p]),
+    "nsq_kv_cache_read": (c_int, [_KV, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
+    "nsq_kv_attention_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "nsq_kv_attention_decode": (c_int, [_KV, c_void_p, c_int, _I64S, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                        c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "nsq_set_pdl": (c_int, [c_int]),
     "nsq_set_wait_limit_ns": (c_int, [ctypes.c_uint64]),
     "nsq_set_sm_reserve": (c_int, [c_int]),

@@ -590,4 +590,190 @@ int nsq_fp8_quantize(const void* w, int w_dtype, int64_t N, int64_t K, uint8_t* 
   return e == cudaSuccess ? NSQ_OK : NSQ_ECUDA;
 }
 
+int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* codes, float* scale, void* stream) {
+  if (M < 0 || K <= 0 || M > kIntMax || K > kIntMax) return NSQ_EINVAL;
+  if (!(valid_act_dtype(x_dtype) || x_dtype == NSQ_DTYPE_F32)) return NSQ_EINVAL;
+  if (M == 0) return NSQ_OK;
+  if (!x || !codes || !scale) return NSQ_EINVAL;
+  int rc = check_device();
+  if (rc != NSQ_OK) return rc;
+  return launch_int8_quantize(x, x_dtype, M, K, codes, scale, static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? NSQ_OK
+             : NSQ_ECUDA;
+}
+
+constexpr int64_t kInt8MaxK = 131072;  // 128 * 127 * 131072 < 2^31
+
+// Workspace: the codes, then (16-byte aligned) the scales.
+static size_t int8_codes_bytes(int64_t M, int64_t K) { return ((size_t)M * (size_t)K + 15) & ~(size_t)15; }
+
+size_t nsq_int8_linear_workspace_size(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || M > kIntMax || K > kInt8MaxK) return 0;
+  return int8_codes_bytes(M, K) + (size_t)M * sizeof(float);
+}
+
+static int int8_check(int64_t M, int64_t K, int64_t N, const void* x, const int8_t* w, const float* ws,
+                      const void* bias, int bias_dtype, const void* y, int y_dtype) {
+  if (M < 0 || K <= 0 || N <= 0 || M > kIntMax || K > kIntMax || N > kIntMax) return NSQ_EINVAL;
+  if (!valid_act_dtype(y_dtype) || !valid_bias_dtype(bias_dtype)) return NSQ_EINVAL;
+  if ((bias_dtype == NSQ_DTYPE_NONE) != (bias == nullptr)) return NSQ_EINVAL;
+  if (K % 16 != 0 || K > kInt8MaxK) return NSQ_ENOTSUP;
+  if (M == 0) return NSQ_OK;
+  if (!x || !w || !ws || !y) return NSQ_EINVAL;
+  if (!aligned16(x) || !aligned16(y) || !aligned16(w)) return NSQ_EALIGN;
+  return check_device();
+}
+
+int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N, const int8_t* weight_int8,
+                    const float* weight_scale, const void* bias, int bias_dtype, void* y, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  int rc = int8_check(M, K, N, x, weight_int8, weight_scale, bias, bias_dtype, y, x_dtype);
+  if (rc != NSQ_OK || M == 0) return rc;
+  if (!workspace || workspace_bytes < nsq_int8_linear_workspace_size(M, K)) return NSQ_EWORKSPACE;
+  if (!aligned16(workspace)) return NSQ_EALIGN;
+  int8_t* codes = static_cast<int8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(codes + int8_codes_bytes(M, K));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (launch_int8_quantize(x, x_dtype, M, K, codes, scale, s) != cudaSuccess) return NSQ_ECUDA;
+  return run_int8_rows(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
+                                x_dtype == NSQ_DTYPE_BF16, y, true},
+                       s);
+}
+
+int nsq_int8_linear_quantized(const int8_t* codes, const float* scale, int64_t M, int64_t K, int64_t N,
+                              const int8_t* weight_int8, const float* weight_scale, const void* bias, int bias_dtype,
+                              void* y, int y_dtype, void* stream) {
+  int rc = int8_check(M, K, N, codes, weight_int8, weight_scale, bias, bias_dtype, y, y_dtype);
+  if (rc != NSQ_OK || M == 0) return rc;
+  if (!scale) return NSQ_EINVAL;
+  return run_int8_rows(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
+                                y_dtype == NSQ_DTYPE_BF16, y, false},
+                       static_cast<cudaStream_t>(stream));
+}
+
+// Checks a cache descriptor; on NSQ_OK `out` is what the kernels take.
+static int kv_check(const nsq_kv_cache* c, KvCache* out) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return NSQ_EINVAL;
+  if (c->codes != NSQ_KV_INT8 && c->codes != NSQ_KV_FP8) return NSQ_EINVAL;
+  if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->head_dim <= 0) return NSQ_EINVAL;
+  if (c->head_dim % 16 != 0 || c->head_dim > 256) return NSQ_ENOTSUP;
+  if (c->num_pages > kIntMax / c->page_size || c->kv_heads > kIntMax) return NSQ_ENOTSUP;
+  if (!aligned16(c->k) || !aligned16(c->v)) return NSQ_EALIGN;
+  for (int i = 0; i < 3; ++i) {
+    if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_scale_stride[i] < 0 || c->v_scale_stride[i] < 0) {
+      return NSQ_EINVAL;
+    }
+    if (c->k_stride[i] % 16 != 0 || c->v_stride[i] % 16 != 0) return NSQ_EALIGN;
+  }
+  KvCache r{};
+  r.k = static_cast<uint8_t*>(c->k);
+  r.v = static_cast<uint8_t*>(c->v);
+  r.ks = c->k_scale;
+  r.vs = c->v_scale;
+  for (int i = 0; i < 3; ++i) {
+    r.k_stride[i] = c->k_stride[i];
+    r.v_stride[i] = c->v_stride[i];
+    r.ks_stride[i] = c->k_scale_stride[i];
+    r.vs_stride[i] = c->v_scale_stride[i];
+  }
+  r.num_pages = (int)c->num_pages;
+  r.page_size = (int)c->page_size;
+  r.kv_heads = (int)c->kv_heads;
+  r.head_dim = (int)c->head_dim;
+  *out = r;
+  return NSQ_OK;
+}
+
+int nsq_kv_cache_write(const nsq_kv_cache* cache, const void* k, const void* v, int x_dtype, const int64_t* k_stride,
+                       const int64_t* v_stride, int64_t T, const int64_t* slots, void* stream) {
+  KvCache c;
+  int rc = kv_check(cache, &c);
+  if (rc != NSQ_OK) return rc;
+  if (T < 0 || !valid_act_dtype(x_dtype) || !k_stride || !v_stride) return NSQ_EINVAL;
+  if (T > ((int64_t)1 << 30) / c.kv_heads) return NSQ_ENOTSUP;
+  if (T == 0) return NSQ_OK;
+  if (!k || !v || !slots) return NSQ_EINVAL;
+  if (!aligned16(k) || !aligned16(v)) return NSQ_EALIGN;
+  for (int i = 0; i < 2; ++i) {
+    if (k_stride[i] < 0 || v_stride[i] < 0) return NSQ_EINVAL;
+    if (k_stride[i] % 8 != 0 || v_stride[i] % 8 != 0) return NSQ_EALIGN;
+  }
+  if ((rc = check_device()) != NSQ_OK) return rc;
+  return launch_kv_write(c, k, k_stride, v, v_stride, slots, (int)T, cache->codes == NSQ_KV_FP8,
+                         x_dtype == NSQ_DTYPE_BF16, static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? NSQ_OK
+             : NSQ_ECUDA;
+}
+
+int nsq_kv_cache_read(const nsq_kv_cache* cache, const int64_t* slots, int64_t T, void* k, void* v, int out_dtype,
+                      void* stream) {
+  KvCache c;
+  int rc = kv_check(cache, &c);
+  if (rc != NSQ_OK) return rc;
+  if (T < 0 || !valid_act_dtype(out_dtype)) return NSQ_EINVAL;
+  if (T > ((int64_t)1 << 30) / c.kv_heads) return NSQ_ENOTSUP;
+  if (T == 0) return NSQ_OK;
+  if (!k || !v || !slots) return NSQ_EINVAL;
+  if (!aligned16(k) || !aligned16(v)) return NSQ_EALIGN;
+  if ((rc = check_device()) != NSQ_OK) return rc;
+  return launch_kv_read(c, slots, (int)T, k, v, cache->codes == NSQ_KV_FP8, out_dtype == NSQ_DTYPE_BF16,
+                        static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? NSQ_OK
+             : NSQ_ECUDA;
+}
+
+// B, H, kv_heads, head_dim and the page table's shape as the kernel can take them
+static int kv_attn_check(int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                         int64_t table_width) {
+  if (B < 0 || H <= 0 || kv_heads <= 0 || head_dim <= 0 || page_size <= 0 || table_width < 0) return NSQ_EINVAL;
+  if (H % kv_heads != 0) return NSQ_EINVAL;
+  if (head_dim % 16 != 0 || head_dim > 256) return NSQ_ENOTSUP;
+  if (H > (1 << 20) || B > ((int64_t)1 << 30) / H) return NSQ_ENOTSUP;
+  if (table_width > ((int64_t)1 << 30) / page_size) return NSQ_ENOTSUP;
+  return NSQ_OK;
+}
+
+size_t nsq_kv_attention_workspace_size(int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                       int64_t table_width) {
+  if (kv_attn_check(B, H, kv_heads, head_dim, page_size, table_width) != NSQ_OK || B == 0) return 0;
+  return kv_attn_workspace(B, (int)(H / kv_heads), (int)kv_heads, (int)head_dim, table_width * page_size);
+}
+
+int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, const int64_t* q_stride, int64_t B,
+                            int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                            const int32_t* seq_lens, float softmax_scale, void* out, float* lse, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  KvAttnArgs a{};
+  int rc = kv_check(cache, &a.c);
+  if (rc != NSQ_OK) return rc;
+  rc = kv_attn_check(B, H, a.c.kv_heads, a.c.head_dim, a.c.page_size, table_width);
+  if (rc != NSQ_OK) return rc;
+  if (!valid_act_dtype(q_dtype) || !q_stride || table_stride < 0) return NSQ_EINVAL;
+  if (!(softmax_scale - softmax_scale == 0.f)) return NSQ_EINVAL;  // NaN or infinite
+  if (B == 0) return NSQ_OK;
+  if (!q || !out || !seq_lens || (table_width > 0 && !page_table)) return NSQ_EINVAL;
+  if (q_stride[0] < 0 || q_stride[1] < 0) return NSQ_EINVAL;
+  if (!aligned16(q) || !aligned16(out) || q_stride[0] % 8 != 0 || q_stride[1] % 8 != 0) return NSQ_EALIGN;
+  if ((rc = check_device()) != NSQ_OK) return rc;
+  const size_t need = nsq_kv_attention_workspace_size(B, H, a.c.kv_heads, a.c.head_dim, a.c.page_size, table_width);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return NSQ_EWORKSPACE;
+  if (need > 0 && !aligned16(workspace)) return NSQ_EALIGN;
+  a.q = q;
+  a.q_stride[0] = q_stride[0];
+  a.q_stride[1] = q_stride[1];
+  a.B = (int)B;
+  a.H = (int)H;
+  a.table = page_table;
+  a.table_stride = table_stride;
+  a.capacity = (int)(table_width * a.c.page_size);
+  a.seq_lens = seq_lens;
+  a.scale = softmax_scale;
+  a.out = out;
+  a.lse = lse;
+  return launch_kv_attn(a, cache->codes == NSQ_KV_FP8, q_dtype == NSQ_DTYPE_BF16, workspace,
+                        static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? NSQ_OK
+             : NSQ_ECUDA;
+}
+
 }  // extern "C"

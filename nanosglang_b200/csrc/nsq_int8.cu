@@ -1,0 +1,227 @@
+// int8 linear (W8A8): y = (xc . wc^T) * xs * ws + bias, with xc, wc int8 codes,
+// one fp32 scale per token (xs) and per output channel (ws); the sums are
+// exact int32. Rows are quantised by int8_quantize_kernel.
+//
+// run_int8_rows: mma.sync.m16n8k32 with the weight rows as the 16 rows and the
+// tokens as the columns. Both operands want four consecutive k per register
+// and the order of k is free, so every lane reads 16 consecutive bytes of its
+// row and feeds them to two MMAs as they come: weights go from global memory
+// to the tensor cores without shared memory or conversion.
+#include "nsq_common.cuh"
+#include "nsq_internal.h"
+#include "nsq_rows8.cuh"
+
+namespace nsq {
+
+namespace {
+
+constexpr int kQThreads = 256;
+
+// ---------------------------------------------------------------------------
+// Row quantiser: one CTA per row. NV vectors of 16 bytes per thread are kept
+// in registers between the maximum and the codes (one pass over DRAM); NV = 0
+// takes any row length, alignment and type, element by element, and reads the
+// row twice (the second time from L2).
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float load_elem(const void* p, int dtype, int64_t i) {
+  if (dtype == NSQ_DTYPE_F32) return static_cast<const float*>(p)[i];
+  const uint16_t u = static_cast<const uint16_t*>(p)[i];
+  return dtype == NSQ_DTYPE_BF16 ? elem_to_float<true>(u) : elem_to_float<false>(u);
+}
+
+__device__ __forceinline__ float block_nan_max(float m) {
+  __shared__ float red[kQThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = nan_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = red[0];
+#pragma unroll
+  for (int i = 1; i < kQThreads / 32; ++i) m = nan_max(m, red[i]);
+  return m;
+}
+
+template <int NV, bool BF16>
+__global__ void __launch_bounds__(kQThreads) int8_quantize_kernel(const uint16_t* __restrict__ x, int K,
+                                                                  int8_t* __restrict__ codes,
+                                                                  float* __restrict__ scale, int pdl) {
+  if (pdl) pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  const uint4* src = reinterpret_cast<const uint4*>(x + row * K);
+  const int nvec = K / 8;
+  uint4 v[NV];
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int i = j * kQThreads + threadIdx.x;
+    v[j] = i < nvec ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = nan_max(m, fabsf(elem_to_float<BF16>((uint16_t)(w[i / 2] >> (16 * (i & 1))))));
+  }
+  const float s = row_scale<false>(block_nan_max(m));
+  if (threadIdx.x == 0) scale[row] = s;
+  const RowDiv dv(s);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int i = j * kQThreads + threadIdx.x;
+    if (i >= nvec) break;
+    const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+    uint32_t c[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c[e / 4] |= (uint32_t)row_code<false>(dv(elem_to_float<BF16>((uint16_t)(w[e / 2] >> (16 * (e & 1))))))
+                  << (8 * (e & 3));
+    }
+    reinterpret_cast<uint2*>(codes + row * K)[i] = make_uint2(c[0], c[1]);
+  }
+}
+
+__global__ void __launch_bounds__(kQThreads) int8_quantize_any_kernel(const void* __restrict__ x, int dtype, int64_t K,
+                                                                      int8_t* __restrict__ codes,
+                                                                      float* __restrict__ scale, int pdl) {
+  if (pdl) pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  float m = 0.f;
+  for (int64_t i = threadIdx.x; i < K; i += kQThreads) m = nan_max(m, fabsf(load_elem(x, dtype, row * K + i)));
+  const float s = row_scale<false>(block_nan_max(m));
+  if (threadIdx.x == 0) scale[row] = s;
+  const RowDiv dv(s);
+  for (int64_t i = threadIdx.x; i < K; i += kQThreads) {
+    codes[row * K + i] = (int8_t)row_code<false>(dv(load_elem(x, dtype, row * K + i)));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Product, rows of the weight streamed through mma.sync
+// ---------------------------------------------------------------------------
+constexpr int kRWarps = 8;
+
+__device__ __forceinline__ void mma_16832_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 ldg_w(const int8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+struct RowsParams {
+  const int8_t* x;
+  const float* xscale;
+  const int8_t* w;
+  const float* wscale;
+  const void* bias;
+  int bias_dtype;
+  void* y;
+  int M, K, N;
+  int pdl_x;  // x and xscale come from the kernel ahead
+};
+
+// 16 weight rows x 8 * MT tokens per CTA; its warps take 64-column chunks in
+// turn and add their int32 sums in shared memory (exact, so the order is free).
+template <int MT, bool BF16>
+__global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParams p) {
+  __shared__ int acc_s[16][8 * MT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (8 * MT);
+  for (int i = threadIdx.x; i < 16 * (8 * MT + 1); i += kRWarps * 32) (&acc_s[0][0])[i] = 0;
+  if (p.pdl_x) pdl_wait_prior_grids();
+  const int8_t* w0 = p.w + (int64_t)(n0 + g) * p.K;
+  const int8_t* w1 = w0 + (int64_t)8 * p.K;
+  const bool r0 = n0 + g < p.N, r1 = n0 + g + 8 < p.N;
+  int d[MT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0;
+#pragma unroll 2
+  for (int k = warp * 64 + t * 16; k - t * 16 < p.K; k += kRWarps * 64) {
+    const bool in = k < p.K;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const uint4 a = in && r0 ? ldg_w(w0 + k) : zero, c = in && r1 ? ldg_w(w1 + k) : zero;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = m0 + 8 * i + g;
+      const uint4 b = in && m < p.M ? *reinterpret_cast<const uint4*>(p.x + (int64_t)m * p.K + k) : zero;
+      mma_16832_s8(d[i], a.x, c.x, a.y, c.y, b.x, b.y);
+      mma_16832_s8(d[i], a.z, c.z, a.w, c.w, b.z, b.w);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    atomicAdd(&acc_s[g][8 * i + 2 * t], d[i][0]);
+    atomicAdd(&acc_s[g][8 * i + 2 * t + 1], d[i][1]);
+    atomicAdd(&acc_s[g + 8][8 * i + 2 * t], d[i][2]);
+    atomicAdd(&acc_s[g + 8][8 * i + 2 * t + 1], d[i][3]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * 8 * MT; i += kRWarps * 32) {
+    const int n = n0 + (i & 15), m = m0 + (i >> 4);
+    if (n < p.N && m < p.M) {
+      const float y = (float)acc_s[i & 15][i >> 4] * p.xscale[m] * __ldg(p.wscale + n);
+      const float bn = load_bias(p.bias, p.bias_dtype, n);
+      static_cast<uint16_t*>(p.y)[(int64_t)m * p.N + n] = float_to_elem<BF16>(p.bias ? y + bn : y);
+    }
+  }
+}
+
+template <typename F, typename... A>
+cudaError_t launch(F kern, dim3 grid, int threads, cudaStream_t stream, bool pdl, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+}  // namespace
+
+cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K, int8_t* codes, float* scale,
+                                 cudaStream_t stream) {
+  const bool pdl = pdl_enabled();
+  const dim3 grid((unsigned)rows);
+  const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 8 * 8 * kQThreads &&
+                   ((reinterpret_cast<uintptr_t>(x) & 15) | (reinterpret_cast<uintptr_t>(codes) & 7)) == 0;
+  if (!vec) return launch(int8_quantize_any_kernel, grid, kQThreads, stream, pdl, x, dtype, K, codes, scale, (int)pdl);
+  const uint16_t* x16 = static_cast<const uint16_t*>(x);
+  const int per = (int)((K / 8 + kQThreads - 1) / kQThreads);
+#define NSQ_Q(NV)                                                                                             \
+  (dtype == NSQ_DTYPE_BF16                                                                                    \
+       ? launch(int8_quantize_kernel<NV, true>, grid, kQThreads, stream, pdl, x16, (int)K, codes, scale, (int)pdl) \
+       : launch(int8_quantize_kernel<NV, false>, grid, kQThreads, stream, pdl, x16, (int)K, codes, scale, (int)pdl))
+  return per <= 1 ? NSQ_Q(1) : per <= 2 ? NSQ_Q(2) : per <= 4 ? NSQ_Q(4) : NSQ_Q(8);
+#undef NSQ_Q
+}
+
+int run_int8_rows(const Int8Args& a, cudaStream_t stream) {
+  const RowsParams p{a.x, a.xscale, a.w, a.wscale, a.bias, a.bias ? a.bias_dtype : NSQ_DTYPE_NONE, a.y, a.M, a.K, a.N,
+                     a.after_quantize || pdl_enabled()};
+  const int mt = a.M <= 8 ? 1 : a.M <= 16 ? 2 : a.M <= 32 ? 4 : 8;
+  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 8 * mt - 1) / (8 * mt)));
+#define NSQ_R(MT)                                                                                      \
+  (a.y_bf16 ? launch(int8_rows_kernel<MT, true>, grid, kRWarps * 32, stream, p.pdl_x, p)               \
+            : launch(int8_rows_kernel<MT, false>, grid, kRWarps * 32, stream, p.pdl_x, p))
+  const cudaError_t e = mt == 1 ? NSQ_R(1) : mt == 2 ? NSQ_R(2) : mt == 4 ? NSQ_R(4) : NSQ_R(8);
+#undef NSQ_R
+  return e == cudaSuccess ? NSQ_OK : NSQ_ECUDA;
+}
+
+}  // namespace nsq

@@ -42,6 +42,51 @@ cudaError_t launch_awq_from_autoawq(const int32_t* qweight_kn8, const int32_t* q
 cudaError_t launch_fp8_quantize(const void* w, int dtype, int64_t total, uint8_t* codes,
                                 float* scale, void* workspace, cudaStream_t stream);
 
+// int8 linear: rows quantised to int8 with one scale each, then the product.
+cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K, int8_t* codes, float* scale,
+                                 cudaStream_t stream);
+struct Int8Args {
+  const int8_t* x;      // codes [M, K]
+  const float* xscale;  // [M]
+  int M, K, N;
+  const int8_t* w;      // codes [N, K]
+  const float* wscale;  // [N]
+  const void* bias;
+  int bias_dtype;
+  int y_bf16;
+  void* y;  // [M, N]
+  bool after_quantize;  // the kernel ahead on the stream is launch_int8_quantize's, writing x and xscale
+};
+int run_int8_rows(const Int8Args& a, cudaStream_t stream);
+
+// 8-bit key/value cache. Strides in elements: page, token, head; head_dim contiguous.
+struct KvCache {
+  uint8_t *k, *v;  // codes
+  float *ks, *vs;  // scales
+  int64_t k_stride[3], v_stride[3], ks_stride[3], vs_stride[3];
+  int num_pages, page_size, kv_heads, head_dim;
+};
+cudaError_t launch_kv_write(const KvCache& c, const void* k, const int64_t* k_stride, const void* v,
+                            const int64_t* v_stride, const int64_t* slots, int T, bool fp8, bool bf16,
+                            cudaStream_t stream);
+cudaError_t launch_kv_read(const KvCache& c, const int64_t* slots, int T, void* k, void* v, bool fp8, bool bf16,
+                           cudaStream_t stream);
+struct KvAttnArgs {
+  KvCache c;
+  const void* q;
+  int64_t q_stride[2];  // sequence, head
+  int B, H;
+  const int32_t* table;
+  int64_t table_stride;
+  int capacity;  // tokens a table row can name
+  const int32_t* seq_lens;
+  float scale;
+  void* out;   // [B, H, head_dim]
+  float* lse;  // [B, H] or null
+};
+size_t kv_attn_workspace(int64_t B, int group, int kv_heads, int head_dim, int64_t capacity);
+cudaError_t launch_kv_attn(const KvAttnArgs& a, bool fp8, bool bf16, void* ws, cudaStream_t stream);
+
 // linears. fmt: 0 = AWQ int4, 1 = FP8 e4m3. Return an NSQ_* code.
 struct LinearArgs {
   int fmt;

@@ -10,6 +10,8 @@ raise: there is no CPU path.
 
 from __future__ import annotations
 
+import contextlib
+import ctypes
 from typing import Optional
 
 import torch
@@ -289,6 +291,272 @@ def fp8_quantize(weight: torch.Tensor):
     _lib.check(rc, "nsq_fp8_quantize")
     absmax_zero = ws[:4].view(torch.int32)[0] == 0
     return codes.view(torch.float8_e4m3fn), scale, absmax_zero
+
+
+# ---------------------------------------------------------------------------
+# int8 linear (W8A8: int8 codes with one scale per token and output channel)
+# ---------------------------------------------------------------------------
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(*ts, what: str):
+    """Checks that every tensor is on one CUDA device and returns the context
+    in which its kernels launch (that device made current where it is not)."""
+    _require_cuda(*ts, what=what)
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def int8_quantize(x: torch.Tensor):
+    """Rows of x to int8 codes and one scale each (weights per output channel,
+    activations per token): scale = max|row| / 127 (1 if that is 0), codes =
+    rint(row / scale). x: [..., K] float16, bfloat16 or float32. Returns
+    (codes int8 [..., K], scale float32 [...])."""
+    guard = _on_device(x, what="int8_quantize")
+    if x.dtype not in _BIAS_CODES:
+        raise TypeError(f"dtype {x.dtype} not supported (float16 / bfloat16 / float32)")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"int8_quantize needs rows of at least one element, got shape {tuple(x.shape)}")
+    x = x.contiguous()
+    k = x.shape[-1]
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with guard:
+        rc = _lib.load().nsq_int8_quantize(_ptr(x), _BIAS_CODES[x.dtype], x.numel() // k, k, _ptr(codes), _ptr(scale),
+                                           _stream(x))
+    _lib.check(rc, "nsq_int8_quantize")
+    return codes, scale
+
+
+def _int8_weight(weight_int8: torch.Tensor, weight_scale: torch.Tensor):
+    if weight_int8.dtype != torch.int8 or weight_int8.dim() != 2:
+        raise TypeError(f"int8 weight must be int8 [N, K], got {weight_int8.dtype} {tuple(weight_int8.shape)}")
+    n, k = weight_int8.shape
+    if weight_scale.dtype != torch.float32 or weight_scale.numel() != n:
+        raise TypeError(f"weight_scale must be float32 with one value per output channel ({n}), "
+                        f"got {weight_scale.dtype} {tuple(weight_scale.shape)}")
+    return _aligned(weight_int8), weight_scale.contiguous(), n, k
+
+
+def _int8_bias(bias: Optional[torch.Tensor], n: int):
+    if bias is None:
+        return None, _lib.DTYPE_NONE
+    if bias.numel() != n:
+        raise ValueError(f"bias has {bias.numel()} elements, the layer has {n} outputs")
+    return _bias_arg(bias)
+
+
+def int8_linear(x: torch.Tensor, weight_int8: torch.Tensor, weight_scale: torch.Tensor,
+                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """W8A8 linear: x is quantised per token (``int8_quantize``), the codes are
+    multiplied in int32 (exact) and the sums scaled in float32:
+    ``y = (codes @ weight_int8^T) * scale * weight_scale + bias``.
+
+    x: [..., K] float16 or bfloat16; weight_int8 int8 [N, K], weight_scale
+    float32 [N]; returns [..., N] in x's dtype. K must be a multiple of 16, at
+    most 131072.
+    """
+    guard = _on_device(x, weight_int8, weight_scale, bias, what="int8_linear")
+    code = _ACT_CODES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"activation dtype {x.dtype} not supported (float16 / bfloat16)")
+    w, ws, n, k = _int8_weight(weight_int8, weight_scale)
+    if x.shape[-1] != k:
+        raise RuntimeError(f"x has {x.shape[-1]} features, the layer expects {k}")
+    x2 = _aligned(x.reshape(-1, k))
+    m = x2.shape[0]
+    b, bcode = _int8_bias(bias, n)
+    lib = _lib.load()
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    nbytes = lib.nsq_int8_linear_workspace_size(m, k)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    with guard:
+        rc = lib.nsq_int8_linear(x2.data_ptr(), code, m, k, n, w.data_ptr(), ws.data_ptr(), _ptr(b), bcode,
+                                 y.data_ptr(), work.data_ptr(), nbytes, _stream(x))
+    _lib.check(rc, "nsq_int8_linear")
+    return y.reshape(*x.shape[:-1], n)
+
+
+def int8_linear_quantized(codes: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor,
+                          weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                          dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The product of ``int8_linear`` for activations already quantised by
+    ``int8_quantize`` (once, for several layers that read the same x): codes
+    int8 [..., K], scale float32 [...]; returns [..., N] in ``dtype``."""
+    guard = _on_device(codes, scale, weight_int8, weight_scale, bias, what="int8_linear_quantized")
+    if codes.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != codes.shape[:-1]:
+        raise TypeError(f"codes must be int8 [..., K] with a float32 scale [...], got {codes.dtype} "
+                        f"{tuple(codes.shape)} and {scale.dtype} {tuple(scale.shape)}")
+    if dtype not in _ACT_CODES:
+        raise TypeError(f"output dtype {dtype} not supported (float16 / bfloat16)")
+    w, ws, n, k = _int8_weight(weight_int8, weight_scale)
+    if codes.shape[-1] != k:
+        raise RuntimeError(f"codes have {codes.shape[-1]} features, the layer expects {k}")
+    c2 = _aligned(codes.reshape(-1, k))
+    s2 = scale.reshape(-1).contiguous()
+    m = c2.shape[0]
+    b, bcode = _int8_bias(bias, n)
+    y = torch.empty((m, n), dtype=dtype, device=codes.device)
+    with guard:
+        rc = _lib.load().nsq_int8_linear_quantized(c2.data_ptr(), s2.data_ptr(), m, k, n, w.data_ptr(), ws.data_ptr(),
+                                                   _ptr(b), bcode, y.data_ptr(), _ACT_CODES[dtype], _stream(codes))
+    _lib.check(rc, "nsq_int8_linear_quantized")
+    return y.reshape(*codes.shape[:-1], n)
+
+
+# ---------------------------------------------------------------------------
+# 8-bit key/value cache and decode attention over it
+# ---------------------------------------------------------------------------
+
+_KV_CODES = {torch.int8: _lib.KV_INT8, torch.float8_e4m3fn: _lib.KV_FP8}
+
+
+def _strides(t: torch.Tensor, dims: int):
+    """The strides of the first dims dimensions, 0 for those of size 1 (whose stride says nothing)."""
+    return (ctypes.c_int64 * dims)(*[0 if t.shape[i] == 1 else t.stride(i) for i in range(dims)])
+
+
+def _kv_desc(k_cache, v_cache, k_scale, v_scale, what: str) -> "_lib.KvCacheDesc":
+    """Checks the four tensors of a cache and describes them to the library."""
+    code = _KV_CODES.get(k_cache.dtype)
+    if code is None or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"{what}: caches must both be int8 or both float8_e4m3fn, got {k_cache.dtype} "
+                        f"and {v_cache.dtype}")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"{what}: caches must be [pages, page_size, kv_heads, head_dim] of one shape, got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    for s in (k_scale, v_scale):
+        if s.dtype != torch.float32 or s.shape != k_cache.shape[:3]:
+            raise ValueError(f"{what}: scales must be float32 {tuple(k_cache.shape[:3])}, got {s.dtype} "
+                             f"{tuple(s.shape)}")
+    pages, page, heads, dim = k_cache.shape
+    for c in (k_cache, v_cache):
+        if dim > 1 and c.stride(3) != 1:
+            raise ValueError(f"{what}: head_dim must be contiguous in the caches")
+    return _lib.KvCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
+                            page, heads, dim, _strides(k_cache, 3), _strides(v_cache, 3), _strides(k_scale, 3),
+                            _strides(v_scale, 3), code)
+
+
+def _kv_rows(t: torch.Tensor):
+    """[T, heads, head_dim] with 16-byte aligned rows of contiguous head_dim (a copy only where needed)."""
+    if t.stride(2) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and (t.stride(i) % 8 or t.stride(i) < 0)
+                                                    for i in (0, 1)):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _slots_arg(slots: torch.Tensor, what: str) -> torch.Tensor:
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise TypeError(f"{what}: slots must be int64 [T], got {slots.dtype} {tuple(slots.shape)}")
+    return slots.contiguous()
+
+
+def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor, v_scale: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise k and v [T, kv_heads, head_dim] (float16 or bfloat16) into an
+    8-bit cache, in place.
+
+    k_cache, v_cache: int8 or float8_e4m3fn [pages, page_size, kv_heads,
+    head_dim], any strides with head_dim contiguous (token-major or head-major
+    pools); k_scale, v_scale: float32 [pages, page_size, kv_heads]. Token t
+    goes to place ``slots[t] = page * page_size + offset`` (int64); a negative
+    slot is a padded token and is skipped, one past the pool is skipped and
+    recorded in the status word. Slots are distinct: of two tokens with the
+    same slot the stored row is unspecified. Per (token, head) row: scale =
+    max|row| / 127 (int8) or / 448 (float8), 1 where that is 0; codes are the
+    nearest to row / scale. A row with a NaN or an infinity reads back as NaN.
+    """
+    what = "kv_cache_write"
+    guard = _on_device(k, v, k_cache, v_cache, k_scale, v_scale, slots, what=what)
+    if k.dtype not in _ACT_CODES or v.dtype != k.dtype:
+        raise TypeError(f"{what}: k and v must both be float16 or both bfloat16, got {k.dtype} and {v.dtype}")
+    desc = _kv_desc(k_cache, v_cache, k_scale, v_scale, what)
+    slots = _slots_arg(slots, what)
+    shape = (slots.shape[0],) + tuple(k_cache.shape[2:])
+    if tuple(k.shape) != shape or tuple(v.shape) != shape:
+        raise ValueError(f"{what}: k and v must be {shape}, got {tuple(k.shape)} and {tuple(v.shape)}")
+    k, v = _kv_rows(k), _kv_rows(v)
+    with guard:
+        rc = _lib.load().nsq_kv_cache_write(ctypes.byref(desc), k.data_ptr(), v.data_ptr(), _ACT_CODES[k.dtype],
+                                            _strides(k, 2), _strides(v, 2), shape[0], slots.data_ptr(),
+                                            _stream(k_cache))
+    _lib.check(rc, "nsq_kv_cache_write")
+
+
+def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  slots: torch.Tensor, dtype: torch.dtype):
+    """The rows at ``slots`` (int64 [T]) of an 8-bit cache, as (k, v)
+    [T, kv_heads, head_dim] in ``dtype`` (float16 or bfloat16): code * scale,
+    rounded once; zeros where a slot is negative."""
+    what = "kv_cache_read"
+    guard = _on_device(k_cache, v_cache, k_scale, v_scale, slots, what=what)
+    if dtype not in _ACT_CODES:
+        raise TypeError(f"{what}: dtype {dtype} not supported (float16 / bfloat16)")
+    desc = _kv_desc(k_cache, v_cache, k_scale, v_scale, what)
+    slots = _slots_arg(slots, what)
+    k = torch.empty((slots.shape[0],) + tuple(k_cache.shape[2:]), dtype=dtype, device=k_cache.device)
+    v = torch.empty_like(k)
+    with guard:
+        rc = _lib.load().nsq_kv_cache_read(ctypes.byref(desc), slots.data_ptr(), slots.shape[0], k.data_ptr(),
+                                           v.data_ptr(), _ACT_CODES[dtype], _stream(k_cache))
+    _lib.check(rc, "nsq_kv_cache_read")
+    return k, v
+
+
+def kv_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                        softmax_scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of one query token per sequence over its 8-bit cache.
+
+    q: [B, heads, head_dim] float16 or bfloat16, heads a multiple of kv_heads
+    (grouped-query); page_table int32 [B, W]: the pages of each sequence in
+    order; seq_lens int32 [B]: tokens held (0 for a padded row: its output is
+    0, its log-sum-exp -inf). ``softmax_scale`` defaults to head_dim ** -0.5.
+    Returns out [B, heads, head_dim] in q's dtype, with ``return_lse`` also the
+    natural log-sum-exp of the scaled scores, float32 [B, heads]. Entries of
+    page_table past a sequence's last page are never read. A page outside the
+    pool or a length past the table (or below 0) is recorded in the status
+    word: that page's tokens are left out, the length is clamped.
+    """
+    what = "kv_attention_decode"
+    guard = _on_device(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, what=what)
+    code = _ACT_CODES.get(q.dtype)
+    if code is None:
+        raise TypeError(f"{what}: query dtype {q.dtype} not supported (float16 / bfloat16)")
+    desc = _kv_desc(k_cache, v_cache, k_scale, v_scale, what)
+    if q.dim() != 3 or q.shape[2] != desc.head_dim or q.shape[1] == 0 or q.shape[1] % desc.kv_heads:
+        raise ValueError(f"{what}: q must be [B, heads, {desc.head_dim}] with heads a multiple of {desc.kv_heads}, "
+                         f"got {tuple(q.shape)}")
+    b, h, d = q.shape
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b:
+        raise TypeError(f"{what}: page_table must be int32 [{b}, W], got {page_table.dtype} {tuple(page_table.shape)}")
+    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (b,):
+        raise TypeError(f"{what}: seq_lens must be int32 [{b}], got {seq_lens.dtype} {tuple(seq_lens.shape)}")
+    q = _kv_rows(q)
+    width = page_table.shape[1]
+    if page_table.stride(1) != 1 and width > 1:
+        page_table = page_table.contiguous()
+    seq_lens = seq_lens.contiguous()
+    lib = _lib.load()
+    out = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((b, h), dtype=torch.float32, device=q.device) if return_lse else None
+    with guard:
+        nbytes = lib.nsq_kv_attention_workspace_size(b, h, desc.kv_heads, d, desc.page_size, width)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        rc = lib.nsq_kv_attention_decode(ctypes.byref(desc), q.data_ptr(), code, _strides(q, 2), b, h,
+                                         page_table.data_ptr(), page_table.stride(0) if b > 1 else 0, width,
+                                         seq_lens.data_ptr(),
+                                         d ** -0.5 if softmax_scale is None else softmax_scale, out.data_ptr(),
+                                         _ptr(lse), _ptr(work), nbytes, _stream(q))
+    _lib.check(rc, "nsq_kv_attention_decode")
+    return (out, lse) if return_lse else out
 
 
 # ---------------------------------------------------------------------------
