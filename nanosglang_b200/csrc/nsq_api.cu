@@ -99,6 +99,24 @@ bool test_withhold() { return g_withhold.load(std::memory_order_relaxed) != 0; }
 
 int device_ready() { return check_device(); }
 
+cudaError_t allow_dynamic_smem(const void* kernel, int bytes) {
+  struct Entry {
+    const void* kernel;
+    int device;
+  };
+  static std::mutex mu;
+  static Entry known[256];
+  static int count = 0;
+  const int d = current_device();
+  std::lock_guard<std::mutex> lk(mu);
+  for (int i = 0; i < count; ++i) {
+    if (known[i].kernel == kernel && known[i].device == d) return cudaSuccess;
+  }
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && count < 256) known[count++] = Entry{kernel, d};
+  return e;
+}
+
 namespace {
 // Per-thread cache of encoded tensor maps: an eager forward encodes the same
 // maps (same weight, same x buffer from the caching allocator) call after
@@ -624,6 +642,10 @@ static int int8_check(int64_t M, int64_t K, int64_t N, const void* x, const int8
   return check_device();
 }
 
+static int int8_product(const Int8Args& a, cudaStream_t stream) {
+  return a.M <= 64 ? run_int8_rows(a, stream) : run_int8_gemm(a, stream);
+}
+
 int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N, const int8_t* weight_int8,
                     const float* weight_scale, const void* bias, int bias_dtype, void* y, void* workspace,
                     size_t workspace_bytes, void* stream) {
@@ -635,9 +657,9 @@ int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N,
   float* scale = reinterpret_cast<float*>(codes + int8_codes_bytes(M, K));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (launch_int8_quantize(x, x_dtype, M, K, codes, scale, s) != cudaSuccess) return NSQ_ECUDA;
-  return run_int8_rows(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
-                                x_dtype == NSQ_DTYPE_BF16, y, true},
-                       s);
+  return int8_product(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
+                               x_dtype == NSQ_DTYPE_BF16, y, true},
+                      s);
 }
 
 int nsq_int8_linear_quantized(const int8_t* codes, const float* scale, int64_t M, int64_t K, int64_t N,
@@ -646,9 +668,9 @@ int nsq_int8_linear_quantized(const int8_t* codes, const float* scale, int64_t M
   int rc = int8_check(M, K, N, codes, weight_int8, weight_scale, bias, bias_dtype, y, y_dtype);
   if (rc != NSQ_OK || M == 0) return rc;
   if (!scale) return NSQ_EINVAL;
-  return run_int8_rows(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
-                                y_dtype == NSQ_DTYPE_BF16, y, false},
-                       static_cast<cudaStream_t>(stream));
+  return int8_product(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
+                               y_dtype == NSQ_DTYPE_BF16, y, false},
+                      static_cast<cudaStream_t>(stream));
 }
 
 // Checks a cache descriptor; on NSQ_OK `out` is what the kernels take.

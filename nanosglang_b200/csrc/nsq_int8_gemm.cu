@@ -1,0 +1,507 @@
+// int8 linear, tensor-core path for more than a few tokens:
+//   y^T = (wc . xc^T) * ws * xs + bias
+// with tcgen05.mma kind::i8 (s8 x s8 -> s32, exact), weight rows as the 128
+// (one CTA) or 256 (CTA pair) rows, tokens as the columns, both operands
+// K-major 128-byte-swizzled tiles that TMA brings from global memory.
+//
+// What bounds it: at 256 x 256 x 128 per step a pair reads 64 KB from L2 for
+// 512 cycles of int8 tensor work, so the L2 path and the tensor pipe are near
+// balance; hence the largest tile whose accumulator still double-buffers in
+// tensor memory (2 x 256 columns), and a tile order in which the tiles that
+// run at the same time share their weight rows and tokens (8 token tiles by as
+// many weight tiles as it takes).
+//
+// Warp roles (per CTA, 320 threads): 0 TMA producer, 1 MMA issuer (of a pair,
+// the even CTA's), 2..9 epilogue. A stage holds two 128-column k-blocks, so a
+// barrier round covers 8 MMAs. The epilogue of one tile runs under the MMAs of
+// the next: s32 -> fp32, scales, bias, one rounding, a staged [token][feature]
+// tile, TMA store (plain stores where N % 8 != 0 leaves no 16-byte row pitch).
+// Every wait is bounded. No TMA multicast.
+#include <atomic>
+
+#include "nsq_common.cuh"
+#include "nsq_internal.h"
+
+namespace nsq {
+
+namespace {
+
+constexpr int kRows = 128;  // weight rows per CTA
+constexpr int kBK = 128;    // columns per k-block: one 128-byte swizzled row
+constexpr int kKps = 2;     // k-blocks per stage
+constexpr int kEpi = 8;     // epilogue warps
+constexpr int kGemmThreads = 32 * (2 + kEpi);
+constexpr int kGroup = 8;   // token tiles that share a pass over the weight
+
+// CG CTAs per tile, TOK tokens per tile.
+template <int CG, int TOK>
+struct GemmShape {
+  static constexpr int kXRows = TOK / CG;  // tokens staged per CTA
+  static constexpr int kWBytes = kRows * kBK, kXBytes = kXRows * kBK;
+  static constexpr int kStage = kKps * (kWBytes + kXBytes);
+  static constexpr int kTokRound = TOK < 128 ? TOK : 128;  // tokens of a staged y tile
+  static constexpr int kYHalf = kTokRound * 64 * 2;        // 64 features
+  static constexpr int NS = (226 * 1024 - 2 * kYHalf - 1024) / kStage < 6 ? (226 * 1024 - 2 * kYHalf - 1024) / kStage : 6;
+  static constexpr int kY = NS * kStage;
+  static constexpr int kBar = kY + 2 * kYHalf;
+  // full[NS], done[NS], full_acc[2], empty_acc[2], drain
+  static constexpr int kBars = 2 * NS + 5;
+  static constexpr int kTmemSlot = kBar + kBars * 8;
+  static constexpr int kAbort = kTmemSlot + 4;
+  static constexpr int kAlloc = kAbort + 4 + 1024;
+  static constexpr uint32_t kTmemCols = 2 * TOK;
+  static_assert(kAlloc <= 227 * 1024 && NS >= 3, "shared memory per CTA");
+  static_assert(kStage % 1024 == 0 && kYHalf % 1024 == 0, "swizzled tiles are 1 KB aligned");
+};
+
+struct GemmParams {
+  const float* xscale;
+  const float* wscale;
+  const void* bias;
+  void* y;
+  DevStatus* status;
+  int M, K, N, bias_dtype;
+  int num_w, num_t, num_kb, num_st;
+  int pdl_x;  // x and its scales come from the kernel ahead on the stream
+};
+
+__device__ __forceinline__ void gemm_unit(const GemmParams& p, int u, int& wt, int& tt) {
+  const int per = kGroup * p.num_w;
+  const int grp = u / per, r = u - grp * per;
+  const int g0 = grp * kGroup;
+  const int gs = p.num_t - g0 < kGroup ? p.num_t - g0 : kGroup;
+  wt = r / gs;
+  tt = g0 + r - wt * gs;
+}
+
+// The MMA's N for token tile tt: all tokens, or the rest rounded up to 32
+// (rows past M read as zero).
+template <int TOK>
+__device__ __forceinline__ int gemm_n(int M, int tt) {
+  const int rem = M - tt * TOK;
+  return rem >= TOK ? TOK : ((rem + 31) & ~31);
+}
+
+// kind::i8: D s32 (2), A and B s8 (1), both K-major
+__host__ __device__ constexpr uint32_t idesc_s8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// The MMAs of one stage, issued back to back by the elected lane of a
+// converged warp: KB k-blocks of four K = 32 steps (+32 bytes = +2 descriptor
+// units a step). Only the first takes `accumulate`.
+template <int CG, int KB>
+__device__ __forceinline__ void umma_i8_elect(uint32_t d, uint64_t a0, uint64_t b0, uint64_t a1, uint64_t b1,
+                                              uint32_t idesc, uint32_t accumulate) {
+#define NSQ_I8_PRE "{\n\t.reg .pred e, p, t;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\t"
+#define NSQ_I8_4(M) M "[%0], %1, %5, %9, p;\n\t" M "[%0], %2, %6, %9, t;\n\t" M "[%0], %3, %7, %9, t;\n\t" M "[%0], %4, %8, %9, t;\n\t"
+#define NSQ_I8_GO(M, acc)                                                                                          \
+  asm volatile(NSQ_I8_PRE "setp.ne.b32 p, %10, 0;\n\tsetp.eq.b32 t, %10, %10;\n\t" NSQ_I8_4(M) "}" ::"r"(d), "l"(a),    \
+               "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc), "r"(acc) \
+               : "memory")
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+    const uint64_t a = i == 0 ? a0 : a1, b = i == 0 ? b0 : b1;
+    const uint32_t acc = i == 0 ? accumulate : 1u;
+    if constexpr (CG == 1) {
+      NSQ_I8_GO("@e tcgen05.mma.cta_group::1.kind::i8 ", acc);
+    } else {
+      NSQ_I8_GO("@e tcgen05.mma.cta_group::2.kind::i8 ", acc);
+    }
+  }
+#undef NSQ_I8_PRE
+#undef NSQ_I8_4
+#undef NSQ_I8_GO
+}
+
+// TMA load whose bytes are counted on a barrier of the pair's even CTA.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int c0,
+                                                 int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return (uint32_t)float_to_elem<BF16>(a) | ((uint32_t)float_to_elem<BF16>(b) << 16);
+}
+
+template <int CG, int TOK, bool BF16, bool STAGED>
+__global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap xmap,
+                                                                    const __grid_constant__ CUtensorMap wmap,
+                                                                    const __grid_constant__ CUtensorMap ymap,
+                                                                    const GemmParams p) {
+  using S = GemmShape<CG, TOK>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar);  // a stage's tiles landed (pair: both CTAs', even CTA's barrier)
+  uint64_t* done = full + S::NS;                                 // its MMAs finished (both CTAs)
+  uint64_t* full_acc = done + S::NS;                             // an accumulator is complete (both CTAs)
+  uint64_t* empty_acc = full_acc + 2;                            // and read out by every epilogue warp (even CTA)
+  uint64_t* drain = empty_acc + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kTmemSlot);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kAbort);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  const int cid = blockIdx.x / CG, ncl = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < S::NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full_acc[i], 1);
+      mbar_init(&empty_acc[i], CG * kEpi);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      tmem_alloc_pair(tmem_slot, S::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, S::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (CG == 2) {
+    cluster_sync_all();
+  } else {
+    __syncthreads();
+  }
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int units = p.num_w * p.num_t;
+  bool ok = true;
+  auto commit = [&](uint64_t* bar) {
+    if constexpr (CG == 2) {
+      tc_commit_pair_mc_elect(bar, 0x3);
+    } else {
+      tc_commit_elect(bar);
+    }
+  };
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      tma_prefetch_desc(&xmap);
+      tma_prefetch_desc(&wmap);
+      const uint32_t full0 = CG == 2 ? dsmem_map(smem_u32(&full[0]), 0) : 0;
+      auto load = [&](bool is_x, int row, int st, int s) {
+        const int kb0 = st * kKps;
+        const int nk = p.num_kb - kb0 < kKps ? p.num_kb - kb0 : kKps;
+        for (int i = 0; i < nk; ++i) {
+          uint8_t* dst = smem + s * S::kStage + (is_x ? kKps * S::kWBytes + i * S::kXBytes : i * S::kWBytes);
+          const CUtensorMap* map = is_x ? &xmap : &wmap;
+          if constexpr (CG == 2) {
+            tma_load_2d_pair(dst, map, full0 + s * 8, (kb0 + i) * kBK, row);
+          } else {
+            tma_load_2d(dst, map, &full[s], (kb0 + i) * kBK, row);
+          }
+        }
+      };
+      // the even CTA arms the barrier for the bytes of both
+      auto arm = [&](int st, int s) {
+        const int nk = p.num_kb - st * kKps < kKps ? p.num_kb - st * kKps : kKps;
+        if (leader) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * nk) * (S::kWBytes + S::kXBytes));
+      };
+      auto w_row = [&](int wt) { return (wt * CG + (int)rank) * kRows; };
+      // the weights do not depend on the kernel ahead: the first stages' are
+      // on their way before it is waited for
+      int pre = 0;
+      for (int u = cid; u < units && pre < S::NS; u += ncl) {
+        int wt, tt;
+        gemm_unit(p, u, wt, tt);
+        for (int st = 0; st < p.num_st && pre < S::NS; ++st, ++pre) {
+          arm(st, pre);
+          load(false, w_row(wt), st, pre);
+        }
+      }
+      if (p.pdl_x) pdl_wait_prior_grids();
+      int it = 0;
+      for (int u = cid; u < units && ok; u += ncl) {
+        int wt, tt;
+        gemm_unit(p, u, wt, tt);
+        const int x_row = tt * TOK + (int)rank * (gemm_n<TOK>(p.M, tt) / CG);
+        for (int st = 0; st < p.num_st; ++st, ++it) {
+          const int s = it % S::NS;
+          if (it >= pre) {
+            if (!(ok = mbar_wait(&done[s], ((it / S::NS) & 1) ^ 1, p.status, 210, abort_flag))) break;
+            arm(st, s);
+            load(false, w_row(wt), st, s);
+          }
+          load(true, x_row, st, s);
+        }
+      }
+      if (!ok && leader) {  // let copies in flight land before the CTA (of a pair, both) can exit
+        const int last = it > pre ? it : pre;
+        for (int j = last > S::NS ? last - S::NS : 0; j < last; ++j) {
+          mbar_wait(&full[j % S::NS], (j / S::NS) & 1, nullptr, 0, nullptr);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (leader) {
+      int it = 0, tc = 0;
+      for (int u = cid; u < units && ok; u += ncl, ++tc) {
+        int wt, tt;
+        gemm_unit(p, u, wt, tt);
+        const uint32_t idesc = idesc_s8(CG * kRows, gemm_n<TOK>(p.M, tt));
+        const int buf = tc & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty_acc[buf], ((tc >> 1) & 1) ^ 1, p.status, 211, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        for (int st = 0; st < p.num_st; ++st, ++it) {
+          const int s = it % S::NS;
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / S::NS) & 1, p.status, 212, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t base = smem_u32(smem + s * S::kStage);
+          const uint64_t a0 = sw128_kmajor_desc(base), a1 = sw128_kmajor_desc(base + S::kWBytes);
+          const uint64_t b0 = sw128_kmajor_desc(base + kKps * S::kWBytes);
+          const uint64_t b1 = sw128_kmajor_desc(base + kKps * S::kWBytes + S::kXBytes);
+          const uint32_t d = tmem + buf * TOK;
+          if (p.num_kb - st * kKps >= 2) {
+            umma_i8_elect<CG, 2>(d, a0, b0, a1, b1, idesc, st > 0);
+          } else {
+            umma_i8_elect<CG, 1>(d, a0, b0, a1, b1, idesc, st > 0);
+          }
+          commit(&done[s]);
+        }
+        if (!ok) break;
+        commit(&full_acc[buf]);
+      }
+      // every MMA issued has finished before tensor memory is released
+      commit(drain);
+      mbar_wait(drain, 0, nullptr, 0, nullptr);
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    if (p.pdl_x) pdl_wait_prior_grids();  // the scales of x, and y's buffer
+    const int sub = warp & 3;             // tensor-memory sub-partition: 32 weight rows
+    const int half = (warp - 2) >> 2;     // half of a round's tokens
+    const int etid = threadIdx.x - 64;
+    const int g = lane >> 2, t = lane & 3;
+    const bool has_bias = p.bias_dtype != NSQ_DTYPE_NONE;
+    const uint32_t empty0 = CG == 2 ? dsmem_map(smem_u32(&empty_acc[0]), 0) : 0;
+    const uint32_t ystage = smem_u32(smem + S::kY + (sub >> 1) * S::kYHalf);
+    const uint32_t ychunk = (uint32_t)((sub & 1) * 4 + (lane >> 3));
+    int tc = 0;
+    for (int u = cid; u < units && ok; u += ncl, ++tc) {
+      int wt, tt;
+      gemm_unit(p, u, wt, tt);
+      const int buf = tc & 1;
+      const int f0 = (wt * CG + (int)rank) * kRows;  // first feature of this CTA
+      // fragment rows of this lane: features sub * 32 + 8 q + g
+      float wsc[4], bf[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = f0 + sub * 32 + 8 * q + g;
+        wsc[q] = n < p.N ? __ldg(p.wscale + n) : 0.f;
+        bf[q] = has_bias && n < p.N ? load_bias(p.bias, p.bias_dtype, n) : 0.f;
+      }
+      ok = mbar_wait(&full_acc[buf], (tc >> 1) & 1, p.status, 213, abort_flag);
+      if (!named_bar_all(1, kEpi * 32, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(sub * 32) << 16) + buf * TOK;
+      constexpr int kWarpTok = S::kTokRound / 2;
+#pragma unroll 1
+      for (int rd = 0; rd < TOK / S::kTokRound; ++rd) {
+        if constexpr (STAGED) {
+          if (etid == 0) bulk_wait_group_read<0>();  // the staged tile's last store has read it
+          named_bar_sync(1, kEpi * 32);
+        }
+        const int col0 = rd * S::kTokRound + half * kWarpTok;
+#pragma unroll 1
+        for (int c = 0; c < kWarpTok && tt * TOK + col0 + c < p.M; c += 32) {
+          uint32_t r0[16], r1[16];
+          tmem_ld_16x256b_x4(acc + col0 + c, r0);
+          tmem_ld_16x256b_x4(acc + (16u << 16) + col0 + c, r1);
+          float xs[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int m = tt * TOK + col0 + c + 8 * (j >> 1) + 2 * t + (j & 1);
+            xs[j] = m < p.M ? p.xscale[m] : 0.f;
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // tokens 8j + 2t, + 1 of features g, g + 8, g + 16, g + 24
+            float v[4][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              v[0][e] = (float)(int)r0[4 * j + e];
+              v[1][e] = (float)(int)r0[4 * j + 2 + e];
+              v[2][e] = (float)(int)r1[4 * j + e];
+              v[3][e] = (float)(int)r1[4 * j + 2 + e];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                v[q][e] = v[q][e] * xs[2 * j + e] * wsc[q];
+                if (has_bias) v[q][e] += bf[q];
+              }
+            }
+            if constexpr (STAGED) {
+              const uint32_t row = (uint32_t)(half * kWarpTok + c + 8 * j + (lane & 7));
+              stmatrix_x4_trans(ystage + row * 128 + ((ychunk ^ (row & 7)) << 4), pack2<BF16>(v[0][0], v[0][1]),
+                                pack2<BF16>(v[1][0], v[1][1]), pack2<BF16>(v[2][0], v[2][1]),
+                                pack2<BF16>(v[3][0], v[3][1]));
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int m = tt * TOK + col0 + c + 8 * j + 2 * t + e, n = f0 + sub * 32 + 8 * q + g;
+                  if (m < p.M && n < p.N) {
+                    static_cast<uint16_t*>(p.y)[(int64_t)m * p.N + n] = float_to_elem<BF16>(v[q][e]);
+                  }
+                }
+              }
+            }
+          }
+        }
+        if (rd == TOK / S::kTokRound - 1) {  // the accumulator is read out
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 2) {
+              mbar_arrive_cluster(empty0 + buf * 8);
+            } else {
+              mbar_arrive(&empty_acc[buf]);
+            }
+          }
+        }
+        if constexpr (STAGED) {
+          fence_proxy_async_smem();
+          named_bar_sync(1, kEpi * 32);
+          if (etid == 0) {
+            for (int h = 0; h < 2; ++h) {
+              const int f = f0 + h * 64, m = tt * TOK + rd * S::kTokRound;
+              if (f < p.N && m < p.M) tma_store_2d(&ymap, smem + S::kY + h * S::kYHalf, f, m);
+            }
+            bulk_commit_group();
+          }
+        }
+      }
+    }
+    if (STAGED && etid == 0) bulk_wait_group<0>();
+  }
+
+  __syncthreads();
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CG == 2) {
+      tmem_dealloc_pair(tmem, S::kTmemCols);
+    } else {
+      tmem_dealloc(tmem, S::kTmemCols);
+    }
+  }
+}
+
+template <int CG, int TOK, bool BF16, bool STAGED>
+cudaError_t launch_gemm(const Int8Args& a, const CUtensorMap& xmap, const CUtensorMap& wmap, const CUtensorMap& ymap,
+                        const GemmParams& p, cudaStream_t stream) {
+  using S = GemmShape<CG, TOK>;
+  auto kern = int8_gemm_kernel<CG, TOK, BF16, STAGED>;
+  cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kern), S::kAlloc);
+  if (e != cudaSuccess) return e;
+  const int64_t units = (int64_t)p.num_w * p.num_t, most = num_sms() / CG;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(CG * (units < most ? units : most)));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = S::kAlloc;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (CG == 2) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = 2;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (p.pdl_x) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kern, xmap, wmap, ymap, p);
+}
+
+template <int CG, int TOK>
+int run_gemm(const Int8Args& a, cudaStream_t stream) {
+  using S = GemmShape<CG, TOK>;
+  const bool staged = a.N % 8 == 0;
+  CUtensorMap xmap, wmap, ymap;
+  if (encode_tensor_map_2d(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<int8_t*>(a.x), a.K, a.M, a.K, kBK,
+                           S::kXRows, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS ||
+      encode_tensor_map_2d(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<int8_t*>(a.w), a.K, a.N, a.K, kBK, kRows,
+                           CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS) {
+    return NSQ_ECUDA;
+  }
+  ymap = xmap;
+  if (staged && encode_tensor_map_2d(&ymap,
+                                     a.y_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.y,
+                                     a.N, a.M, (uint64_t)a.N * 2, 64, S::kTokRound,
+                                     CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS) {
+    return NSQ_ECUDA;
+  }
+  GemmParams p{};
+  p.xscale = a.xscale;
+  p.wscale = a.wscale;
+  p.bias = a.bias;
+  p.bias_dtype = a.bias ? a.bias_dtype : NSQ_DTYPE_NONE;
+  p.y = a.y;
+  p.status = device_status_ptr();
+  p.M = a.M;
+  p.K = a.K;
+  p.N = a.N;
+  p.num_w = (a.N + CG * kRows - 1) / (CG * kRows);
+  p.num_t = (a.M + TOK - 1) / TOK;
+  p.num_kb = (a.K + kBK - 1) / kBK;
+  p.num_st = (p.num_kb + kKps - 1) / kKps;
+  p.pdl_x = a.after_quantize || pdl_enabled();
+  if ((int64_t)p.num_w * p.num_t > 0x3FFFFFFF) return NSQ_ENOTSUP;
+  cudaError_t e;
+  if (staged) {
+    e = a.y_bf16 ? launch_gemm<CG, TOK, true, true>(a, xmap, wmap, ymap, p, stream)
+                 : launch_gemm<CG, TOK, false, true>(a, xmap, wmap, ymap, p, stream);
+  } else {
+    e = a.y_bf16 ? launch_gemm<CG, TOK, true, false>(a, xmap, wmap, ymap, p, stream)
+                 : launch_gemm<CG, TOK, false, false>(a, xmap, wmap, ymap, p, stream);
+  }
+  return e == cudaSuccess ? NSQ_OK : NSQ_ECUDA;
+}
+
+}  // namespace
+
+// Tile choice: waves of tiles times a tile's time in cycles, per k-block and
+// fixed (fill, epilogue of the last tile).
+int run_int8_gemm(const Int8Args& a, cudaStream_t stream) {
+  const int64_t sms = num_sms(), kb = (a.K + kBK - 1) / kBK;
+  auto cost = [&](int cg, int tok, int per_kb, int fixed) {
+    const int64_t tiles = (int64_t)((a.N + cg * kRows - 1) / (cg * kRows)) * ((a.M + tok - 1) / tok);
+    const int64_t at_once = sms / cg;
+    return (tiles + at_once - 1) / at_once * (kb * per_kb) + fixed;
+  };
+  const int64_t c2 = cost(2, 256, 640, 6000), c1 = cost(1, 128, 320, 4000), ch = cost(1, 64, 200, 3000);
+  if (c2 <= c1 && c2 <= ch) return run_gemm<2, 256>(a, stream);
+  return c1 <= ch ? run_gemm<1, 128>(a, stream) : run_gemm<1, 64>(a, stream);
+}
+
+}  // namespace nsq

@@ -14,6 +14,8 @@ int num_sms();                  // SM count of the current device (cached per de
 int device_ready();             // NSQ_OK if the current device is sm_100, else an NSQ_E* code
 DevStatus* device_status_ptr(); // device address of this device's status word (lazily set up)
 bool pdl_enabled();
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device (set once per kernel and device).
+cudaError_t allow_dynamic_smem(const void* kernel, int bytes);
 bool test_withhold();  // failure-path test hook: the multi-wave decode kernel skips one weight load
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (libnsq does
@@ -57,7 +59,8 @@ struct Int8Args {
   void* y;  // [M, N]
   bool after_quantize;  // the kernel ahead on the stream is launch_int8_quantize's, writing x and xscale
 };
-int run_int8_rows(const Int8Args& a, cudaStream_t stream);
+int run_int8_rows(const Int8Args& a, cudaStream_t stream);  // mma.sync, weight rows streamed: decode batches
+int run_int8_gemm(const Int8Args& a, cudaStream_t stream);  // tcgen05 tiles: larger ones
 
 // 8-bit key/value cache. Strides in elements: page, token, head; head_dim contiguous.
 struct KvCache {
