@@ -123,13 +123,14 @@ namespace {
 // call. The key is every input of the encoding, so a hit is exactly what the
 // driver would return.
 struct MapKey {
-  uint64_t base, dim[3], stride[2];
-  uint32_t box[3];
+  uint64_t base, dim[4], stride[3];
+  uint32_t box[4];
   int rank, dtype, swizzle;
   bool operator==(const MapKey& o) const {
-    return base == o.base && dim[0] == o.dim[0] && dim[1] == o.dim[1] && dim[2] == o.dim[2] &&
-           stride[0] == o.stride[0] && stride[1] == o.stride[1] && box[0] == o.box[0] && box[1] == o.box[1] &&
-           box[2] == o.box[2] && rank == o.rank && dtype == o.dtype && swizzle == o.swizzle;
+    return base == o.base && dim[0] == o.dim[0] && dim[1] == o.dim[1] && dim[2] == o.dim[2] && dim[3] == o.dim[3] &&
+           stride[0] == o.stride[0] && stride[1] == o.stride[1] && stride[2] == o.stride[2] && box[0] == o.box[0] &&
+           box[1] == o.box[1] && box[2] == o.box[2] && box[3] == o.box[3] && rank == o.rank && dtype == o.dtype &&
+           swizzle == o.swizzle;
   }
 };
 struct MapEntry {
@@ -151,10 +152,11 @@ inline uint32_t map_slot(const MapKey& k) {
 }  // namespace
 
 static CUresult encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, void* base, int rank,
-                                  const uint64_t (&dim)[3], const uint64_t (&stride)[2], const uint32_t (&boxd)[3],
+                                  const uint64_t (&dim)[4], const uint64_t (&stride)[3], const uint32_t (&boxd)[4],
                                   CUtensorMapSwizzle swizzle) {
-  const MapKey key{reinterpret_cast<uint64_t>(base), {dim[0], dim[1], dim[2]}, {stride[0], stride[1]},
-                   {boxd[0], boxd[1], boxd[2]}, rank, (int)dtype, (int)swizzle};
+  const MapKey key{reinterpret_cast<uint64_t>(base), {dim[0], dim[1], dim[2], dim[3]},
+                   {stride[0], stride[1], stride[2]}, {boxd[0], boxd[1], boxd[2], boxd[3]}, rank, (int)dtype,
+                   (int)swizzle};
   MapEntry& slot = t_map_cache[map_slot(key)];
   if (slot.valid && slot.key == key) {
     *map = slot.map;
@@ -176,10 +178,10 @@ static CUresult encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, v
       g_encode.store(encode, std::memory_order_release);
     }
   }
-  const cuuint64_t dims[3] = {dim[0], dim[1], dim[2]};
-  const cuuint64_t strides[2] = {stride[0], stride[1]};
-  const cuuint32_t box[3] = {boxd[0], boxd[1], boxd[2]};
-  const cuuint32_t estr[3] = {1, 1, 1};
+  const cuuint64_t dims[4] = {dim[0], dim[1], dim[2], dim[3]};
+  const cuuint64_t strides[3] = {stride[0], stride[1], stride[2]};
+  const cuuint32_t box[4] = {boxd[0], boxd[1], boxd[2], boxd[3]};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, dtype, (cuuint32_t)rank, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) {
@@ -193,14 +195,20 @@ static CUresult encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, v
 CUresult encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, void* base,
                               uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                               uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
-  return encode_tensor_map(map, dtype, base, 2, {inner, outer, 0}, {row_stride_bytes, 0}, {box_inner, box_outer, 0},
-                           swizzle);
+  return encode_tensor_map(map, dtype, base, 2, {inner, outer, 0, 0}, {row_stride_bytes, 0, 0},
+                           {box_inner, box_outer, 0, 0}, swizzle);
 }
 
 CUresult encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, void* base, uint64_t d0, uint64_t d1,
                               uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1,
                               uint32_t b2, CUtensorMapSwizzle swizzle) {
-  return encode_tensor_map(map, dtype, base, 3, {d0, d1, d2}, {stride1_bytes, stride2_bytes}, {b0, b1, b2}, swizzle);
+  return encode_tensor_map(map, dtype, base, 3, {d0, d1, d2, 0}, {stride1_bytes, stride2_bytes, 0}, {b0, b1, b2, 0},
+                           swizzle);
+}
+
+CUresult encode_tensor_map_4d(CUtensorMap* map, CUtensorMapDataType dtype, void* base, const uint64_t (&dims)[4],
+                              const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
+  return encode_tensor_map(map, dtype, base, 4, dims, strides, box, swizzle);
 }
 
 }  // namespace nsq

@@ -29,6 +29,10 @@ CUresult encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, void*
                               uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1,
                               uint32_t b2, CUtensorMapSwizzle swizzle);
 
+// Rank 4: as above with three byte strides.
+CUresult encode_tensor_map_4d(CUtensorMap* map, CUtensorMapDataType dtype, void* base, const uint64_t (&dims)[4],
+                              const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle);
+
 // elementwise
 cudaError_t launch_awq_dequant(const int32_t* qweight, const uint16_t* scales,
                                const uint16_t* zeros, uint16_t* out, int64_t N, int64_t K,

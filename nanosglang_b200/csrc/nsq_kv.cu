@@ -40,6 +40,7 @@ struct KvRead {
 struct KvAttn : KvAttnArgs {
   int group, head_blocks;
   FastDiv page_div;
+  bool k_swap, v_swap;  // the tensor map has head before token
   float scale_log2;
   float* partial;
   int4* meta;
@@ -180,28 +181,31 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 // One query token per sequence: out[h] = sum_t p[t] v[t] / sum_t p[t],
 // p[t] = exp2(s[t] - m), s[t] = scale * log2(e) * q . k[t], m the running
 // maximum. Bound by reading the codes once; so
-//   * a warp takes 16 tokens at a time and reads their codes from global
-//     memory straight into the registers that are the A operands of
-//     mma.m16n8k16 (rows = tokens for q . k, rows = dims for p . v), the query
-//     heads that share the kv head being the 8 columns. The order of the k
-//     index within an MMA is free, so 16 consecutive bytes per lane are used
-//     as they come; no shared memory, no barriers, in the loop;
-//   * codes become fp16 exactly; q is scaled per head by a power of two into
-//     fp16's range, exact for fp16 and for every bf16 within 2^-14 of the
-//     head's largest. Scores, maxima and sums are fp32;
+//   * each warp keeps its own ring of 32-token stages in shared memory, filled
+//     ahead by TMA (one box per 16 tokens of a page and head) or, where pages
+//     are not multiples of 16 tokens, by 16-byte asynchronous copies, and
+//     works through them alone: no block barrier in the loop;
+//   * mma.m16n8k16 with 16 tokens as rows for q . k and 16 dims as rows for
+//     p . v; the query heads that share the kv head are the 8 columns. The
+//     codes are read in the swizzled tile without bank conflicts (ldmatrix for
+//     k, 16-byte reads for v) and become fp16 in registers, exactly;
+//   * q is scaled per head by a power of two into fp16's range, exact for fp16
+//     and for every bf16 within 2^-14 of the head's largest. Scores, maxima
+//     and sums are fp32;
 //   * the scale of v is folded into the exponent: the fp16 weights of p . v
 //     are exp2(s + log2(vs) - m'), with a maximum m' of their own, so that
 //     they use fp16's range whatever the scales are (half-ulp 2^-12 each); the
 //     denominator is summed in fp32 from unrounded terms. At the end the
 //     accumulator is multiplied by exp2(m' - m);
-//   * work is cut into units of 64 tokens of one (sequence, kv head) and dealt
+//   * work is cut into units of 128 tokens of one (sequence, kv head) and dealt
 //     evenly to the CTAs on the device, from seq_lens: long and ragged batches
 //     fill the machine alike. A CTA's range covers whole items and at most two
 //     cut ones; those go to the workspace as fp32 partials, and a second small
 //     kernel joins them in order.
 
 constexpr int kAttnWarps = 4;
-constexpr int kUnit = 16 * kAttnWarps;
+constexpr int kTile = 32;  // tokens of a stage
+constexpr int kUnit = kTile * kAttnWarps;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -250,17 +254,40 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
-__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
+}
+// Asynchronous copies to shared memory; with bytes = 0 the place is zeroed and nothing is read.
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// One arrival on the barrier when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
 }
 
 // Tokens a sequence holds: seq_lens clamped to what its page-table row can name.
@@ -274,29 +301,67 @@ __device__ __forceinline__ int seq_tokens(const KvAttn& p, int b, bool tell) {
 }
 __device__ __forceinline__ int item_units(int n) { return n == 0 ? 1 : (n + kUnit - 1) / kUnit; }
 
-// One warp's 16 tokens. k[r]: row r = token g + 8r, 16-byte chunks of 64 dims;
-// v[i]: tokens 2t, 2t+1, 2t+8, 2t+9, dims [g * DP / 8, + DP / 8).
-template <int DP>
-struct KvTile {
-  uint4 k[2][DP / 64];
-  uint32_t v[4][DP / 32];
-  float ks[2], vs[2];
-  bool in[2];  // token g + 8r is held
+// A warp's ring: stages of 32 tokens, k then v, each as two 16-token tiles of
+// HALVES x 16 rows of RB bytes (swizzled in RB-byte rows as TMA does), and the
+// 64 scales. The partial results of the block's warps take the ring's place
+// when a segment is done.
+constexpr int kScaleBytes = 272;
+template <int DP, int NT>
+struct AttnShape {
+  static constexpr int RB = DP < 128 ? DP : 128;  // bytes of a tile row
+  static constexpr int HALVES = DP / RB;
+  static constexpr int kTileBytes = 16 * DP;
+  static constexpr int kStage = 4 * kTileBytes;
+  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr int HEADS = 8 * NT;
+  static constexpr int kRing = kAttnWarps * kStages * kStage;
+  static constexpr int kJoinBytes = kAttnWarps * HEADS * (DP + 3) * 4;
+  static constexpr int kScale = kRing > kJoinBytes ? kRing : kJoinBytes;  // [warp][stage] 64 fp32 scales and a mask of tokens
+  static constexpr int kBar = kScale + kAttnWarps * kStages * kScaleBytes;
+  static constexpr int kAlloc = kBar + kAttnWarps * kStages * 8 + 1024;
+  static constexpr int kCtas = 227 * 1024 / (kAlloc + 1024) < 4 ? 227 * 1024 / (kAlloc + 1024) : 4;
+  static constexpr int kPerSm = DP * NT <= 128 ? (kCtas < 3 ? kCtas : 3) : (kCtas < 2 ? kCtas : 2);
 };
 
-template <int DP, int NT, bool FP8, bool BF16, bool PAGE16>
-__global__ void __launch_bounds__(kAttnWarps * 32, DP * NT <= 128 ? 3 : 2) kv_attn_kernel(const KvAttn p) {
-  constexpr int KC = DP / 64;      // 16-byte chunks of a K row per lane
-  constexpr int VW = DP / 32;      // words of a V row per lane
+// Place of 16-byte chunk c of tile row r
+template <int RB>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  return (uint32_t)(r * RB + ((c ^ (RB == 128 ? (r & 7) : ((r >> 1) & 3))) << 4));
+}
+// Token of MMA row i (of 16): the identity, or for 64-byte rows bits 0 and 1
+// exchanged, so that the v reads of a warp fall into different banks.
+template <int RB>
+__device__ __forceinline__ int row_token(int i) {
+  return RB == 128 ? i : (i & 12) | ((i & 1) << 1) | ((i >> 1) & 1);
+}
+
+template <int DP, int NT, bool FP8, bool BF16, bool TMA>
+__global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv_attn_kernel(
+    const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const KvAttn p) {
+  using S = AttnShape<DP, NT>;
+  constexpr int RB = S::RB, HALVES = S::HALVES;
+  constexpr int KCH = RB / 16;     // 16-byte chunks of a tile row
   constexpr int MT = DP / 16;      // 16-dim tiles of the output
-  constexpr int HEADS = 8 * NT;
-  __shared__ float s_o[kAttnWarps][HEADS][DP];
-  __shared__ float s_m[kAttnWarps][HEADS], s_mv[kAttnWarps][HEADS], s_l[kAttnWarps][HEADS];
+  constexpr int VW = RB / 32;      // words of a v row per lane and half
+  constexpr int HEADS = S::HEADS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float(*s_o)[HEADS][DP] = reinterpret_cast<float(*)[HEADS][DP]>(smem);
+  float(*s_m)[HEADS] = reinterpret_cast<float(*)[HEADS]>(smem + kAttnWarps * HEADS * DP * 4);
+  float(*s_mv)[HEADS] = s_m + kAttnWarps;
+  float(*s_l)[HEADS] = s_mv + kAttnWarps;
   __shared__ long long s_scan[kAttnWarps];
   __shared__ long long s_start[2];  // first unit's sequence, and its index within it
+  __shared__ int s_abort;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar) + warp * S::kStages;
+  const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStage;
+  const uint32_t ring_sc = smem_u32(smem) + S::kScale + warp * S::kStages * kScaleBytes;
+  if (lane < S::kStages) mbar_init(&full[lane], 33);  // the lanes' copies, and one arrival of lane 0 (TMA: with the bytes)
+  if (tid == 0) s_abort = 0;
+  fence_barrier_init();
   if (p.pdl) pdl_wait_prior_grids();
 
   // ---- deal the units: this CTA takes [u0, u1) of the batch's total ----
@@ -348,53 +413,48 @@ __global__ void __launch_bounds__(kAttnWarps * 32, DP * NT <= 128 ? 3 : 2) kv_at
   int kh = (int)(s_start[1] / nu);
   int tu = (int)(s_start[1] - (long long)kh * nu);
 
+  uint32_t used = 0;  // parity of each stage's barrier phase
+  bool broken = false;
   for (bool first = true; u < u1; first = false) {
     // ---- one segment: units [tu, tu + cnt) of item (b, kh) ----
     const int cnt = (int)((long long)(nu - tu) < u1 - u ? (long long)(nu - tu) : u1 - u);
     const int head = kh / p.head_blocks;
     const int hb0 = (kh - head * p.head_blocks) * HEADS;  // first query head of this block within the group
-    const uint8_t* kbase = p.c.k + head * p.c.k_stride[2];
-    const uint8_t* vbase = p.c.v + head * p.c.v_stride[2];
-    const float* ksbase = p.c.ks + head * p.c.ks_stride[2];
-    const float* vsbase = p.c.vs + head * p.c.vs_stride[2];
+    const float* sbase = lane < 16 ? p.c.ks + head * p.c.ks_stride[2] : p.c.vs + head * p.c.vs_stride[2];
 
-    // q as the B operand: lane (g, t) holds head g, dims c * 64 + 16 t + 0..15
-    uint32_t qf[NT][KC][8];
+    // q as the B operand: lane (g, t) holds head g, dims 16 j + 4 t + 0..3 of every j
+    uint32_t qf[NT][MT][2];
     float sc[NT][2];  // score scale of heads 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int hl = hb0 + nt * 8 + g;
       const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
                              (int64_t)(head * p.group + (hl < p.group ? hl : 0)) * p.q_stride[1];
-      uint32_t raw[KC][8];
       float m = 0.f;
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const bool in = hl < p.group && c * 64 + t * 16 < p.c.head_dim;
+      for (int j = 0; j < MT; ++j) {
+        const int d = 16 * j + 4 * t;
+        const uint2 x = hl < p.group && d < p.c.head_dim ? __ldg(reinterpret_cast<const uint2*>(qrow + d)) : make_uint2(0, 0);
+        qf[nt][j][0] = x.x;
+        qf[nt][j][1] = x.y;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 x = in ? __ldg(reinterpret_cast<const uint4*>(qrow + c * 64 + t * 16 + h * 8))
-                             : make_uint4(0, 0, 0, 0);
-          raw[c][4 * h] = x.x, raw[c][4 * h + 1] = x.y, raw[c][4 * h + 2] = x.z, raw[c][4 * h + 3] = x.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)raw[c][i])));
-          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)(raw[c][i] >> 16))));
+        for (int i = 0; i < 2; ++i) {
+          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)qf[nt][j][i])));
+          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)(qf[nt][j][i] >> 16))));
         }
       }
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
       // the largest lands in [1, 2): e = its exponent, applied in two steps so
       // that neither factor leaves fp32's range
-      int e = m > 0.f && m <= 3.4e38f ? ilogbf(m) : 0;
+      const int e = m > 0.f && m <= 3.4e38f ? ilogbf(m) : 0;
       const float f1 = exp2f((float)(-e / 2)), f2 = exp2f((float)(-e - (-e / 2)));
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
+      for (int j = 0; j < MT; ++j) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          qf[nt][c][i] = pack_f16(elem_to_float<BF16>((uint16_t)raw[c][i]) * f1 * f2,
-                                  elem_to_float<BF16>((uint16_t)(raw[c][i] >> 16)) * f1 * f2);
+        for (int i = 0; i < 2; ++i) {
+          qf[nt][j][i] = pack_f16(elem_to_float<BF16>((uint16_t)qf[nt][j][i]) * f1 * f2,
+                                  elem_to_float<BF16>((uint16_t)(qf[nt][j][i] >> 16)) * f1 * f2);
         }
       }
       const float s = p.scale_log2 / f1 / f2;
@@ -413,14 +473,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, DP * NT <= 128 ? 3 : 2) kv_at
     }
 
     const int32_t* table = p.table + b * p.table_stride;
-    // Page of this warp's tile in unit i (PAGE16: the whole tile lies in one
-    // page; otherwise lane j < 16 looks up token j). A masked token or a page
-    // outside the pool gives -1: nothing of it is read.
-    auto lookup = [&](int i, int& page, int& off) {
-      const int tok = (tu + i) * kUnit + warp * 16 + (PAGE16 ? 0 : (lane & 15));
-      page = -1;
+    const int first_tok = tu * kUnit + warp * kTile;  // of this warp; its stage i starts kUnit * i later
+    const int held = n - first_tok;                   // tokens from there to the end
+    const int stages = held <= 0 ? 0 : (held - 1) / kUnit + 1 < cnt ? (held - 1) / kUnit + 1 : cnt;
+
+    // Page of token tok, or -1 (past the end, or not a page of the pool): such tokens are never read.
+    auto page_of = [&](int tok, int& off) {
+      int page = -1;
       off = 0;
-      if (i < cnt && tok < n) {
+      if (tok < n) {
         const uint32_t pi = fdiv((uint32_t)tok, p.page_div);
         off = tok - (int)pi * p.c.page_size;
         page = __ldg(table + pi);
@@ -429,152 +490,266 @@ __global__ void __launch_bounds__(kAttnWarps * 32, DP * NT <= 128 ? 3 : 2) kv_at
           page = -1;
         }
       }
+      return page;
     };
-    auto load = [&](KvTile<DP>& x, int i, int page, int off) {
-      const int t0 = (tu + i) * kUnit + warp * 16;
-      auto place = [&](int j, int64_t& pg, int64_t& of) -> bool {
-        if constexpr (PAGE16) {
-          pg = page;
-          of = off + j;
-        } else {
-          pg = __shfl_sync(0xffffffffu, page, j);
-          of = __shfl_sync(0xffffffffu, off, j);
+    // TMA: lane j holds the page of this warp's 16-token tile 32 k + j, for the
+    // batch k in use and the one after; otherwise lane j the page of token j of
+    // the next stage.
+    int off_a = 0, off_b = 0;
+    auto tile_page = [&](int j) { return page_of(first_tok + (j >> 1) * kUnit + (j & 1) * 16, off_b); };
+    auto stage_page = [&](int i) { return page_of(first_tok + i * kUnit + lane, off_b); };
+    int pg_a = TMA ? tile_page(lane) : stage_page(0);
+    off_a = off_b;
+    int pg_b = TMA ? tile_page(32 + lane) : 0;
+
+    auto fill = [&](int i) {  // starts the copies of stage i
+      const int slot = i % S::kStages;
+      const uint32_t dst = ring + slot * S::kStage;
+      const int t0 = first_tok + i * kUnit;
+      int pg[2], of[2];  // page and offset: TMA, of a tile's first token; else of this lane's token
+      if constexpr (TMA) {
+        if ((i & 15) == 0 && i > 0) {
+          pg_a = pg_b;
+          pg_b = tile_page(2 * i + 32 + lane);
         }
-        return pg >= 0 && t0 + j < n;
-      };
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        int64_t pg, of;
-        const bool in = place(g + 8 * r, pg, of);
-        const uint8_t* row = kbase + pg * p.c.k_stride[0] + of * p.c.k_stride[1];
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const int d = c * 64 + t * 16;
-          x.k[r][c] = in && d < p.c.head_dim ? ld_stream16(row + d) : make_uint4(0, 0, 0, 0);
-        }
-        x.ks[r] = in ? __ldg(ksbase + pg * p.c.ks_stride[0] + of * p.c.ks_stride[1]) : 0.f;
-        x.vs[r] = in ? __ldg(vsbase + pg * p.c.vs_stride[0] + of * p.c.vs_stride[1]) : 0.f;
-        x.in[r] = in;
+      } else if (i > 0) {
+        pg_a = stage_page(i);
+        off_a = off_b;
       }
 #pragma unroll
-      for (int i2 = 0; i2 < 4; ++i2) {
-        int64_t pg, of;
-        const bool in = place(2 * t + (i2 & 1) + 8 * (i2 >> 1), pg, of);
-        const uint8_t* row = vbase + pg * p.c.v_stride[0] + of * p.c.v_stride[1];
-        const int d0 = g * (DP / 8);
-        if constexpr (VW == 2) {
-          const uint2 y = in && d0 < p.c.head_dim ? ld_stream8(row + d0) : make_uint2(0, 0);
-          x.v[i2][0] = y.x, x.v[i2][1] = y.y;
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (TMA) {
+          pg[h] = __shfl_sync(0xffffffffu, pg_a, (2 * i + h) & 31);
+          const int tok = t0 + 16 * h;
+          of[h] = tok - (int)fdiv((uint32_t)tok, p.page_div) * p.c.page_size;
         } else {
+          pg[h] = __shfl_sync(0xffffffffu, pg_a, 16 * h + (lane & 15));
+          of[h] = __shfl_sync(0xffffffffu, off_a, 16 * h + (lane & 15));
+        }
+      }
+      if constexpr (TMA) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[slot], ((pg[0] >= 0) + (pg[1] >= 0)) * 2 * S::kTileBytes);
 #pragma unroll
-          for (int h = 0; h < VW / 4; ++h) {
-            const uint4 y = in && d0 + 16 * h < p.c.head_dim ? ld_stream16(row + d0 + 16 * h) : make_uint4(0, 0, 0, 0);
-            x.v[i2][4 * h] = y.x, x.v[i2][4 * h + 1] = y.y, x.v[i2][4 * h + 2] = y.z, x.v[i2][4 * h + 3] = y.w;
+          for (int h = 0; h < 2; ++h) {
+            if (pg[h] < 0) continue;
+#pragma unroll
+            for (int half = 0; half < HALVES; ++half) {
+              const uint32_t at = dst + h * S::kTileBytes + half * 16 * RB;
+              const int cd = half * RB;
+              tma_load_4d(at, &kmap, &full[slot], cd, p.k_swap ? head : of[h], p.k_swap ? of[h] : head, pg[h]);
+              tma_load_4d(at + 2 * S::kTileBytes, &vmap, &full[slot], cd, p.v_swap ? head : of[h],
+                          p.v_swap ? of[h] : head, pg[h]);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll 4
+          for (int x = lane; x < 16 * HALVES * KCH; x += 32) {
+            const int row = (x / KCH) & 15, c = x % KCH, half = x / (16 * KCH);
+            const int64_t pr = __shfl_sync(0xffffffffu, pg_a, 16 * h + row);
+            const int64_t orow = __shfl_sync(0xffffffffu, off_a, 16 * h + row);
+            const int d = half * RB + 16 * c;
+            const bool ok = pr >= 0 && d < p.c.head_dim;
+            const uint32_t at = dst + h * S::kTileBytes + half * 16 * RB + tile_at<RB>(row, c);
+            cp_async16(at, ok ? p.c.k + head * p.c.k_stride[2] + pr * p.c.k_stride[0] + orow * p.c.k_stride[1] + d : p.c.k,
+                       ok ? 16 : 0);
+            cp_async16(at + 2 * S::kTileBytes,
+                       ok ? p.c.v + head * p.c.v_stride[2] + pr * p.c.v_stride[0] + orow * p.c.v_stride[1] + d : p.c.v,
+                       ok ? 16 : 0);
           }
         }
       }
+      // scales of k (lanes 0..15) and v (16..31), and which tokens there are
+      uint32_t there = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t o64 = of[h] + (TMA ? (lane & 15) : 0);
+        const bool in = pg[h] >= 0 && t0 + 16 * h + (lane & 15) < n;
+        const float* src = sbase + (lane < 16 ? pg[h] * p.c.ks_stride[0] + o64 * p.c.ks_stride[1]
+                                              : pg[h] * p.c.vs_stride[0] + o64 * p.c.vs_stride[1]);
+        cp_async4(ring_sc + slot * kScaleBytes + h * 128 + lane * 4, in ? src : p.c.ks, in ? 4 : 0);
+        there |= (__ballot_sync(0xffffffffu, in) & 0xffffu) << (16 * h);
+      }
+      if (lane == 0) {
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring_sc + slot * kScaleBytes + 256), "r"(there) : "memory");
+        if constexpr (!TMA) mbar_arrive(&full[slot]);
+      }
+      cp_async_arrive(&full[slot]);
     };
-    auto step = [&](const KvTile<DP>& x) {
-      float s[NT][4];
+
+    // places in a tile: ldmatrix rows of k, and this lane's chunk of the four tokens of v
+    const int krow = row_token<RB>(lane & 15);
+    uint32_t v_at[4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const int r = row_token<RB>(2 * t + (i & 1) + 8 * (i >> 1));
+      v_at[i] = RB == 128 ? tile_at<RB>(r, g) : tile_at<RB>(r, g >> 1) + 8 * (g & 1);
+    }
+
+    auto step = [&](int i) {
+      const int slot = i % S::kStages;
+      const uint32_t kt = ring + slot * S::kStage, vt = kt + 2 * S::kTileBytes, st = ring_sc + slot * kScaleBytes;
+      float s[2][NT][4], lv[2][2];
+      const uint32_t there = __float_as_uint(lds_f32(st + 256));  // the tokens to attend to
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const uint32_t w0[4] = {x.k[0][c].x, x.k[0][c].y, x.k[0][c].z, x.k[0][c].w};
-        const uint32_t w1[4] = {x.k[1][c].x, x.k[1][c].y, x.k[1][c].z, x.k[1][c].w};
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t a[4];
-          codes_to_f16<FP8>(w0[w], a[0], a[2]);
-          codes_to_f16<FP8>(w1[w], a[1], a[3]);
+        for (int nt = 0; nt < NT; ++nt) s[h][nt][0] = s[h][nt][1] = s[h][nt][2] = s[h][nt][3] = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<false>(s[nt], a, qf[nt][c][2 * w], qf[nt][c][2 * w + 1]);
+        for (int half = 0; half < HALVES; ++half) {
+#pragma unroll
+          for (int c = 0; c < KCH; c += 2) {
+            uint32_t r[4], a[4];
+            ldmatrix_x4(kt + h * S::kTileBytes + half * 16 * RB + tile_at<RB>(krow, c + (lane >> 4)), r);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              codes_to_f16<FP8>(r[2 * j], a[0], a[2]);
+              codes_to_f16<FP8>(r[2 * j + 1], a[1], a[3]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_16816<false>(s[h][nt], a, qf[nt][half * KCH + c + j][0], qf[nt][half * KCH + c + j][1]);
+              }
+            }
+          }
         }
       }
-      const float lv0 = lg2(x.vs[0]), lv1 = lg2(x.vs[1]);
-      uint32_t pb[NT][2];
+      float mv_t[NT][2], mx_t[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mv_t[nt][0] = mv_t[nt][1] = mx_t[nt][0] = mx_t[nt][1] = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int tok = row_token<RB>(g) + 8 * r;
+          const float ks = lds_f32(st + h * 128 + tok * 4), vs = lds_f32(st + h * 128 + 64 + tok * 4);
+          lv[h][r] = lg2(vs);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = s[h][nt][2 * r + e] * (ks * sc[nt][e]);
+              if (!((there >> (16 * h + tok)) & 1)) x = -INFINITY;
+              s[h][nt][2 * r + e] = x;
+              mx_t[nt][e] = fmaxf(mx_t[nt][e], x);
+              mv_t[nt][e] = fmaxf(mv_t[nt][e], x + lv[h][r]);
+            }
+          }
+        }
+      }
       bool grew = false;
-      float sv[NT][4], m_new[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[nt][e] = x.in[0] ? s[nt][e] * (x.ks[0] * sc[nt][e]) : -INFINITY;
-          s[nt][2 + e] = x.in[1] ? s[nt][2 + e] * (x.ks[1] * sc[nt][e]) : -INFINITY;
-          sv[nt][e] = s[nt][e] + lv0;
-          sv[nt][2 + e] = s[nt][2 + e] + lv1;
-          float a = fmaxf(s[nt][e], s[nt][2 + e]), v = fmaxf(sv[nt][e], sv[nt][2 + e]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
-            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+            mx_t[nt][e] = fmaxf(mx_t[nt][e], __shfl_xor_sync(0xffffffffu, mx_t[nt][e], d));
+            mv_t[nt][e] = fmaxf(mv_t[nt][e], __shfl_xor_sync(0xffffffffu, mv_t[nt][e], d));
           }
-          if (a > mx[nt][e]) {
-            l[nt][e] *= ex2(mx[nt][e] - a);
-            mx[nt][e] = a;
-          }
-          m_new[nt][e] = fmaxf(mv[nt][e], v);
-          grew |= m_new[nt][e] > mv[nt][e];
+          grew |= mx_t[nt][e] > mx[nt][e] || mv_t[nt][e] > mv[nt][e];
         }
       }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float f0 = m_new[nt][0] > mv[nt][0] ? ex2(mv[nt][0] - m_new[nt][0]) : 1.f;
-          const float f1 = m_new[nt][1] > mv[nt][1] ? ex2(mv[nt][1] - m_new[nt][1]) : 1.f;
-          mv[nt][0] = m_new[nt][0];
-          mv[nt][1] = m_new[nt][1];
 #pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            o[j][nt][0] *= f0, o[j][nt][2] *= f0;
-            o[j][nt][1] *= f1, o[j][nt][3] *= f1;
+          for (int e = 0; e < 2; ++e) {
+            if (mx_t[nt][e] > mx[nt][e]) {
+              l[nt][e] *= ex2(mx[nt][e] - mx_t[nt][e]);
+              mx[nt][e] = mx_t[nt][e];
+            }
+            float f = 1.f;
+            if (mv_t[nt][e] > mv[nt][e]) {
+              f = ex2(mv[nt][e] - mv_t[nt][e]);
+              mv[nt][e] = mv_t[nt][e];
+            }
+#pragma unroll
+            for (int j = 0; j < MT; ++j) o[j][nt][e] *= f, o[j][nt][2 + e] *= f;
           }
         }
       }
+      uint32_t pb[2][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         // a maximum of -inf (nothing unmasked yet): every term is exp2(-inf) = 0
         const float a0 = mx[nt][0] == -INFINITY ? 0.f : mx[nt][0], a1 = mx[nt][1] == -INFINITY ? 0.f : mx[nt][1];
         const float v0 = mv[nt][0] == -INFINITY ? 0.f : mv[nt][0], v1 = mv[nt][1] == -INFINITY ? 0.f : mv[nt][1];
-        l[nt][0] += ex2(s[nt][0] - a0) + ex2(s[nt][2] - a0);
-        l[nt][1] += ex2(s[nt][1] - a1) + ex2(s[nt][3] - a1);
-        pb[nt][0] = movmatrix_trans(pack_f16(ex2(sv[nt][0] - v0), ex2(sv[nt][1] - v1)));
-        pb[nt][1] = movmatrix_trans(pack_f16(ex2(sv[nt][2] - v0), ex2(sv[nt][3] - v1)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float x0 = s[h][nt][2 * r], x1 = s[h][nt][2 * r + 1];
+            l[nt][0] += ex2(x0 - a0);
+            l[nt][1] += ex2(x1 - a1);
+            pb[h][nt][r] = movmatrix_trans(pack_f16(ex2(x0 + lv[h][r] - v0), ex2(x1 + lv[h][r] - v1)));
+          }
+        }
       }
-      // dims 2j, 2j + 1 of this lane's DP / 8 are rows g, g + 8 of tile j
+      // dims 2j, 2j + 1 of this lane's 16 (or 8) are rows g, g + 8 of output tile j
 #pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        uint32_t a[4], c[4];
-        codes_to_f16<FP8>(prmt(x.v[0][j], x.v[1][j], 0x5140), a[0], a[1]);
-        codes_to_f16<FP8>(prmt(x.v[2][j], x.v[3][j], 0x5140), a[2], a[3]);
-        codes_to_f16<FP8>(prmt(x.v[0][j], x.v[1][j], 0x7362), c[0], c[1]);
-        codes_to_f16<FP8>(prmt(x.v[2][j], x.v[3][j], 0x7362), c[2], c[3]);
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t part = (there >> (16 * h)) & 0xffffu;
+        if (part == 0) continue;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_16816<false>(o[2 * j][nt], a, pb[nt][0], pb[nt][1]);
-          mma_16816<false>(o[2 * j + 1][nt], c, pb[nt][0], pb[nt][1]);
+        for (int half = 0; half < HALVES; ++half) {
+          uint32_t v[4][VW];
+#pragma unroll
+          for (int i2 = 0; i2 < 4; ++i2) {
+            const uint32_t at = vt + h * S::kTileBytes + half * 16 * RB + v_at[i2];
+            if constexpr (VW == 2) {
+              const uint2 y = lds64(at);
+              v[i2][0] = y.x, v[i2][1] = y.y;
+            } else {
+              const uint4 y = lds128(at);
+              v[i2][0] = y.x, v[i2][1] = y.y, v[i2][2] = y.z, v[i2][3] = y.w;
+            }
+          }
+          if (part != 0xffffu) {  // codes of tokens not held may be NaN, which a weight of 0 does not stop
+#pragma unroll
+            for (int i2 = 0; i2 < 4; ++i2) {
+              if (!((part >> row_token<RB>(2 * t + (i2 & 1) + 8 * (i2 >> 1))) & 1)) {
+#pragma unroll
+                for (int j = 0; j < VW; ++j) v[i2][j] = 0;
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            uint32_t a[4], c[4];
+            codes_to_f16<FP8>(prmt(v[0][j], v[1][j], 0x5140), a[0], a[1]);
+            codes_to_f16<FP8>(prmt(v[2][j], v[3][j], 0x5140), a[2], a[3]);
+            codes_to_f16<FP8>(prmt(v[0][j], v[1][j], 0x7362), c[0], c[1]);
+            codes_to_f16<FP8>(prmt(v[2][j], v[3][j], 0x7362), c[2], c[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816<false>(o[half * (RB / 16) + 2 * j][nt], a, pb[h][nt][0], pb[h][nt][1]);
+              mma_16816<false>(o[half * (RB / 16) + 2 * j + 1][nt], c, pb[h][nt][0], pb[h][nt][1]);
+            }
+          }
         }
       }
     };
 
-    // The next tile's codes are in flight while this one is used, and the
-    // page of the one after is looked up.
-    {
-      KvTile<DP> x0, x1;
-      int pg, of;
-      lookup(0, pg, of);
-      load(x0, 0, pg, of);
-      lookup(1, pg, of);
-      for (int i = 0; i < cnt; i += 2) {
-        load(x1, i + 1, pg, of);
-        lookup(i + 2, pg, of);
-        step(x0);
-        if (i + 1 >= cnt) break;
-        load(x0, i + 2, pg, of);
-        lookup(i + 3, pg, of);
-        step(x1);
+    for (int i = 0; i < S::kStages && i < stages; ++i) fill(i);
+    for (int i = 0; i < stages; ++i) {
+      const bool ok = mbar_wait(&full[i % S::kStages], (used >> (i % S::kStages)) & 1, p.status, 204, &s_abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        broken = true;
+        // copies in flight land before the block can end
+        for (int k = i; k < stages && k < i + S::kStages; ++k) {
+          mbar_wait(&full[k % S::kStages], (used >> (k % S::kStages)) & 1, nullptr, 0, nullptr);
+        }
+        break;
       }
+      used ^= 1u << (i % S::kStages);
+      step(i);
+      __syncwarp();
+      if (i + S::kStages < stages) fill(i + S::kStages);
     }
+    if (__syncthreads_or(broken)) return;  // reported; also: every ring is read out and can hold partial results
 
     // ---- join the warps ----
 #pragma unroll
@@ -591,8 +766,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, DP * NT <= 128 ? 3 : 2) kv_at
         }
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          s_o[warp][h][g * (DP / 8) + 2 * j] = o[j][nt][e];
-          s_o[warp][h][g * (DP / 8) + 2 * j + 1] = o[j][nt][2 + e];
+          const int d = (j / (RB / 16)) * RB + g * (RB / 8) + 2 * (j % (RB / 16));
+          s_o[warp][h][d] = o[j][nt][e];
+          s_o[warp][h][d + 1] = o[j][nt][2 + e];
         }
       }
     }
@@ -637,7 +813,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, DP * NT <= 128 ? 3 : 2) kv_at
       const int last = (int)(((u + nu) * ctas + total - 1) / total) - 1;
       p.meta[blockIdx.x] = make_int4(b * kh_n + kh, slot, last, 0);
     }
-    __syncthreads();  // the next segment reuses the shared arrays
+    // the next segment's copies (the asynchronous proxy) take the place of the partial results
+    fence_proxy_async_smem();
+    __syncthreads();
 
     u += cnt;
     tu = 0;
@@ -709,18 +887,19 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const KvAttn
   }
 }
 
-template <typename F, typename P>
-cudaError_t launch(F kern, dim3 grid, int threads, cudaStream_t stream, bool pdl, const P& p) {
+template <typename F, typename... P>
+cudaError_t launch(F kern, dim3 grid, int threads, int smem, cudaStream_t stream, bool pdl, const P&... p) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  return cudaLaunchKernelEx(&cfg, kern, p...);
 }
 
 struct AttnPlan {
@@ -733,22 +912,50 @@ AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t cap
   a.dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
   a.nt = group <= 8 || a.dp == 256 ? 1 : 2;
   a.head_blocks = (group + 8 * a.nt - 1) / (8 * a.nt);
+  const int per_sm = a.dp == 64    ? (a.nt == 1 ? AttnShape<64, 1>::kPerSm : AttnShape<64, 2>::kPerSm)
+                     : a.dp == 128 ? (a.nt == 1 ? AttnShape<128, 1>::kPerSm : AttnShape<128, 2>::kPerSm)
+                                   : AttnShape<256, 1>::kPerSm;
   const int64_t units = capacity <= kUnit ? 1 : (capacity + kUnit - 1) / kUnit;
   const int64_t items = B * kv_heads * a.head_blocks;
-  const int64_t most = (int64_t)num_sms() * (a.dp * a.nt <= 128 ? 3 : 2);
+  const int64_t most = (int64_t)num_sms() * per_sm;
   a.ctas = (int)(items > most / units ? most : items * units);
   a.cut = units > 1;
   return a;
 }
 
+// The codes as a 4-D tensor (head_dim, token and head in the order of their
+// strides, page); a box is 16 tokens of one head.
+bool encode_pool(CUtensorMap* map, const KvCache& c, uint8_t* base, const int64_t (&stride)[3], bool* swap) {
+  *swap = stride[2] < stride[1];
+  const uint64_t tok = (uint64_t)stride[1] ? stride[1] : 16, head = (uint64_t)stride[2] ? stride[2] : 16,
+                 page = (uint64_t)stride[0] ? stride[0] : 16;
+  const uint32_t rb = c.head_dim <= 64 ? 64 : 128;
+  const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)(*swap ? c.kv_heads : c.page_size),
+                            (uint64_t)(*swap ? c.page_size : c.kv_heads), (uint64_t)c.num_pages};
+  const uint64_t strides[3] = {*swap ? head : tok, *swap ? tok : head, page};
+  const uint32_t box[4] = {rb, *swap ? 1u : 16u, *swap ? 16u : 1u, 1u};
+  return encode_tensor_map_4d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dims, strides, box,
+                              rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B) == CUDA_SUCCESS;
+}
+
 template <int DP, int NT, bool FP8, bool BF16>
 cudaError_t run_attn(KvAttn p, const AttnPlan& a, cudaStream_t stream) {
-  cudaError_t e = p.c.page_size % 16 == 0
-                      ? launch(kv_attn_kernel<DP, NT, FP8, BF16, true>, dim3(a.ctas), kAttnWarps * 32, stream, p.pdl, p)
-                      : launch(kv_attn_kernel<DP, NT, FP8, BF16, false>, dim3(a.ctas), kAttnWarps * 32, stream, p.pdl, p);
+  using S = AttnShape<DP, NT>;
+  CUtensorMap kmap{}, vmap{};
+  // whole 16-token tiles per page, and strides the tensor map can hold (else the copies of 16 bytes)
+  const bool tma = p.c.page_size % 16 == 0 && encode_pool(&kmap, p.c, p.c.k, p.c.k_stride, &p.k_swap) &&
+                   encode_pool(&vmap, p.c, p.c.v, p.c.v_stride, &p.v_swap);
+  auto go = [&](auto kern) {
+    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kern), S::kAlloc);
+    return e != cudaSuccess
+               ? e
+               : launch(kern, dim3(a.ctas), kAttnWarps * 32, S::kAlloc, stream, p.pdl, kmap, vmap, p);
+  };
+  const cudaError_t e =
+      tma ? go(kv_attn_kernel<DP, NT, FP8, BF16, true>) : go(kv_attn_kernel<DP, NT, FP8, BF16, false>);
   if (e != cudaSuccess || !a.cut) return e;
   // programmatic launch: its blocks are resident by the time the partials are written
-  return launch(kv_attn_join_kernel<DP, NT, BF16>, dim3(a.ctas, p.group < 8 * NT ? p.group : 8 * NT), kJoinThreads,
+  return launch(kv_attn_join_kernel<DP, NT, BF16>, dim3(a.ctas, p.group < 8 * NT ? p.group : 8 * NT), kJoinThreads, 0,
                 stream, true, p);
 }
 
@@ -774,7 +981,7 @@ cudaError_t launch_kv_write(const KvCache& c, const void* k, const int64_t* k_st
                   make_fastdiv((uint32_t)c.kv_heads), make_fastdiv((uint32_t)c.page_size), device_status_ptr(),
                   pdl_enabled()};
   auto go = [&](auto k8, auto k16, auto k32) {
-    return launch(lpr == 8 ? k8 : lpr == 16 ? k16 : k32, grid, 256, stream, p.pdl, p);
+    return launch(lpr == 8 ? k8 : lpr == 16 ? k16 : k32, grid, 256, 0, stream, p.pdl, p);
   };
 #define NSQ_KV_GO(F, B) go(kv_write_kernel<F, B, 8>, kv_write_kernel<F, B, 16>, kv_write_kernel<F, B, 32>)
   if (fp8) return bf16 ? NSQ_KV_GO(true, true) : NSQ_KV_GO(true, false);
@@ -789,7 +996,7 @@ cudaError_t launch_kv_read(const KvCache& c, const int64_t* slots, int T, void* 
   const KvRead p{c, k, v, slots, T, make_fastdiv((uint32_t)c.kv_heads), make_fastdiv((uint32_t)c.page_size),
                  device_status_ptr(), pdl_enabled()};
   auto go = [&](auto k8, auto k16, auto k32) {
-    return launch(lpr == 8 ? k8 : lpr == 16 ? k16 : k32, grid, 256, stream, p.pdl, p);
+    return launch(lpr == 8 ? k8 : lpr == 16 ? k16 : k32, grid, 256, 0, stream, p.pdl, p);
   };
 #define NSQ_KV_GO(F, B) go(kv_read_kernel<F, B, 8>, kv_read_kernel<F, B, 16>, kv_read_kernel<F, B, 32>)
   if (fp8) return bf16 ? NSQ_KV_GO(true, true) : NSQ_KV_GO(true, false);
