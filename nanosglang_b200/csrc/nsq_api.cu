@@ -153,10 +153,10 @@ inline uint32_t map_slot(const MapKey& k) {
 
 static CUresult encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, void* base, int rank,
                                   const uint64_t (&dim)[4], const uint64_t (&stride)[3], const uint32_t (&boxd)[4],
-                                  CUtensorMapSwizzle swizzle) {
+                                  CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promo) {
   const MapKey key{reinterpret_cast<uint64_t>(base), {dim[0], dim[1], dim[2], dim[3]},
                    {stride[0], stride[1], stride[2]}, {boxd[0], boxd[1], boxd[2], boxd[3]}, rank, (int)dtype,
-                   (int)swizzle};
+                   (int)swizzle | ((int)promo << 8)};
   MapEntry& slot = t_map_cache[map_slot(key)];
   if (slot.valid && slot.key == key) {
     *map = slot.map;
@@ -183,7 +183,7 @@ static CUresult encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, v
   const cuuint32_t box[4] = {boxd[0], boxd[1], boxd[2], boxd[3]};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, dtype, (cuuint32_t)rank, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                            swizzle, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) {
     slot.key = key;
     slot.map = *map;
@@ -196,19 +196,19 @@ CUresult encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, void*
                               uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                               uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
   return encode_tensor_map(map, dtype, base, 2, {inner, outer, 0, 0}, {row_stride_bytes, 0, 0},
-                           {box_inner, box_outer, 0, 0}, swizzle);
+                           {box_inner, box_outer, 0, 0}, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 CUresult encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, void* base, uint64_t d0, uint64_t d1,
                               uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1,
                               uint32_t b2, CUtensorMapSwizzle swizzle) {
   return encode_tensor_map(map, dtype, base, 3, {d0, d1, d2, 0}, {stride1_bytes, stride2_bytes, 0}, {b0, b1, b2, 0},
-                           swizzle);
+                           swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 CUresult encode_tensor_map_4d(CUtensorMap* map, CUtensorMapDataType dtype, void* base, const uint64_t (&dims)[4],
                               const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
-  return encode_tensor_map(map, dtype, base, 4, dims, strides, box, swizzle);
+  return encode_tensor_map(map, dtype, base, 4, dims, strides, box, swizzle, CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
 }  // namespace nsq
@@ -692,6 +692,10 @@ static int kv_check(const nsq_kv_cache* c, KvCache* out) {
   for (int i = 0; i < 3; ++i) {
     if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_scale_stride[i] < 0 || c->v_scale_stride[i] < 0) {
       return NSQ_EINVAL;
+    }
+    // 32-bit strides: a page, token or head is less than 4 G elements from the next
+    if (c->k_stride[i] >> 32 || c->v_stride[i] >> 32 || c->k_scale_stride[i] >> 32 || c->v_scale_stride[i] >> 32) {
+      return NSQ_ENOTSUP;
     }
     if (c->k_stride[i] % 16 != 0 || c->v_stride[i] % 16 != 0) return NSQ_EALIGN;
   }

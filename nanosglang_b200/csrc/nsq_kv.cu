@@ -38,7 +38,8 @@ struct KvRead {
 };
 
 struct KvAttn : KvAttnArgs {
-  int group, head_blocks;
+  int group, head_blocks, slot_heads;
+  int least;  // units of the smallest share
   FastDiv page_div;
   bool k_swap, v_swap;  // the tensor map has head before token
   float scale_log2;
@@ -181,10 +182,11 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 // One query token per sequence: out[h] = sum_t p[t] v[t] / sum_t p[t],
 // p[t] = exp2(s[t] - m), s[t] = scale * log2(e) * q . k[t], m the running
 // maximum. Bound by reading the codes once; so
-//   * each warp keeps its own ring of 32-token stages in shared memory, filled
-//     ahead by TMA (one box per 16 tokens of a page and head) or, where pages
-//     are not multiples of 16 tokens, by 16-byte asynchronous copies, and
-//     works through them alone: no block barrier in the loop;
+//   * every warp works alone on its share of the tokens: it keeps a ring of
+//     32-token stages in shared memory, filled ahead by TMA (one box per 16
+//     tokens of a page and head) or, where pages are not multiples of 16
+//     tokens, by 16-byte asynchronous copies; the ring runs on from one
+//     sequence and head to the next, and no warp waits for another;
 //   * mma.m16n8k16 with 16 tokens as rows for q . k and 16 dims as rows for
 //     p . v; the query heads that share the kv head are the 8 columns. The
 //     codes are read in the swizzled tile without bank conflicts (ldmatrix for
@@ -192,20 +194,23 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 //   * q is scaled per head by a power of two into fp16's range, exact for fp16
 //     and for every bf16 within 2^-14 of the head's largest. Scores, maxima
 //     and sums are fp32;
-//   * the scale of v is folded into the exponent: the fp16 weights of p . v
-//     are exp2(s + log2(vs) - m'), with a maximum m' of their own, so that
-//     they use fp16's range whatever the scales are (half-ulp 2^-12 each); the
-//     denominator is summed in fp32 from unrounded terms. At the end the
-//     accumulator is multiplied by exp2(m' - m);
-//   * work is cut into units of 128 tokens of one (sequence, kv head) and dealt
-//     evenly to the CTAs on the device, from seq_lens: long and ragged batches
-//     fill the machine alike. A CTA's range covers whole items and at most two
-//     cut ones; those go to the workspace as fp32 partials, and a second small
-//     kernel joins them in order.
+//   * the fp16 weights of p . v are p * vs relative to a reference m' of their
+//     own (log2 of their largest), so that they use fp16's range whatever the
+//     scales are (half-ulp 2^-12 each); the denominator is summed in fp32 from
+//     unrounded terms. At the end the accumulator is multiplied by
+//     exp2(m' - m). Both references follow lazily, when a score passes m by 8
+//     or a weight passes 2^12: rescaling and the maximum over the warp are
+//     rare, and fp16 and fp32 have the room;
+//   * work is cut into units of 32 tokens of one item (sequence, kv head) and
+//     dealt evenly to the warps on the device, from seq_lens: long and ragged
+//     batches fill the machine alike. A warp's range covers whole items and at
+//     most two cut ones; those go to the workspace as fp32 partials, and a
+//     second kernel joins them in order. Where no sequence can hold more than
+//     128 tokens an item is one unit: nothing is cut and one launch does.
 
 constexpr int kAttnWarps = 4;
 constexpr int kTile = 32;  // tokens of a stage
-constexpr int kUnit = kTile * kAttnWarps;
+constexpr int kWhole = 4;  // stages of an item that is not cut
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -214,15 +219,24 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float lg2(float x) {
   float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+constexpr float kNoMax = -3e38f;  // below every score: exp2(x - kNoMax) is 0 for a masked x, and nothing is NaN
+
+// 2^(m - mm): what turns exp2(x - m) * vs into a weight relative to mm (0 while there is none)
+__device__ __forceinline__ float weight_factor(float m, float mm) {
+  return mm == kNoMax ? 0.f : ex2(fminf(m - mm, 126.f));
+}
 // acc * 2^(mm - m) / sum: the output of a head whose weights of v were taken
-// relative to mm and whose denominator relative to m (0 for an empty row; no
-// term with a scale above 0 leaves mm at -inf and acc at 0 or NaN).
+// relative to mm and whose denominator relative to m (0 for an empty row;
+// without a scale above 0, mm is kNoMax and acc 0 or NaN).
 __device__ __forceinline__ float finish(float acc, float sum, float mm, float m) {
   if (sum == 0.f) return 0.f;
-  return acc * (mm == -INFINITY ? 0.f : ex2(mm - (m == -INFINITY ? 0.f : m))) / sum;
+  return acc * (mm == kNoMax ? 0.f : ex2(mm - m)) / sum;
+}
+__device__ __forceinline__ float head_lse(float sum, float m) {
+  return sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
@@ -290,6 +304,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// Strides are below 2^32 elements (checked on the host).
+__device__ __forceinline__ int64_t mul_wide(uint32_t a, int64_t stride) {
+  return (int64_t)((uint64_t)a * (uint32_t)stride);
+}
+
 // Tokens a sequence holds: seq_lens clamped to what its page-table row can name.
 __device__ __forceinline__ int seq_tokens(const KvAttn& p, int b, bool tell) {
   int n = __ldg(p.seq_lens + b);
@@ -299,12 +318,14 @@ __device__ __forceinline__ int seq_tokens(const KvAttn& p, int b, bool tell) {
   }
   return n;
 }
-__device__ __forceinline__ int item_units(int n) { return n == 0 ? 1 : (n + kUnit - 1) / kUnit; }
+// Units of an item: its stages, or 1 where items are not cut.
+__device__ __forceinline__ int item_units(const KvAttn& p, int n) {
+  return n <= kTile || p.meta == nullptr ? 1 : (n + kTile - 1) / kTile;
+}
 
 // A warp's ring: stages of 32 tokens, k then v, each as two 16-token tiles of
-// HALVES x 16 rows of RB bytes (swizzled in RB-byte rows as TMA does), and the
-// 64 scales. The partial results of the block's warps take the ring's place
-// when a segment is done.
+// HALVES x 16 rows of RB bytes (swizzled in RB-byte rows as TMA does), the 64
+// scales and a mask of the tokens to attend to.
 constexpr int kScaleBytes = 272;
 template <int DP, int NT>
 struct AttnShape {
@@ -314,13 +335,36 @@ struct AttnShape {
   static constexpr int kStage = 4 * kTileBytes;
   static constexpr int kStages = DP == 64 ? 4 : 2;
   static constexpr int HEADS = 8 * NT;
-  static constexpr int kRing = kAttnWarps * kStages * kStage;
-  static constexpr int kJoinBytes = kAttnWarps * HEADS * (DP + 3) * 4;
-  static constexpr int kScale = kRing > kJoinBytes ? kRing : kJoinBytes;  // [warp][stage] 64 fp32 scales and a mask of tokens
+  static constexpr int kScale = kAttnWarps * kStages * kStage;
   static constexpr int kBar = kScale + kAttnWarps * kStages * kScaleBytes;
   static constexpr int kAlloc = kBar + kAttnWarps * kStages * 8 + 1024;
-  static constexpr int kCtas = 227 * 1024 / (kAlloc + 1024) < 4 ? 227 * 1024 / (kAlloc + 1024) : 4;
+  static constexpr int kCtas = 227 * 1024 / (kAlloc + 1024);
   static constexpr int kPerSm = DP * NT <= 128 ? (kCtas < 3 ? kCtas : 3) : (kCtas < 2 ? kCtas : 2);
+};
+
+// A worker's place: stage s (of 32 tokens) of item (b, kh), in the segment of
+// `cnt` units from unit tu that ends before stage s_end; `left` units to go,
+// the segment's included.
+struct Cursor {
+  int b, kh, n, nu, tu, cnt, s, s_end;
+  long long left;
+  __device__ __forceinline__ void segment() {
+    cnt = (long long)(nu - tu) < left ? nu - tu : (int)left;
+    s = tu;
+    s_end = nu == 1 && n > kTile ? (n + kTile - 1) / kTile : tu + cnt;
+  }
+  // the next item (there is one: left > cnt)
+  __device__ __forceinline__ void next(const KvAttn& p, int kh_n) {
+    left -= cnt;
+    tu = 0;
+    if (++kh == kh_n) {
+      kh = 0;
+      ++b;
+      n = seq_tokens(p, b, false);
+      nu = item_units(p, n);
+    }
+    segment();
+  }
 };
 
 // Place of 16-byte chunk c of tile row r
@@ -346,31 +390,26 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
   constexpr int HEADS = S::HEADS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float(*s_o)[HEADS][DP] = reinterpret_cast<float(*)[HEADS][DP]>(smem);
-  float(*s_m)[HEADS] = reinterpret_cast<float(*)[HEADS]>(smem + kAttnWarps * HEADS * DP * 4);
-  float(*s_mv)[HEADS] = s_m + kAttnWarps;
-  float(*s_l)[HEADS] = s_mv + kAttnWarps;
   __shared__ long long s_scan[kAttnWarps];
-  __shared__ long long s_start[2];  // first unit's sequence, and its index within it
-  __shared__ int s_abort;
+  __shared__ long long s_excl[kAttnWarps * 32];  // units ahead of each thread's sequences
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar) + warp * S::kStages;
   const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStage;
-  const uint32_t ring_sc = smem_u32(smem) + S::kScale + warp * S::kStages * kScaleBytes;
+  const uint32_t ring_sc = smem_u32(smem) + S::kScale + warp * S::kStages * kScaleBytes;  // scales, mask
   if (lane < S::kStages) mbar_init(&full[lane], 33);  // the lanes' copies, and one arrival of lane 0 (TMA: with the bytes)
-  if (tid == 0) s_abort = 0;
   fence_barrier_init();
   if (p.pdl) pdl_wait_prior_grids();
+  pdl_launch_dependents();  // the join's blocks may queue up behind this grid's; they wait for its end
 
-  // ---- deal the units: this CTA takes [u0, u1) of the batch's total ----
+  // ---- deal the units: each warp is a worker with its share of the batch's total ----
   const int kh_n = p.c.kv_heads * p.head_blocks;
   const int vpt = (p.B + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
   long long mine = 0;
   for (int i = 0; i < vpt; ++i) {
     const int b = tid * vpt + i;
-    if (b < p.B) mine += (long long)item_units(seq_tokens(p, b, blockIdx.x == 0)) * kh_n;
+    if (b < p.B) mine += (long long)item_units(p, seq_tokens(p, b, blockIdx.x == 0)) * kh_n;
   }
   long long incl = mine;
 #pragma unroll
@@ -386,42 +425,205 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
     if (w < warp) before += s_scan[w];
     total += s_scan[w];
   }
-  // (to no more CTAs than units, so that the CTAs of a cut item are neighbours)
-  const long long ctas = total < (long long)gridDim.x ? total : (long long)gridDim.x;
-  const bool idle = blockIdx.x >= ctas;
-  long long u = idle ? total : total * blockIdx.x / ctas;
-  const long long u1 = idle ? total : total * (blockIdx.x + 1) / ctas;
-  const long long excl = before + incl - mine;
-  if (u >= excl && u < excl + mine) {
-    long long rel = u - excl;
-    int b = tid * vpt;
+  s_excl[tid] = before + incl - mine;
+  // dealt so that every worker has a share, an item's workers are neighbours,
+  // and the first workers are one to a block
+  const long long all_workers = (long long)gridDim.x * kAttnWarps;
+  const long long most = total / p.least > 1 ? total / p.least : 1;
+  const long long workers = most < all_workers ? most : all_workers;
+  const long long me = (long long)warp * gridDim.x + blockIdx.x;
+  __syncthreads();  // the last one: from here on every warp is on its own
+  if (me >= workers) return;
+  const long long u0 = total * me / workers;
+  Cursor cur;  // what is worked on
+  {
+    int lo = 0, hi = kAttnWarps * 32 - 1;  // last thread with s_excl <= u0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_excl[mid] <= u0) {
+        lo = mid;
+      } else {
+        hi = mid - 1;
+      }
+    }
+    long long rel = u0 - s_excl[lo];
+    cur.b = lo * vpt;
     for (;;) {
-      const long long nb = (long long)item_units(seq_tokens(p, b, false)) * kh_n;
+      cur.n = seq_tokens(p, cur.b, false);
+      cur.nu = item_units(p, cur.n);
+      const long long nb = (long long)cur.nu * kh_n;
       if (rel < nb) break;
       rel -= nb;
-      ++b;
+      ++cur.b;
     }
-    s_start[0] = b;
-    s_start[1] = rel;
+    cur.kh = (int)(rel / cur.nu);
+    cur.tu = (int)(rel - (long long)cur.kh * cur.nu);
+    cur.left = total * (me + 1) / workers - u0;
+    cur.segment();
   }
-  if (p.meta != nullptr && tid == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  __syncthreads();
-  if (u >= u1) return;
-  int b = (int)s_start[0];
-  int n = seq_tokens(p, b, false);
-  int nu = item_units(n);
-  int kh = (int)(s_start[1] / nu);
-  int tu = (int)(s_start[1] - (long long)kh * nu);
+  Cursor ahead = cur;  // what is being fetched
 
-  uint32_t used = 0;  // parity of each stage's barrier phase
-  bool broken = false;
-  for (bool first = true; u < u1; first = false) {
-    // ---- one segment: units [tu, tu + cnt) of item (b, kh) ----
-    const int cnt = (int)((long long)(nu - tu) < u1 - u ? (long long)(nu - tu) : u1 - u);
-    const int head = kh / p.head_blocks;
-    const int hb0 = (kh - head * p.head_blocks) * HEADS;  // first query head of this block within the group
-    const float* sbase = lane < 16 ? p.c.ks + head * p.c.ks_stride[2] : p.c.vs + head * p.c.vs_stride[2];
+  // Page of token tok of the sequence in `at`, or -1 (past its end, or not a
+  // page of the pool): such tokens are never read.
+  auto page_of = [&](const Cursor& at, int tok, int& off) {
+    int page = -1;
+    off = 0;
+    if (tok < at.n) {
+      const uint32_t pi = fdiv((uint32_t)tok, p.page_div);
+      off = tok - (int)pi * p.c.page_size;
+      page = __ldg(p.table + at.b * p.table_stride + pi);
+      if ((uint32_t)page >= (uint32_t)p.c.num_pages) {
+        report(p.status, 202);
+        page = -1;
+      }
+    }
+    return page;
+  };
+  // TMA: lane j holds the page of 16-token tile 32 k + j of the item being
+  // fetched, for the batch k in use (pg_a) and the one after (pg_b), and that
+  // of tile j of the next item (pg_n).
+  int off_a = 0, pg_a = -1, pg_b = -1, pg_n = -1;
+  bool more = true;  // stages to fetch
+  auto tile_page = [&](const Cursor& at, int j) {
+    int off;
+    return page_of(at, 16 * j, off);
+  };
+  auto look_ahead = [&]() {  // pg_b and pg_n for the segment that `ahead` enters
+    const int k = (2 * ahead.s) & ~31;
+    pg_b = tile_page(ahead, k + 32 + lane);
+    if (ahead.left > ahead.cnt) {
+      Cursor nx = ahead;
+      nx.next(p, kh_n);
+      pg_n = tile_page(nx, lane);
+    }
+  };
+  if constexpr (TMA) {
+    pg_a = tile_page(ahead, ((2 * ahead.s) & ~31) + lane);
+  }
+  bool entering = true;
 
+  // this lane's scale (lanes 0..15 of k, 16..31 of v) of the first token of page 0, for the head in `ahead`
+  const float* sc_base = nullptr;
+  uint32_t sc_page = 0, sc_tok = 0;
+  int off = 0;  // offset in its page of the next stage's first token (TMA)
+  auto enter = [&]() {  // `ahead` has entered a segment
+    const int head = ahead.kh / p.head_blocks;
+    const bool is_k = lane < 16;
+    sc_page = (uint32_t)(is_k ? p.c.ks_stride[0] : p.c.vs_stride[0]);
+    sc_tok = (uint32_t)(is_k ? p.c.ks_stride[1] : p.c.vs_stride[1]);
+    sc_base = (is_k ? p.c.ks : p.c.vs) + head * (is_k ? p.c.ks_stride[2] : p.c.vs_stride[2]);
+    if constexpr (TMA) {
+      sc_base += (uint64_t)(lane & 15) * sc_tok;
+      const int tok = ahead.s * kTile;
+      off = tok - (int)fdiv((uint32_t)tok, p.page_div) * p.c.page_size;
+    }
+  };
+  enter();
+
+  auto fill = [&](int slot) {  // starts the copies of stage `ahead` and moves on
+    const uint32_t dst = ring + slot * S::kStage;
+    const int left = ahead.n - ahead.s * kTile;  // tokens from the stage's first to the end
+    const int head = ahead.kh / p.head_blocks;
+    int pg[2], of[2];  // page and offset: TMA, of a tile's first token; else of this lane's token
+    if constexpr (TMA) {
+      if (!entering && (ahead.s & 15) == 0) {
+        pg_a = pg_b;
+        pg_b = tile_page(ahead, 2 * ahead.s + 32 + lane);
+      }
+    } else {
+      pg_a = page_of(ahead, ahead.s * kTile + lane, off_a);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (TMA) {
+        pg[h] = __shfl_sync(0xffffffffu, pg_a, (2 * ahead.s + h) & 31);
+        of[h] = off;
+        off = off + 16 == p.c.page_size ? 0 : off + 16;
+      } else {
+        pg[h] = __shfl_sync(0xffffffffu, pg_a, 16 * h + (lane & 15));
+        of[h] = __shfl_sync(0xffffffffu, off_a, 16 * h + (lane & 15));
+      }
+    }
+    if constexpr (TMA) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[slot], ((pg[0] >= 0) + (pg[1] >= 0)) * 2 * S::kTileBytes);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (pg[h] < 0) continue;
+#pragma unroll
+          for (int half = 0; half < HALVES; ++half) {
+            const uint32_t at = dst + h * S::kTileBytes + half * 16 * RB;
+            const int cd = half * RB;
+            tma_load_4d(at, &kmap, &full[slot], cd, p.k_swap ? head : of[h], p.k_swap ? of[h] : head, pg[h]);
+            tma_load_4d(at + 2 * S::kTileBytes, &vmap, &full[slot], cd, p.v_swap ? head : of[h],
+                        p.v_swap ? of[h] : head, pg[h]);
+          }
+        }
+      }
+    } else {
+      const uint8_t* kb = p.c.k + head * p.c.k_stride[2];
+      const uint8_t* vb = p.c.v + head * p.c.v_stride[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll 4
+        for (int x = lane; x < 16 * HALVES * KCH; x += 32) {
+          const int row = (x / KCH) & 15, c = x % KCH, half = x / (16 * KCH);
+          const int pr = __shfl_sync(0xffffffffu, pg_a, 16 * h + row);
+          const uint32_t orow = __shfl_sync(0xffffffffu, off_a, 16 * h + row);
+          const int d = half * RB + 16 * c;
+          const bool ok = pr >= 0 && d < p.c.head_dim;
+          const uint32_t at = dst + h * S::kTileBytes + half * 16 * RB + tile_at<RB>(row, c);
+          cp_async16(at, ok ? kb + mul_wide(pr, p.c.k_stride[0]) + mul_wide(orow, p.c.k_stride[1]) + d : p.c.k, ok ? 16 : 0);
+          cp_async16(at + 2 * S::kTileBytes,
+                     ok ? vb + mul_wide(pr, p.c.v_stride[0]) + mul_wide(orow, p.c.v_stride[1]) + d : p.c.v, ok ? 16 : 0);
+        }
+      }
+    }
+    // the scales, and which tokens there are
+    uint32_t there = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool in = pg[h] >= 0 && 16 * h + (lane & 15) < left;
+      const float* src = sc_base + (uint64_t)(uint32_t)pg[h] * sc_page + (uint64_t)(uint32_t)of[h] * sc_tok;
+      cp_async4(ring_sc + slot * kScaleBytes + h * 128 + lane * 4, in ? src : p.c.ks, in ? 4 : 0);
+      there |= (__ballot_sync(0xffffffffu, in) & 0xffffu) << (16 * h);
+    }
+    if (lane == 0) {
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring_sc + slot * kScaleBytes + 256), "r"(there) : "memory");
+      if constexpr (!TMA) mbar_arrive(&full[slot]);
+    }
+    cp_async_arrive(&full[slot]);
+    __syncwarp();  // the mask is the warp's own: seen by all lanes from here on
+    if (TMA && entering) look_ahead();
+    entering = false;
+    if (++ahead.s == ahead.s_end) {
+      more = ahead.left > ahead.cnt;
+      if (more) {
+        ahead.next(p, kh_n);
+        entering = true;
+        pg_a = pg_n;
+        enter();
+      }
+    }
+  };
+
+  // places in a tile: ldmatrix rows of k, and this lane's chunk of the four tokens of v
+      const int krow = row_token<RB>(lane & 15);
+      uint32_t v_at[4];
+  #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = row_token<RB>(2 * t + (i & 1) + 8 * (i >> 1));
+        v_at[i] = RB == 128 ? tile_at<RB>(r, g) : tile_at<RB>(r, g >> 1) + 8 * (g & 1);
+      }
+
+  uint32_t filled = 0, done = 0;  // stages
+  for (; filled < S::kStages && more; ++filled) fill(filled % S::kStages);
+
+  for (bool first = true;; first = false) {
+    // ---- one segment of item (b, kh) ----
+    const int b = cur.b;
+    const int head = cur.kh / p.head_blocks;
+    const int hb0 = (cur.kh - head * p.head_blocks) * HEADS;  // first query head of this block within the group
     // q as the B operand: lane (g, t) holds head g, dims 16 j + 4 t + 0..3 of every j
     uint32_t qf[NT][MT][2];
     float sc[NT][2];  // score scale of heads 2t, 2t + 1
@@ -463,136 +665,19 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
     }
 
     float o[MT][NT][4];
-    float mx[NT][2], mv[NT][2], l[NT][2];
+    // references m and m' (kNoMax: no term yet), 2^(m - m'), denominators (this lane's tokens)
+    float mx[NT][2], mv[NT][2], vf[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
-      mx[nt][0] = mx[nt][1] = mv[nt][0] = mv[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+      mx[nt][0] = mx[nt][1] = mv[nt][0] = mv[nt][1] = kNoMax;
+      vf[nt][0] = vf[nt][1] = l[nt][0] = l[nt][1] = 0.f;
     }
 
-    const int32_t* table = p.table + b * p.table_stride;
-    const int first_tok = tu * kUnit + warp * kTile;  // of this warp; its stage i starts kUnit * i later
-    const int held = n - first_tok;                   // tokens from there to the end
-    const int stages = held <= 0 ? 0 : (held - 1) / kUnit + 1 < cnt ? (held - 1) / kUnit + 1 : cnt;
-
-    // Page of token tok, or -1 (past the end, or not a page of the pool): such tokens are never read.
-    auto page_of = [&](int tok, int& off) {
-      int page = -1;
-      off = 0;
-      if (tok < n) {
-        const uint32_t pi = fdiv((uint32_t)tok, p.page_div);
-        off = tok - (int)pi * p.c.page_size;
-        page = __ldg(table + pi);
-        if ((uint32_t)page >= (uint32_t)p.c.num_pages) {
-          report(p.status, 202);
-          page = -1;
-        }
-      }
-      return page;
-    };
-    // TMA: lane j holds the page of this warp's 16-token tile 32 k + j, for the
-    // batch k in use and the one after; otherwise lane j the page of token j of
-    // the next stage.
-    int off_a = 0, off_b = 0;
-    auto tile_page = [&](int j) { return page_of(first_tok + (j >> 1) * kUnit + (j & 1) * 16, off_b); };
-    auto stage_page = [&](int i) { return page_of(first_tok + i * kUnit + lane, off_b); };
-    int pg_a = TMA ? tile_page(lane) : stage_page(0);
-    off_a = off_b;
-    int pg_b = TMA ? tile_page(32 + lane) : 0;
-
-    auto fill = [&](int i) {  // starts the copies of stage i
-      const int slot = i % S::kStages;
-      const uint32_t dst = ring + slot * S::kStage;
-      const int t0 = first_tok + i * kUnit;
-      int pg[2], of[2];  // page and offset: TMA, of a tile's first token; else of this lane's token
-      if constexpr (TMA) {
-        if ((i & 15) == 0 && i > 0) {
-          pg_a = pg_b;
-          pg_b = tile_page(2 * i + 32 + lane);
-        }
-      } else if (i > 0) {
-        pg_a = stage_page(i);
-        off_a = off_b;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (TMA) {
-          pg[h] = __shfl_sync(0xffffffffu, pg_a, (2 * i + h) & 31);
-          const int tok = t0 + 16 * h;
-          of[h] = tok - (int)fdiv((uint32_t)tok, p.page_div) * p.c.page_size;
-        } else {
-          pg[h] = __shfl_sync(0xffffffffu, pg_a, 16 * h + (lane & 15));
-          of[h] = __shfl_sync(0xffffffffu, off_a, 16 * h + (lane & 15));
-        }
-      }
-      if constexpr (TMA) {
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&full[slot], ((pg[0] >= 0) + (pg[1] >= 0)) * 2 * S::kTileBytes);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (pg[h] < 0) continue;
-#pragma unroll
-            for (int half = 0; half < HALVES; ++half) {
-              const uint32_t at = dst + h * S::kTileBytes + half * 16 * RB;
-              const int cd = half * RB;
-              tma_load_4d(at, &kmap, &full[slot], cd, p.k_swap ? head : of[h], p.k_swap ? of[h] : head, pg[h]);
-              tma_load_4d(at + 2 * S::kTileBytes, &vmap, &full[slot], cd, p.v_swap ? head : of[h],
-                          p.v_swap ? of[h] : head, pg[h]);
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll 4
-          for (int x = lane; x < 16 * HALVES * KCH; x += 32) {
-            const int row = (x / KCH) & 15, c = x % KCH, half = x / (16 * KCH);
-            const int64_t pr = __shfl_sync(0xffffffffu, pg_a, 16 * h + row);
-            const int64_t orow = __shfl_sync(0xffffffffu, off_a, 16 * h + row);
-            const int d = half * RB + 16 * c;
-            const bool ok = pr >= 0 && d < p.c.head_dim;
-            const uint32_t at = dst + h * S::kTileBytes + half * 16 * RB + tile_at<RB>(row, c);
-            cp_async16(at, ok ? p.c.k + head * p.c.k_stride[2] + pr * p.c.k_stride[0] + orow * p.c.k_stride[1] + d : p.c.k,
-                       ok ? 16 : 0);
-            cp_async16(at + 2 * S::kTileBytes,
-                       ok ? p.c.v + head * p.c.v_stride[2] + pr * p.c.v_stride[0] + orow * p.c.v_stride[1] + d : p.c.v,
-                       ok ? 16 : 0);
-          }
-        }
-      }
-      // scales of k (lanes 0..15) and v (16..31), and which tokens there are
-      uint32_t there = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t o64 = of[h] + (TMA ? (lane & 15) : 0);
-        const bool in = pg[h] >= 0 && t0 + 16 * h + (lane & 15) < n;
-        const float* src = sbase + (lane < 16 ? pg[h] * p.c.ks_stride[0] + o64 * p.c.ks_stride[1]
-                                              : pg[h] * p.c.vs_stride[0] + o64 * p.c.vs_stride[1]);
-        cp_async4(ring_sc + slot * kScaleBytes + h * 128 + lane * 4, in ? src : p.c.ks, in ? 4 : 0);
-        there |= (__ballot_sync(0xffffffffu, in) & 0xffffu) << (16 * h);
-      }
-      if (lane == 0) {
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring_sc + slot * kScaleBytes + 256), "r"(there) : "memory");
-        if constexpr (!TMA) mbar_arrive(&full[slot]);
-      }
-      cp_async_arrive(&full[slot]);
-    };
-
-    // places in a tile: ldmatrix rows of k, and this lane's chunk of the four tokens of v
-    const int krow = row_token<RB>(lane & 15);
-    uint32_t v_at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = row_token<RB>(2 * t + (i & 1) + 8 * (i >> 1));
-      v_at[i] = RB == 128 ? tile_at<RB>(r, g) : tile_at<RB>(r, g >> 1) + 8 * (g & 1);
-    }
-
-    auto step = [&](int i) {
-      const int slot = i % S::kStages;
+    auto step = [&](int slot) {
       const uint32_t kt = ring + slot * S::kStage, vt = kt + 2 * S::kTileBytes, st = ring_sc + slot * kScaleBytes;
-      float s[2][NT][4], lv[2][2];
+      float s[2][NT][4];
       const uint32_t there = __float_as_uint(lds_f32(st + 256));  // the tokens to attend to
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -616,76 +701,116 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
           }
         }
       }
-      float mv_t[NT][2], mx_t[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mv_t[nt][0] = mv_t[nt][1] = mx_t[nt][0] = mx_t[nt][1] = -INFINITY;
+      // scores x, relative to the reference m their exponentials
+      float vs[2][2];
+      bool over = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int tok = row_token<RB>(g) + 8 * r;
-          const float ks = lds_f32(st + h * 128 + tok * 4), vs = lds_f32(st + h * 128 + 64 + tok * 4);
-          lv[h][r] = lg2(vs);
+          const float ks = lds_f32(st + h * 128 + tok * 4);
+          vs[h][r] = lds_f32(st + h * 128 + 64 + tok * 4);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = s[h][nt][2 * r + e] * (ks * sc[nt][e]);
-              if (!((there >> (16 * h + tok)) & 1)) x = -INFINITY;
-              s[h][nt][2 * r + e] = x;
-              mx_t[nt][e] = fmaxf(mx_t[nt][e], x);
-              mv_t[nt][e] = fmaxf(mv_t[nt][e], x + lv[h][r]);
-            }
+            for (int e = 0; e < 2; ++e) s[h][nt][2 * r + e] *= ks * sc[nt][e];
           }
         }
       }
-      bool grew = false;
+      if (there != 0xffffffffu) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if ((there >> (16 * h + row_token<RB>(g) + 8 * r)) & 1) continue;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[h][nt][2 * r] = s[h][nt][2 * r + 1] = -INFINITY;
+          }
+        }
+      }
+      float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            mx_t[nt][e] = fmaxf(mx_t[nt][e], __shfl_xor_sync(0xffffffffu, mx_t[nt][e], d));
-            mv_t[nt][e] = fmaxf(mv_t[nt][e], __shfl_xor_sync(0xffffffffu, mv_t[nt][e], d));
-          }
-          grew |= mx_t[nt][e] > mx[nt][e] || mv_t[nt][e] > mv[nt][e];
+          top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e]));
+          over |= top[nt][e] > mx[nt][e] + 8.f;
         }
       }
-      if (__any_sync(0xffffffffu, grew)) {
+      if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            if (mx_t[nt][e] > mx[nt][e]) {
-              l[nt][e] *= ex2(mx[nt][e] - mx_t[nt][e]);
-              mx[nt][e] = mx_t[nt][e];
+            float a = top[nt][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+            if (a > mx[nt][e]) {
+              l[nt][e] *= ex2(mx[nt][e] - a);
+              mx[nt][e] = a;
+              vf[nt][e] = weight_factor(a, mv[nt][e]);
             }
-            float f = 1.f;
-            if (mv_t[nt][e] > mv[nt][e]) {
-              f = ex2(mv[nt][e] - mv_t[nt][e]);
-              mv[nt][e] = mv_t[nt][e];
+          }
+        }
+      }
+      float wt[2][NT][4];
+      over = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float big = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float x = ex2(s[h][nt][2 * r + e] - mx[nt][e]);
+              l[nt][e] += x;
+              wt[h][nt][2 * r + e] = x * (vs[h][r] * vf[nt][e]);
+              big = fmaxf(big, wt[h][nt][2 * r + e]);
+            }
+          }
+          over |= big > 4096.f || mv[nt][e] == kNoMax;
+        }
+      }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) v = fmaxf(v, s[h][nt][2 * r + e] + lg2(vs[h][r]));
             }
 #pragma unroll
-            for (int j = 0; j < MT; ++j) o[j][nt][e] *= f, o[j][nt][2 + e] *= f;
+            for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+            if (v > mv[nt][e]) {
+              const float f = ex2(mv[nt][e] - v);
+              mv[nt][e] = v;
+              vf[nt][e] = weight_factor(mx[nt][e], v);
+#pragma unroll
+              for (int j = 0; j < MT; ++j) o[j][nt][e] *= f, o[j][nt][2 + e] *= f;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                wt[h][nt][2 * r + e] = ex2(s[h][nt][2 * r + e] - mx[nt][e]) * (vs[h][r] * vf[nt][e]);
+              }
+            }
           }
         }
       }
       uint32_t pb[2][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        // a maximum of -inf (nothing unmasked yet): every term is exp2(-inf) = 0
-        const float a0 = mx[nt][0] == -INFINITY ? 0.f : mx[nt][0], a1 = mx[nt][1] == -INFINITY ? 0.f : mx[nt][1];
-        const float v0 = mv[nt][0] == -INFINITY ? 0.f : mv[nt][0], v1 = mv[nt][1] == -INFINITY ? 0.f : mv[nt][1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float x0 = s[h][nt][2 * r], x1 = s[h][nt][2 * r + 1];
-            l[nt][0] += ex2(x0 - a0);
-            l[nt][1] += ex2(x1 - a1);
-            pb[h][nt][r] = movmatrix_trans(pack_f16(ex2(x0 + lv[h][r] - v0), ex2(x1 + lv[h][r] - v1)));
-          }
+          for (int r = 0; r < 2; ++r) pb[h][nt][r] = movmatrix_trans(pack_f16(wt[h][nt][2 * r], wt[h][nt][2 * r + 1]));
         }
       }
       // dims 2j, 2j + 1 of this lane's 16 (or 8) are rows g, g + 8 of output tile j
@@ -733,25 +858,27 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
       }
     };
 
-    for (int i = 0; i < S::kStages && i < stages; ++i) fill(i);
-    for (int i = 0; i < stages; ++i) {
-      const bool ok = mbar_wait(&full[i % S::kStages], (used >> (i % S::kStages)) & 1, p.status, 204, &s_abort);
-      if (!__all_sync(0xffffffffu, ok)) {
-        broken = true;
-        // copies in flight land before the block can end
-        for (int k = i; k < stages && k < i + S::kStages; ++k) {
-          mbar_wait(&full[k % S::kStages], (used >> (k % S::kStages)) & 1, nullptr, 0, nullptr);
+    for (; cur.s < cur.s_end; ++cur.s, ++done) {
+      const int slot = done % S::kStages;
+      const bool ok = mbar_wait(&full[slot], (done / S::kStages) & 1, p.status, 204, nullptr);
+      if (!__all_sync(0xffffffffu, ok)) {  // recorded; the copies in flight land before the block can end
+        for (; done < filled; ++done) {
+          mbar_wait(&full[done % S::kStages], (done / S::kStages) & 1, nullptr, 0, nullptr);
         }
-        break;
+        return;
       }
-      used ^= 1u << (i % S::kStages);
-      step(i);
+      step(slot);
       __syncwarp();
-      if (i + S::kStages < stages) fill(i + S::kStages);
+      if (more) {
+        fill(slot);
+        ++filled;
+      }
     }
-    if (__syncthreads_or(broken)) return;  // reported; also: every ring is read out and can hold partial results
 
-    // ---- join the warps ----
+    // ---- the segment's result: lane (g, t) holds heads 2t, 2t + 1 and the dims of its chunk ----
+    const bool opens = cur.tu == 0, closes = cur.tu + cur.cnt == cur.nu;
+    const bool whole = opens && closes;
+    const long long slot = 2 * me + (first ? 0 : 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -759,131 +886,221 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
         const int h = nt * 8 + 2 * t + e;
-        if (g == 0) {
-          s_m[warp][h] = mx[nt][e];
-          s_mv[warp][h] = mv[nt][e];
-          s_l[warp][h] = l[nt][e];
-        }
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const int d = (j / (RB / 16)) * RB + g * (RB / 8) + 2 * (j % (RB / 16));
-          s_o[warp][h][d] = o[j][nt][e];
-          s_o[warp][h][d + 1] = o[j][nt][2 + e];
-        }
-      }
-    }
-    __syncthreads();
-    const bool whole = cnt == nu;
-    const int slot = 2 * blockIdx.x + (first ? 0 : 1);
-    const int heads = p.group - hb0 < HEADS ? p.group - hb0 : HEADS;
-    for (int i = tid; i < heads * DP; i += kAttnWarps * 32) {
-      const int h = i / DP, d = i - h * DP;
-      float m = -INFINITY, mm = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        m = fmaxf(m, s_m[w][h]);
-        mm = fmaxf(mm, s_mv[w][h]);
-      }
-      const float m0 = m == -INFINITY ? 0.f : m, mm0 = mm == -INFINITY ? 0.f : mm;
-      float acc = 0.f, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        acc += s_o[w][h][d] * ex2(s_mv[w][h] - mm0);
-        sum += s_l[w][h] * ex2(s_m[w][h] - m0);
-      }
-      if (whole) {
+        if (hb0 + h >= p.group) continue;
+        const float m = mx[nt][e], mm = mv[nt][e], sum = l[nt][e];
         const int64_t row = (int64_t)b * p.H + head * p.group + hb0 + h;
-        if (d < p.c.head_dim) {
-          const float y = finish(acc, sum, mm, m);
-          static_cast<uint16_t*>(p.out)[row * p.c.head_dim + d] = float_to_elem<BF16>(y);
+        float* ws = whole ? nullptr : p.partial + (slot * p.slot_heads + h) * (DP + 4);
+        if (g == 0) {
+          if (whole) {
+            if (p.lse != nullptr) p.lse[row] = head_lse(sum, m);
+          } else {
+            *reinterpret_cast<float4*>(ws) = make_float4(m, mm, sum, 0.f);
+          }
         }
-        if (d == 0 && p.lse != nullptr) p.lse[row] = sum == 0.f ? -INFINITY : (m0 + log2f(sum)) * 0.69314718055994531f;
-      } else {
-        float* ws = p.partial + (int64_t)slot * HEADS * (DP + 4) + h * (DP + 4);
-        ws[4 + d] = acc;
-        if (d == 0) {
-          ws[0] = m;
-          ws[1] = mm;
-          ws[2] = sum;
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+          const int d0 = half * RB + g * (RB / 8);
+#pragma unroll
+          for (int c = 0; c < RB / 64; ++c) {  // 8 dims at a time
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              y[2 * j] = o[half * (RB / 16) + 4 * c + j][nt][e];
+              y[2 * j + 1] = o[half * (RB / 16) + 4 * c + j][nt][2 + e];
+            }
+            if (whole) {
+              if (d0 + 8 * c < p.c.head_dim) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  w[j] = (uint32_t)float_to_elem<BF16>(finish(y[2 * j], sum, mm, m)) |
+                         ((uint32_t)float_to_elem<BF16>(finish(y[2 * j + 1], sum, mm, m)) << 16);
+                }
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.c.head_dim + d0 + 8 * c) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            } else {
+              *reinterpret_cast<float4*>(ws + 4 + d0 + 8 * c) = make_float4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<float4*>(ws + 8 + d0 + 8 * c) = make_float4(y[4], y[5], y[6], y[7]);
+            }
+          }
         }
       }
     }
-    // the CTA that opens a cut item says which slot it used and which CTA closes the item
-    if (!whole && tu == 0 && tid == 0) {
-      const int last = (int)(((u + nu) * ctas + total - 1) / total) - 1;
-      p.meta[blockIdx.x] = make_int4(b * kh_n + kh, slot, last, 0);
+    // the worker that opens an item says whether it is cut, and then which slot
+    // it used and which workers follow
+    if (whole && p.meta != nullptr && lane == 0) p.meta[b * kh_n + cur.kh] = make_int4(-1, 0, 0, 0);
+    if (opens && !closes && lane == 0) {
+      const long long end = total * (me + 1) / workers - cur.left + cur.nu;  // units up to the item's end
+      const long long last = (end * workers + total - 1) / total - 1;
+      p.meta[b * kh_n + cur.kh] = make_int4((int)(last - me) + 1, (int)slot, (int)me, 0);
     }
-    // the next segment's copies (the asynchronous proxy) take the place of the partial results
-    fence_proxy_async_smem();
-    __syncthreads();
-
-    u += cnt;
-    tu = 0;
-    if (++kh == kh_n && u < u1) {
-      kh = 0;
-      ++b;
-      n = seq_tokens(p, b, false);
-      nu = item_units(n);
-    }
+    if (cur.left == cur.cnt) return;
+    cur.next(p, kh_n);
   }
 }
 
-// Joins the partials of cut items, one CTA per (opening CTA, query head): its
-// slot, then the first slots of the CTAs after it up to the one that closes
-// the item, always in that order, so results do not depend on timing.
-constexpr int kJoinThreads = 256;
-template <int DP, int NT, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const KvAttn p) {
-  constexpr int HEADS = 8 * NT;
-  constexpr int KG = kJoinThreads / DP;  // groups of threads that share the partials out
-  constexpr int64_t kRow = DP + 4, kSlot = (int64_t)HEADS * kRow;
-  __shared__ float s_part[KG][DP], s_m[KG], s_mv[KG], s_l[KG];
+// Joins the partials of cut items: the slot that the opening worker named and
+// the first slots of the workers after it, always in the same order, so
+// results do not depend on timing. A pair (query head, item) is a warp's, or,
+// from more than kJoinWarp partials on, all warps' of its block; with PAIRS =
+// 1 (few pairs) a block has 32 dims of one pair. Consecutive pairs are different items,
+// so one long item is spread over blocks.
+constexpr int kJoinWarp = 16;
+template <int DP, int NT, bool BF16, int PAIRS>
+__global__ void __launch_bounds__(PAIRS == 1 ? 256 : 32 * PAIRS) kv_attn_join_kernel(const KvAttn p, int items) {
+  constexpr int kJoinThreads = PAIRS == 1 ? 256 : 32 * PAIRS;
+  constexpr int LANES = PAIRS == 1 ? 8 : DP / 4;  // threads that share a partial's row (or 32 dims of it), four dims each
+  constexpr int KG = kJoinThreads / LANES;        // partials read side by side
+  constexpr int V4 = DP > 128 ? DP / 128 : 1;     // four-dim pieces of a row per lane, in the one-warp form
+  constexpr int64_t kRow = DP + 4;
+  __shared__ float4 s_part[KG][LANES];
+  __shared__ float s_w[kJoinThreads], s_red[3][kJoinThreads / 32];
   pdl_wait_prior_grids();
-  const int4 me = p.meta[blockIdx.x];
-  if (me.x < 0) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kh_n = p.c.kv_heads * p.head_blocks;
-  const int b = me.x / kh_n, kh = me.x - b * kh_n;
-  const int head = kh / p.head_blocks, h = blockIdx.y;
-  const int hq = (kh - head * p.head_blocks) * HEADS + h;
-  if (hq >= p.group) return;
-  const int count = me.z - (int)blockIdx.x + 1;
-  const int d = threadIdx.x % DP, kg = threadIdx.x / DP;
-  const float* ws = p.partial + h * kRow;
-  float m = -INFINITY, mm = -INFINITY, acc = 0.f, sum = 0.f;
-#pragma unroll 4
-  for (int k = kg; k < count; k += KG) {
-    const float* x = ws + (k == 0 ? me.y : 2 * ((int64_t)blockIdx.x + k)) * kSlot;
-    const float mk = x[0], mmk = x[1], lk = x[2], ok = x[4 + d];
-    const float mn = fmaxf(m, mk), mmn = fmaxf(mm, mmk);
-    const float z = mn == -INFINITY ? 0.f : mn, zz = mmn == -INFINITY ? 0.f : mmn;
-    acc = acc * ex2(mm - zz) + ok * ex2(mmk - zz);
-    sum = sum * ex2(m - z) + lk * ex2(mk - z);
-    m = mn;
-    mm = mmn;
-  }
-  s_part[kg][d] = acc;
-  if (d == 0) {
-    s_m[kg] = m;
-    s_mv[kg] = mm;
-    s_l[kg] = sum;
-  }
-  __syncthreads();
-  if (kg != 0) return;
+  const int64_t slot_row = p.slot_heads * kRow;
+  // item and query head (of its block) of a pair; partials to join (0: none)
+  auto look = [&](int pair, int& item, int& h, int4& me) -> int {
+    h = pair / items;
+    item = pair - h * items;
+    if (h >= p.slot_heads || ((item % kh_n) % p.head_blocks) * (8 * NT) + h >= p.group) return 0;
+    me = __ldg(p.meta + item);
+    return me.x < 0 ? 0 : me.x;
+  };
+  auto store = [&](int item, int h, int d4, float4 acc, float sum, float mm, float m) {
+    const int b = item / kh_n, kh = item - b * kh_n;
+    const int head = kh / p.head_blocks;
+    const int64_t row = (int64_t)b * p.H + head * p.group + (kh - head * p.head_blocks) * (8 * NT) + h;
+    if (4 * d4 < p.c.head_dim) {
+      const uint32_t lo = (uint32_t)float_to_elem<BF16>(finish(acc.x, sum, mm, m)) |
+                          ((uint32_t)float_to_elem<BF16>(finish(acc.y, sum, mm, m)) << 16);
+      const uint32_t hi = (uint32_t)float_to_elem<BF16>(finish(acc.z, sum, mm, m)) |
+                          ((uint32_t)float_to_elem<BF16>(finish(acc.w, sum, mm, m)) << 16);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * p.c.head_dim + 4 * d4) = make_uint2(lo, hi);
+    }
+    if (d4 == 0 && p.lse != nullptr) p.lse[row] = head_lse(sum, m);
+  };
+
+  int item, h;
+  int4 me;
+  const int count = look(blockIdx.x * PAIRS + (PAIRS == 1 ? 0 : warp), item, h, me);
+  if (PAIRS > 1 && count > 0 && count <= kJoinWarp) {
+    auto part = [&](int k) { return p.partial + (k == 0 ? (int64_t)me.y : 2 * ((int64_t)me.z + k)) * slot_row + h * kRow; };
+    const float4 x0 = lane < count ? *reinterpret_cast<const float4*>(part(lane)) : make_float4(kNoMax, kNoMax, 0.f, 0.f);
+    float4 x[kJoinWarp][V4];  // all in flight at once
 #pragma unroll
-  for (int k = 1; k < KG; ++k) {
-    const float mn = fmaxf(m, s_m[k]), mmn = fmaxf(mm, s_mv[k]);
-    const float z = mn == -INFINITY ? 0.f : mn, zz = mmn == -INFINITY ? 0.f : mmn;
-    acc = acc * ex2(mm - zz) + s_part[k][d] * ex2(s_mv[k] - zz);
-    sum = sum * ex2(m - z) + s_l[k] * ex2(s_m[k] - z);
-    m = mn;
-    mm = mmn;
+    for (int k = 0; k < kJoinWarp; ++k) {
+#pragma unroll
+      for (int v = 0; v < V4; ++v) {
+        x[k][v] = k < count && lane + 32 * v < LANES
+                      ? *reinterpret_cast<const float4*>(part(k) + 4 + 4 * (lane + 32 * v))
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    float m = x0.x, mm = x0.y;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    }
+    m = __shfl_sync(0xffffffffu, m, 0);
+    mm = __shfl_sync(0xffffffffu, mm, 0);
+    float sum = x0.z * ex2(x0.x - m);
+    const float w0 = ex2(x0.y - mm);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    float4 acc[V4];
+#pragma unroll
+    for (int v = 0; v < V4; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kJoinWarp; ++k) {
+      const float f = __shfl_sync(0xffffffffu, w0, k);
+#pragma unroll
+      for (int v = 0; v < V4; ++v) {
+        if (k < count) {
+          acc[v].x = fmaf(x[k][v].x, f, acc[v].x);
+          acc[v].y = fmaf(x[k][v].y, f, acc[v].y);
+          acc[v].z = fmaf(x[k][v].z, f, acc[v].z);
+          acc[v].w = fmaf(x[k][v].w, f, acc[v].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V4; ++v) {
+      if (lane + 32 * v < LANES) store(item, h, lane + 32 * v, acc[v], sum, mm, m);
+    }
   }
-  const int64_t row = (int64_t)b * p.H + head * p.group + hq;
-  if (d < p.c.head_dim) {
-    static_cast<uint16_t*>(p.out)[row * p.c.head_dim + d] = float_to_elem<BF16>(finish(acc, sum, mm, m));
-  }
-  if (d == 0 && p.lse != nullptr) {
-    p.lse[row] = sum == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(sum)) * 0.69314718055994531f;
+  if (PAIRS > 1 && !__syncthreads_or(count > kJoinWarp)) return;
+
+  for (int i = 0; i < PAIRS; ++i) {
+    int item, h;
+    int4 me;
+    const int count = look(blockIdx.x * PAIRS + i, item, h, me);
+    if (count == 0 || (PAIRS > 1 && count <= kJoinWarp)) continue;
+    auto part = [&](int k) { return p.partial + (k == 0 ? (int64_t)me.y : 2 * ((int64_t)me.z + k)) * slot_row + h * kRow; };
+    // the maxima over all partials
+    float m = kNoMax, mm = kNoMax;
+    for (int k = tid; k < count; k += kJoinThreads) {
+      const float4 x = *reinterpret_cast<const float4*>(part(k));
+      m = fmaxf(m, x.x);
+      mm = fmaxf(mm, x.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    }
+    __syncthreads();  // the item before is done with the shared arrays
+    if ((tid & 31) == 0) {
+      s_red[0][tid >> 5] = m;
+      s_red[1][tid >> 5] = mm;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) {
+      m = fmaxf(m, s_red[0][i]);
+      mm = fmaxf(mm, s_red[1][i]);
+    }
+    // weights of kJoinThreads partials at a time, then their sum
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int d = tid % LANES + (PAIRS == 1 ? blockIdx.y * LANES : 0), kg = tid / LANES;
+    for (int k0 = 0; k0 < count; k0 += kJoinThreads) {
+      const int here = count - k0 < kJoinThreads ? count - k0 : kJoinThreads;
+      if (k0 > 0) __syncthreads();
+      if (tid < here) {
+        const float4 x = *reinterpret_cast<const float4*>(part(k0 + tid));
+        sum += x.z * ex2(x.x - m);
+        s_w[tid] = ex2(x.y - mm);
+      }
+      __syncthreads();
+#pragma unroll 8
+      for (int k = kg; k < here; k += KG) {
+        const float4 x = *reinterpret_cast<const float4*>(part(k0 + k) + 4 + 4 * d);
+        const float f = s_w[k];
+        acc.x = fmaf(x.x, f, acc.x);
+        acc.y = fmaf(x.y, f, acc.y);
+        acc.z = fmaf(x.z, f, acc.z);
+        acc.w = fmaf(x.w, f, acc.w);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((tid & 31) == 0) s_red[2][tid >> 5] = sum;
+    s_part[kg][tid % LANES] = acc;
+    __syncthreads();
+    if (kg == 0) {
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kJoinThreads / 32; ++i) sum += s_red[2][i];
+#pragma unroll
+      for (int i = 1; i < KG; ++i) {
+        const float4 x = s_part[i][tid % LANES];
+        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+      }
+      store(item, h, d, acc, sum, mm, m);
+    }
   }
 }
 
@@ -903,8 +1120,8 @@ cudaError_t launch(F kern, dim3 grid, int threads, int smem, cudaStream_t stream
 }
 
 struct AttnPlan {
-  int dp, nt, head_blocks, ctas;
-  bool cut;  // an item can span CTAs: the join kernel and its workspace are needed
+  int dp, nt, head_blocks, ctas, slot_heads;
+  bool cut;  // an item can span workers: the join kernel and its workspace are needed
 };
 
 AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t capacity) {
@@ -915,11 +1132,12 @@ AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t cap
   const int per_sm = a.dp == 64    ? (a.nt == 1 ? AttnShape<64, 1>::kPerSm : AttnShape<64, 2>::kPerSm)
                      : a.dp == 128 ? (a.nt == 1 ? AttnShape<128, 1>::kPerSm : AttnShape<128, 2>::kPerSm)
                                    : AttnShape<256, 1>::kPerSm;
-  const int64_t units = capacity <= kUnit ? 1 : (capacity + kUnit - 1) / kUnit;
+  const int64_t units = capacity <= kWhole * kTile ? 1 : (capacity + kTile - 1) / kTile;
   const int64_t items = B * kv_heads * a.head_blocks;
   const int64_t most = (int64_t)num_sms() * per_sm;
   a.ctas = (int)(items > most / units ? most : items * units);
   a.cut = units > 1;
+  a.slot_heads = group < 8 * a.nt ? group : 8 * a.nt;
   return a;
 }
 
@@ -954,9 +1172,10 @@ cudaError_t run_attn(KvAttn p, const AttnPlan& a, cudaStream_t stream) {
   const cudaError_t e =
       tma ? go(kv_attn_kernel<DP, NT, FP8, BF16, true>) : go(kv_attn_kernel<DP, NT, FP8, BF16, false>);
   if (e != cudaSuccess || !a.cut) return e;
-  // programmatic launch: its blocks are resident by the time the partials are written
-  return launch(kv_attn_join_kernel<DP, NT, BF16>, dim3(a.ctas, p.group < 8 * NT ? p.group : 8 * NT), kJoinThreads, 0,
-                stream, true, p);
+  const int items = p.B * p.c.kv_heads * p.head_blocks;
+  const int64_t pairs = (int64_t)items * p.slot_heads;
+  if (pairs <= 4 * num_sms()) return launch(kv_attn_join_kernel<DP, NT, BF16, 1>, dim3(pairs, DP / 32), 256, 0, stream, true, p, items);
+  return launch(kv_attn_join_kernel<DP, NT, BF16, 4>, dim3((pairs + 3) / 4), 128, 0, stream, true, p, items);
 }
 
 template <int DP, int NT>
@@ -1004,13 +1223,16 @@ cudaError_t launch_kv_read(const KvCache& c, const int64_t* slots, int T, void* 
 #undef NSQ_KV_GO
 }
 
-// Workspace: per CTA two partial slots ([heads][head_dim + 4] fp32 each: two
-// maxima, the denominator, a pad, the accumulator), then one int4: the item
-// that the CTA opens without closing it (or -1), its slot, the closing CTA.
+// Workspace: per worker two partial slots ([heads][head_dim + 4] fp32 each: two
+// references, the denominator, a pad, the accumulator), then one int4 per item:
+// its partials (-1: not cut), the first one's slot, and the worker of that slot.
+static size_t attn_slot_bytes(const AttnPlan& a) {
+  return (size_t)a.ctas * kAttnWarps * 2 * a.slot_heads * (a.dp + 4) * sizeof(float);
+}
+
 size_t kv_attn_workspace(int64_t B, int group, int kv_heads, int head_dim, int64_t capacity) {
   const AttnPlan a = attn_plan(B, group, kv_heads, head_dim, capacity);
-  if (!a.cut) return 0;
-  return (size_t)a.ctas * (2 * (size_t)8 * a.nt * (a.dp + 4) * 4 + sizeof(int4));
+  return a.cut ? attn_slot_bytes(a) + (size_t)B * kv_heads * a.head_blocks * sizeof(int4) : 0;
 }
 
 cudaError_t launch_kv_attn(const KvAttnArgs& args, bool fp8, bool bf16, void* ws, cudaStream_t stream) {
@@ -1021,9 +1243,10 @@ cudaError_t launch_kv_attn(const KvAttnArgs& args, bool fp8, bool bf16, void* ws
   p.head_blocks = a.head_blocks;
   p.page_div = make_fastdiv((uint32_t)args.c.page_size);
   p.scale_log2 = args.scale * 1.4426950408889634f;
-  const size_t slots = (size_t)a.ctas * 2 * 8 * a.nt * (a.dp + 4) * sizeof(float);
+  p.slot_heads = a.slot_heads;
+  p.least = a.cut ? 2 : 1;
   p.partial = a.cut ? static_cast<float*>(ws) : nullptr;
-  p.meta = a.cut ? reinterpret_cast<int4*>(static_cast<uint8_t*>(ws) + slots) : nullptr;
+  p.meta = a.cut ? reinterpret_cast<int4*>(static_cast<uint8_t*>(ws) + attn_slot_bytes(a)) : nullptr;
   p.status = device_status_ptr();
   p.pdl = pdl_enabled();
   if (a.dp == 64) return a.nt == 1 ? run_attn_t<64, 1>(p, a, fp8, bf16, stream) : run_attn_t<64, 2>(p, a, fp8, bf16, stream);

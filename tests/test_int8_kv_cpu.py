@@ -87,12 +87,12 @@ def test_cache_call_refusals():
 
 def test_attention_workspace_size():
     size = _lib.load().nsq_kv_attention_workspace_size
-    assert size(4, 8, 2, 64, 16, 4) == 0  # 64 tokens at most: no item is cut
-    assert size(4, 8, 2, 64, 16, 5) > 0
+    assert size(4, 8, 2, 64, 16, 8) == 0  # 128 tokens at most: no item is cut
+    assert size(4, 8, 2, 64, 16, 9) > 0
     assert size(0, 8, 2, 64, 16, 5) == 0
     # bounded by the machine, not by the batch or the length
-    assert size(4096, 64, 8, 128, 16, 8192) <= 512 * 2 * (8 * 132 * 4 + 16)
-    assert size(1, 12, 1, 128, 16, 65536) <= 512 * 2 * (16 * 132 * 4 + 16)
+    assert size(4096, 64, 8, 128, 16, 8192) <= 2400 * 2 * (8 * 132 * 4 + 16)
+    assert size(1, 12, 1, 128, 16, 65536) <= 2400 * 2 * (16 * 132 * 4 + 16)
 
 
 def test_ops_refuse_cpu_tensors():
