@@ -242,7 +242,8 @@ int nsq_int8_linear_quantized(const int8_t* codes, const float* scale, int64_t M
  *   value = code * scale
  * (scales are >= 0; a row with a NaN or an infinity reads back as NaN).
  * Strides are in elements, in the order page, token, head; head_dim is
- * contiguous, so token-major and head-major pools both fit. Code strides are
+ * contiguous, so token-major and head-major pools both fit; strides are below
+ * 2^32 (one of a dimension of size 1 is not looked at). Code strides are
  * multiples of 16, code pointers 16-byte aligned, head_dim a multiple of 16 up
  * to 256, num_pages * page_size < 2^31.
  *
@@ -271,8 +272,9 @@ typedef struct nsq_kv_cache {
  * token and is skipped. Places that no slot names stay as they were. Slots are
  * distinct: of two tokens with the same slot the stored row is unspecified.
  */
-int nsq_kv_cache_write(const nsq_kv_cache* cache, const void* k, const void* v, int x_dtype, const int64_t* k_stride,
-                       const int64_t* v_stride, int64_t T, const int64_t* slots, void* stream);
+int nsq_kv_cache_write(const nsq_kv_cache* cache, const void* k, const void* v, int x_dtype, int64_t k_token_stride,
+                       int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int64_t T,
+                       const int64_t* slots, void* stream);
 
 /* Read rows back as F16 or BF16: k, v [T, kv_heads, head_dim] contiguous,
  * code * scale rounded once; zeros where a slot is negative. */
@@ -297,8 +299,8 @@ int nsq_kv_cache_read(const nsq_kv_cache* cache, const int64_t* slots, int64_t T
  */
 size_t nsq_kv_attention_workspace_size(int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                                        int64_t table_width);
-int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, const int64_t* q_stride, int64_t B,
-                            int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, int64_t q_seq_stride,
+                            int64_t q_head_stride, int64_t B, int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
                             const int32_t* seq_lens, float softmax_scale, void* out, float* lse, void* workspace,
                             size_t workspace_bytes, void* stream);
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -38,16 +39,10 @@ KV_INT8 = 0
 KV_FP8 = 1
 
 
-class KvCacheDesc(ctypes.Structure):
-    """struct nsq_kv_cache of include/nsq.h."""
-    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
-                ("num_pages", c_int64), ("page_size", c_int64), ("kv_heads", c_int64), ("head_dim", c_int64),
-                ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3),
-                ("k_scale_stride", c_int64 * 3), ("v_scale_stride", c_int64 * 3), ("codes", c_int)]
-
-
-_KV = ctypes.POINTER(KvCacheDesc)
-_I64S = ctypes.POINTER(c_int64)
+# struct nsq_kv_cache of include/nsq.h: four pointers; pages, page_size, kv_heads,
+# head_dim; page, token and head strides of k, v and their scales; the code type.
+# Packed bytes are what the calls take (cheaper than a ctypes.Structure).
+KV_CACHE = struct.Struct("@4P16qi4x")
 
 # name -> (restype, argtypes); the complete exported surface of include/nsq.h
 SIGNATURES = {
@@ -84,11 +79,12 @@ SIGNATURES = {
                                 c_void_p, c_void_p, c_size_t, c_void_p]),
     "nsq_int8_linear_quantized": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                           c_int, c_void_p, c_int, c_void_p]),
-    "nsq_kv_cache_write": (c_int, [_KV, c_void_p, c_void_p, c_int, _I64S, _I64S, c_int64, c_void_p, c_void_p]),
-    "nsq_kv_cache_read": (c_int, [_KV, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
+    "nsq_kv_cache_write": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                   c_void_p, c_void_p]),
+    "nsq_kv_cache_read": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
     "nsq_kv_attention_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64]),
-    "nsq_kv_attention_decode": (c_int, [_KV, c_void_p, c_int, _I64S, c_int64, c_int64, c_void_p, c_int64, c_int64,
-                                        c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "nsq_kv_attention_decode": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                        c_int64, c_int64, c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "nsq_set_pdl": (c_int, [c_int]),
     "nsq_set_wait_limit_ns": (c_int, [ctypes.c_uint64]),
     "nsq_set_sm_reserve": (c_int, [c_int]),

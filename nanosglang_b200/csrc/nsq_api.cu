@@ -689,26 +689,24 @@ static int kv_check(const nsq_kv_cache* c, KvCache* out) {
   if (c->head_dim % 16 != 0 || c->head_dim > 256) return NSQ_ENOTSUP;
   if (c->num_pages > kIntMax / c->page_size || c->kv_heads > kIntMax) return NSQ_ENOTSUP;
   if (!aligned16(c->k) || !aligned16(c->v)) return NSQ_EALIGN;
-  for (int i = 0; i < 3; ++i) {
-    if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_scale_stride[i] < 0 || c->v_scale_stride[i] < 0) {
-      return NSQ_EINVAL;
-    }
-    // 32-bit strides: a page, token or head is less than 4 G elements from the next
-    if (c->k_stride[i] >> 32 || c->v_stride[i] >> 32 || c->k_scale_stride[i] >> 32 || c->v_scale_stride[i] >> 32) {
-      return NSQ_ENOTSUP;
-    }
-    if (c->k_stride[i] % 16 != 0 || c->v_stride[i] % 16 != 0) return NSQ_EALIGN;
-  }
   KvCache r{};
   r.k = static_cast<uint8_t*>(c->k);
   r.v = static_cast<uint8_t*>(c->v);
   r.ks = c->k_scale;
   r.vs = c->v_scale;
+  const int64_t sizes[3] = {c->num_pages, c->page_size, c->kv_heads};
   for (int i = 0; i < 3; ++i) {
-    r.k_stride[i] = c->k_stride[i];
-    r.v_stride[i] = c->v_stride[i];
-    r.ks_stride[i] = c->k_scale_stride[i];
-    r.vs_stride[i] = c->v_scale_stride[i];
+    const int64_t given[4] = {c->k_stride[i], c->v_stride[i], c->k_scale_stride[i], c->v_scale_stride[i]};
+    int64_t* const take[4] = {&r.k_stride[i], &r.v_stride[i], &r.ks_stride[i], &r.vs_stride[i]};
+    for (int j = 0; j < 4; ++j) {
+      *take[j] = 0;
+      if (sizes[i] == 1) continue;
+      if (given[j] < 0) return NSQ_EINVAL;
+      // 32-bit strides: a page, token or head is less than 4 G elements from the next
+      if (given[j] >> 32) return NSQ_ENOTSUP;
+      if (j < 2 && given[j] % 16 != 0) return NSQ_EALIGN;
+      *take[j] = given[j];
+    }
   }
   r.num_pages = (int)c->num_pages;
   r.page_size = (int)c->page_size;
@@ -718,16 +716,19 @@ static int kv_check(const nsq_kv_cache* c, KvCache* out) {
   return NSQ_OK;
 }
 
-int nsq_kv_cache_write(const nsq_kv_cache* cache, const void* k, const void* v, int x_dtype, const int64_t* k_stride,
-                       const int64_t* v_stride, int64_t T, const int64_t* slots, void* stream) {
+int nsq_kv_cache_write(const nsq_kv_cache* cache, const void* k, const void* v, int x_dtype, int64_t k_token_stride,
+                       int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int64_t T,
+                       const int64_t* slots, void* stream) {
   KvCache c;
   int rc = kv_check(cache, &c);
   if (rc != NSQ_OK) return rc;
-  if (T < 0 || !valid_act_dtype(x_dtype) || !k_stride || !v_stride) return NSQ_EINVAL;
+  if (T < 0 || !valid_act_dtype(x_dtype)) return NSQ_EINVAL;
   if (T > ((int64_t)1 << 30) / c.kv_heads) return NSQ_ENOTSUP;
   if (T == 0) return NSQ_OK;
   if (!k || !v || !slots) return NSQ_EINVAL;
   if (!aligned16(k) || !aligned16(v)) return NSQ_EALIGN;
+  const int64_t k_stride[2] = {T == 1 ? 0 : k_token_stride, c.kv_heads == 1 ? 0 : k_head_stride};
+  const int64_t v_stride[2] = {T == 1 ? 0 : v_token_stride, c.kv_heads == 1 ? 0 : v_head_stride};
   for (int i = 0; i < 2; ++i) {
     if (k_stride[i] < 0 || v_stride[i] < 0) return NSQ_EINVAL;
     if (k_stride[i] % 8 != 0 || v_stride[i] % 8 != 0) return NSQ_EALIGN;
@@ -773,8 +774,8 @@ size_t nsq_kv_attention_workspace_size(int64_t B, int64_t H, int64_t kv_heads, i
   return kv_attn_workspace(B, (int)(H / kv_heads), (int)kv_heads, (int)head_dim, table_width * page_size);
 }
 
-int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, const int64_t* q_stride, int64_t B,
-                            int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, int64_t q_seq_stride,
+                            int64_t q_head_stride, int64_t B, int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
                             const int32_t* seq_lens, float softmax_scale, void* out, float* lse, void* workspace,
                             size_t workspace_bytes, void* stream) {
   KvAttnArgs a{};
@@ -782,10 +783,11 @@ int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtyp
   if (rc != NSQ_OK) return rc;
   rc = kv_attn_check(B, H, a.c.kv_heads, a.c.head_dim, a.c.page_size, table_width);
   if (rc != NSQ_OK) return rc;
-  if (!valid_act_dtype(q_dtype) || !q_stride || table_stride < 0) return NSQ_EINVAL;
+  if (!valid_act_dtype(q_dtype) || table_stride < 0) return NSQ_EINVAL;
   if (!(softmax_scale - softmax_scale == 0.f)) return NSQ_EINVAL;  // NaN or infinite
   if (B == 0) return NSQ_OK;
   if (!q || !out || !seq_lens || (table_width > 0 && !page_table)) return NSQ_EINVAL;
+  const int64_t q_stride[2] = {B == 1 ? 0 : q_seq_stride, H == 1 ? 0 : q_head_stride};
   if (q_stride[0] < 0 || q_stride[1] < 0) return NSQ_EINVAL;
   if (!aligned16(q) || !aligned16(out) || q_stride[0] % 8 != 0 || q_stride[1] % 8 != 0) return NSQ_EALIGN;
   if ((rc = check_device()) != NSQ_OK) return rc;

@@ -1174,7 +1174,9 @@ cudaError_t run_attn(KvAttn p, const AttnPlan& a, cudaStream_t stream) {
   if (e != cudaSuccess || !a.cut) return e;
   const int items = p.B * p.c.kv_heads * p.head_blocks;
   const int64_t pairs = (int64_t)items * p.slot_heads;
-  if (pairs <= 4 * num_sms()) return launch(kv_attn_join_kernel<DP, NT, BF16, 1>, dim3(pairs, DP / 32), 256, 0, stream, true, p, items);
+  // more than 16 partials an item on average: blocks for 32 dims of a pair
+  if ((int64_t)items * 16 < (int64_t)a.ctas * kAttnWarps) return launch(kv_attn_join_kernel<DP, NT, BF16, 1>, dim3(pairs, DP / 32), 256, 0,
+                                                                        stream, true, p, items);
   return launch(kv_attn_join_kernel<DP, NT, BF16, 4>, dim3((pairs + 3) / 4), 128, 0, stream, true, p, items);
 }
 

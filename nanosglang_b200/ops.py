@@ -10,7 +10,6 @@ raise: there is no CPU path.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional
 
@@ -297,18 +296,36 @@ def fp8_quantize(weight: torch.Tensor):
 # int8 linear (W8A8: int8 codes with one scale per token and output channel)
 # ---------------------------------------------------------------------------
 
-_NO_GUARD = contextlib.nullcontext()
+try:  # the current device without torch.cuda's initialisation checks (hot path)
+    _current_device = torch._C._cuda_getDevice
+except AttributeError:  # pragma: no cover - builds of torch without CUDA
+    _current_device = torch.cuda.current_device
 
 
-def _on_device(*ts, what: str):
-    """Checks that every tensor is on one CUDA device and returns the context
-    in which its kernels launch (that device made current where it is not)."""
-    _require_cuda(*ts, what=what)
-    dev = ts[0].device
+def _device_of(what: str, *ts) -> int:
+    """The index of the one CUDA device that holds every tensor; raises otherwise."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t.get_device() != dev or dev < 0:
+            _require_cuda(*ts, what=what)
+            raise RuntimeError(f"{what}: tensors on {ts[0].device} and {t.device}")
+    return dev
+
+
+def _call(dev: int, name: str, *args) -> None:
+    """Runs an entry point on device ``dev`` (made current where it is not)."""
+    fn = getattr(_lib.load(), name)
+    if dev == _current_device():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc:
+        _lib.check(rc, name)
+
+
+def _stream_on(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 def int8_quantize(x: torch.Tensor):
@@ -316,38 +333,40 @@ def int8_quantize(x: torch.Tensor):
     activations per token): scale = max|row| / 127 (1 if that is 0), codes =
     rint(row / scale). x: [..., K] float16, bfloat16 or float32. Returns
     (codes int8 [..., K], scale float32 [...])."""
-    guard = _on_device(x, what="int8_quantize")
-    if x.dtype not in _BIAS_CODES:
+    dev = _device_of("int8_quantize", x)
+    code = _BIAS_CODES.get(x.dtype)
+    if code is None:
         raise TypeError(f"dtype {x.dtype} not supported (float16 / bfloat16 / float32)")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"int8_quantize needs rows of at least one element, got shape {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"int8_quantize needs rows of at least one element, got shape {tuple(shape)}")
     x = x.contiguous()
-    k = x.shape[-1]
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with guard:
-        rc = _lib.load().nsq_int8_quantize(_ptr(x), _BIAS_CODES[x.dtype], x.numel() // k, k, _ptr(codes), _ptr(scale),
-                                           _stream(x))
-    _lib.check(rc, "nsq_int8_quantize")
+    k = shape[-1]
+    codes = x.new_empty(shape, dtype=torch.int8)
+    scale = x.new_empty(shape[:-1], dtype=torch.float32)
+    _call(dev, "nsq_int8_quantize", x.data_ptr(), code, x.numel() // k, k, codes.data_ptr(), scale.data_ptr(),
+          _stream_on(dev))
     return codes, scale
 
 
-def _int8_weight(weight_int8: torch.Tensor, weight_scale: torch.Tensor):
+def _int8_operands(weight_int8: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor]):
+    """Checks an int8 layer: (weight, weight_scale, N, K, bias or None, its dtype code)."""
     if weight_int8.dtype != torch.int8 or weight_int8.dim() != 2:
         raise TypeError(f"int8 weight must be int8 [N, K], got {weight_int8.dtype} {tuple(weight_int8.shape)}")
     n, k = weight_int8.shape
     if weight_scale.dtype != torch.float32 or weight_scale.numel() != n:
         raise TypeError(f"weight_scale must be float32 with one value per output channel ({n}), "
                         f"got {weight_scale.dtype} {tuple(weight_scale.shape)}")
-    return _aligned(weight_int8), weight_scale.contiguous(), n, k
-
-
-def _int8_bias(bias: Optional[torch.Tensor], n: int):
+    if not weight_int8.is_contiguous() or weight_int8.data_ptr() & 15:
+        weight_int8 = _aligned(weight_int8)
+    if not weight_scale.is_contiguous():
+        weight_scale = weight_scale.contiguous()
     if bias is None:
-        return None, _lib.DTYPE_NONE
+        return weight_int8, weight_scale, n, k, None, _lib.DTYPE_NONE
     if bias.numel() != n:
         raise ValueError(f"bias has {bias.numel()} elements, the layer has {n} outputs")
-    return _bias_arg(bias)
+    bias, code = _bias_arg(bias)
+    return weight_int8, weight_scale, n, k, bias, code
 
 
 def int8_linear(x: torch.Tensor, weight_int8: torch.Tensor, weight_scale: torch.Tensor,
@@ -360,25 +379,27 @@ def int8_linear(x: torch.Tensor, weight_int8: torch.Tensor, weight_scale: torch.
     float32 [N]; returns [..., N] in x's dtype. K must be a multiple of 16, at
     most 131072.
     """
-    guard = _on_device(x, weight_int8, weight_scale, bias, what="int8_linear")
+    if bias is None:
+        dev = _device_of("int8_linear", x, weight_int8, weight_scale)
+    else:
+        dev = _device_of("int8_linear", x, weight_int8, weight_scale, bias)
     code = _ACT_CODES.get(x.dtype)
     if code is None:
         raise TypeError(f"activation dtype {x.dtype} not supported (float16 / bfloat16)")
-    w, ws, n, k = _int8_weight(weight_int8, weight_scale)
-    if x.shape[-1] != k:
-        raise RuntimeError(f"x has {x.shape[-1]} features, the layer expects {k}")
-    x2 = _aligned(x.reshape(-1, k))
+    w, ws, n, k, b, bcode = _int8_operands(weight_int8, weight_scale, bias)
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise RuntimeError(f"x has shape {tuple(shape)}, the layer expects {k} features")
+    x2 = x if len(shape) == 2 else x.reshape(-1, k)
+    if not x2.is_contiguous() or x2.data_ptr() & 15:
+        x2 = _aligned(x2)
     m = x2.shape[0]
-    b, bcode = _int8_bias(bias, n)
-    lib = _lib.load()
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    nbytes = lib.nsq_int8_linear_workspace_size(m, k)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    with guard:
-        rc = lib.nsq_int8_linear(x2.data_ptr(), code, m, k, n, w.data_ptr(), ws.data_ptr(), _ptr(b), bcode,
-                                 y.data_ptr(), work.data_ptr(), nbytes, _stream(x))
-    _lib.check(rc, "nsq_int8_linear")
-    return y.reshape(*x.shape[:-1], n)
+    y = x2.new_empty((m, n))
+    nbytes = (m * k + 15 & ~15) + 4 * m  # nsq_int8_linear_workspace_size
+    work = x2.new_empty(nbytes, dtype=torch.uint8)
+    _call(dev, "nsq_int8_linear", x2.data_ptr(), code, m, k, n, w.data_ptr(), ws.data_ptr(),
+          None if b is None else b.data_ptr(), bcode, y.data_ptr(), work.data_ptr(), nbytes, _stream_on(dev))
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
 
 
 def int8_linear_quantized(codes: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor,
@@ -387,25 +408,27 @@ def int8_linear_quantized(codes: torch.Tensor, scale: torch.Tensor, weight_int8:
     """The product of ``int8_linear`` for activations already quantised by
     ``int8_quantize`` (once, for several layers that read the same x): codes
     int8 [..., K], scale float32 [...]; returns [..., N] in ``dtype``."""
-    guard = _on_device(codes, scale, weight_int8, weight_scale, bias, what="int8_linear_quantized")
-    if codes.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != codes.shape[:-1]:
+    if bias is None:
+        dev = _device_of("int8_linear_quantized", codes, scale, weight_int8, weight_scale)
+    else:
+        dev = _device_of("int8_linear_quantized", codes, scale, weight_int8, weight_scale, bias)
+    shape = codes.shape
+    if codes.dtype != torch.int8 or scale.dtype != torch.float32 or not shape or scale.shape != shape[:-1]:
         raise TypeError(f"codes must be int8 [..., K] with a float32 scale [...], got {codes.dtype} "
-                        f"{tuple(codes.shape)} and {scale.dtype} {tuple(scale.shape)}")
-    if dtype not in _ACT_CODES:
+                        f"{tuple(shape)} and {scale.dtype} {tuple(scale.shape)}")
+    code = _ACT_CODES.get(dtype)
+    if code is None:
         raise TypeError(f"output dtype {dtype} not supported (float16 / bfloat16)")
-    w, ws, n, k = _int8_weight(weight_int8, weight_scale)
-    if codes.shape[-1] != k:
-        raise RuntimeError(f"codes have {codes.shape[-1]} features, the layer expects {k}")
+    w, ws, n, k, b, bcode = _int8_operands(weight_int8, weight_scale, bias)
+    if shape[-1] != k:
+        raise RuntimeError(f"codes have {shape[-1]} features, the layer expects {k}")
     c2 = _aligned(codes.reshape(-1, k))
     s2 = scale.reshape(-1).contiguous()
     m = c2.shape[0]
-    b, bcode = _int8_bias(bias, n)
-    y = torch.empty((m, n), dtype=dtype, device=codes.device)
-    with guard:
-        rc = _lib.load().nsq_int8_linear_quantized(c2.data_ptr(), s2.data_ptr(), m, k, n, w.data_ptr(), ws.data_ptr(),
-                                                   _ptr(b), bcode, y.data_ptr(), _ACT_CODES[dtype], _stream(codes))
-    _lib.check(rc, "nsq_int8_linear_quantized")
-    return y.reshape(*codes.shape[:-1], n)
+    y = codes.new_empty((m, n), dtype=dtype)
+    _call(dev, "nsq_int8_linear_quantized", c2.data_ptr(), s2.data_ptr(), m, k, n, w.data_ptr(), ws.data_ptr(),
+          None if b is None else b.data_ptr(), bcode, y.data_ptr(), code, _stream_on(dev))
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
 
 
 # ---------------------------------------------------------------------------
@@ -415,41 +438,37 @@ def int8_linear_quantized(codes: torch.Tensor, scale: torch.Tensor, weight_int8:
 _KV_CODES = {torch.int8: _lib.KV_INT8, torch.float8_e4m3fn: _lib.KV_FP8}
 
 
-def _strides(t: torch.Tensor, dims: int):
-    """The strides of the first dims dimensions, 0 for those of size 1 (whose stride says nothing)."""
-    return (ctypes.c_int64 * dims)(*[0 if t.shape[i] == 1 else t.stride(i) for i in range(dims)])
-
-
-def _kv_desc(k_cache, v_cache, k_scale, v_scale, what: str) -> "_lib.KvCacheDesc":
-    """Checks the four tensors of a cache and describes them to the library."""
+def _kv_desc(k_cache, v_cache, k_scale, v_scale, what: str):
+    """Checks the four tensors of a cache; returns the packed struct nsq_kv_cache and the cache's shape."""
     code = _KV_CODES.get(k_cache.dtype)
     if code is None or v_cache.dtype != k_cache.dtype:
         raise TypeError(f"{what}: caches must both be int8 or both float8_e4m3fn, got {k_cache.dtype} "
                         f"and {v_cache.dtype}")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"{what}: caches must be [pages, page_size, kv_heads, head_dim] of one shape, got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.shape != k_cache.shape[:3]:
-            raise ValueError(f"{what}: scales must be float32 {tuple(k_cache.shape[:3])}, got {s.dtype} "
-                             f"{tuple(s.shape)}")
-    pages, page, heads, dim = k_cache.shape
-    for c in (k_cache, v_cache):
-        if dim > 1 and c.stride(3) != 1:
-            raise ValueError(f"{what}: head_dim must be contiguous in the caches")
-    return _lib.KvCacheDesc(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
-                            page, heads, dim, _strides(k_cache, 3), _strides(v_cache, 3), _strides(k_scale, 3),
-                            _strides(v_scale, 3), code)
+                         f"{tuple(shape)} and {tuple(v_cache.shape)}")
+    rows = shape[:3]
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != rows or (
+            v_scale.shape != rows):
+        raise ValueError(f"{what}: scales must be float32 {tuple(rows)}, got {k_scale.dtype} {tuple(k_scale.shape)} "
+                         f"and {v_scale.dtype} {tuple(v_scale.shape)}")
+    k0, k1, k2, kd = k_cache.stride()
+    v0, v1, v2, vd = v_cache.stride()
+    if (kd != 1 or vd != 1) and shape[3] > 1:
+        raise ValueError(f"{what}: head_dim must be contiguous in the caches")
+    return _lib.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *shape,
+                              k0, k1, k2, v0, v1, v2, *k_scale.stride(), *v_scale.stride(), code), shape
 
 
 def _kv_rows(t: torch.Tensor):
-    """[T, heads, head_dim] with 16-byte aligned rows of contiguous head_dim (a copy only where needed)."""
-    if t.stride(2) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and (t.stride(i) % 8 or t.stride(i) < 0)
-                                                    for i in (0, 1)):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
+    """[T, heads, head_dim] with 16-byte aligned rows of contiguous head_dim (a
+    copy only where needed), and its token and head strides."""
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or t.data_ptr() & 15 or (s0 & 7 and t.shape[0] > 1) or (s1 & 7 and t.shape[1] > 1):
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, _ = t.stride()
+    return t, s0, s1
 
 
 def _slots_arg(slots: torch.Tensor, what: str) -> torch.Tensor:
@@ -473,21 +492,20 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     max|row| / 127 (int8) or / 448 (float8), 1 where that is 0; codes are the
     nearest to row / scale. A row with a NaN or an infinity reads back as NaN.
     """
-    what = "kv_cache_write"
-    guard = _on_device(k, v, k_cache, v_cache, k_scale, v_scale, slots, what=what)
-    if k.dtype not in _ACT_CODES or v.dtype != k.dtype:
-        raise TypeError(f"{what}: k and v must both be float16 or both bfloat16, got {k.dtype} and {v.dtype}")
-    desc = _kv_desc(k_cache, v_cache, k_scale, v_scale, what)
-    slots = _slots_arg(slots, what)
-    shape = (slots.shape[0],) + tuple(k_cache.shape[2:])
-    if tuple(k.shape) != shape or tuple(v.shape) != shape:
-        raise ValueError(f"{what}: k and v must be {shape}, got {tuple(k.shape)} and {tuple(v.shape)}")
-    k, v = _kv_rows(k), _kv_rows(v)
-    with guard:
-        rc = _lib.load().nsq_kv_cache_write(ctypes.byref(desc), k.data_ptr(), v.data_ptr(), _ACT_CODES[k.dtype],
-                                            _strides(k, 2), _strides(v, 2), shape[0], slots.data_ptr(),
-                                            _stream(k_cache))
-    _lib.check(rc, "nsq_kv_cache_write")
+    dev = _device_of("kv_cache_write", k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    code = _ACT_CODES.get(k.dtype)
+    if code is None or v.dtype != k.dtype:
+        raise TypeError(f"kv_cache_write: k and v must both be float16 or both bfloat16, got {k.dtype} and {v.dtype}")
+    desc, (_, _, heads, dim) = _kv_desc(k_cache, v_cache, k_scale, v_scale, "kv_cache_write")
+    slots = _slots_arg(slots, "kv_cache_write")
+    n = slots.shape[0]
+    if k.shape != (n, heads, dim) or v.shape != (n, heads, dim):
+        raise ValueError(f"kv_cache_write: k and v must be {(n, heads, dim)}, got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    k, kt, kh = _kv_rows(k)
+    v, vt, vh = _kv_rows(v)
+    _call(dev, "nsq_kv_cache_write", desc, k.data_ptr(), v.data_ptr(), code, kt, kh, vt, vh, n, slots.data_ptr(),
+          _stream_on(dev))
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -495,18 +513,16 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
     """The rows at ``slots`` (int64 [T]) of an 8-bit cache, as (k, v)
     [T, kv_heads, head_dim] in ``dtype`` (float16 or bfloat16): code * scale,
     rounded once; zeros where a slot is negative."""
-    what = "kv_cache_read"
-    guard = _on_device(k_cache, v_cache, k_scale, v_scale, slots, what=what)
-    if dtype not in _ACT_CODES:
-        raise TypeError(f"{what}: dtype {dtype} not supported (float16 / bfloat16)")
-    desc = _kv_desc(k_cache, v_cache, k_scale, v_scale, what)
-    slots = _slots_arg(slots, what)
-    k = torch.empty((slots.shape[0],) + tuple(k_cache.shape[2:]), dtype=dtype, device=k_cache.device)
-    v = torch.empty_like(k)
-    with guard:
-        rc = _lib.load().nsq_kv_cache_read(ctypes.byref(desc), slots.data_ptr(), slots.shape[0], k.data_ptr(),
-                                           v.data_ptr(), _ACT_CODES[dtype], _stream(k_cache))
-    _lib.check(rc, "nsq_kv_cache_read")
+    dev = _device_of("kv_cache_read", k_cache, v_cache, k_scale, v_scale, slots)
+    code = _ACT_CODES.get(dtype)
+    if code is None:
+        raise TypeError(f"kv_cache_read: dtype {dtype} not supported (float16 / bfloat16)")
+    desc, (_, _, heads, dim) = _kv_desc(k_cache, v_cache, k_scale, v_scale, "kv_cache_read")
+    slots = _slots_arg(slots, "kv_cache_read")
+    n = slots.shape[0]
+    k = k_scale.new_empty((n, heads, dim), dtype=dtype)
+    v = k_scale.new_empty((n, heads, dim), dtype=dtype)
+    _call(dev, "nsq_kv_cache_read", desc, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code, _stream_on(dev))
     return k, v
 
 
@@ -526,36 +542,37 @@ def kv_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     word: that page's tokens are left out, the length is clamped.
     """
     what = "kv_attention_decode"
-    guard = _on_device(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, what=what)
+    dev = _device_of(what, q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens)
     code = _ACT_CODES.get(q.dtype)
     if code is None:
         raise TypeError(f"{what}: query dtype {q.dtype} not supported (float16 / bfloat16)")
-    desc = _kv_desc(k_cache, v_cache, k_scale, v_scale, what)
-    if q.dim() != 3 or q.shape[2] != desc.head_dim or q.shape[1] == 0 or q.shape[1] % desc.kv_heads:
-        raise ValueError(f"{what}: q must be [B, heads, {desc.head_dim}] with heads a multiple of {desc.kv_heads}, "
-                         f"got {tuple(q.shape)}")
-    b, h, d = q.shape
+    desc, (_, page, heads, dim) = _kv_desc(k_cache, v_cache, k_scale, v_scale, what)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != dim or shape[1] == 0 or heads == 0 or shape[1] % heads:
+        raise ValueError(f"{what}: q must be [B, heads, {dim}] with heads a multiple of {heads}, got {tuple(shape)}")
+    b, h, _ = shape
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b:
         raise TypeError(f"{what}: page_table must be int32 [{b}, W], got {page_table.dtype} {tuple(page_table.shape)}")
-    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (b,):
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (b,):
         raise TypeError(f"{what}: seq_lens must be int32 [{b}], got {seq_lens.dtype} {tuple(seq_lens.shape)}")
-    q = _kv_rows(q)
+    q, qs, qh = _kv_rows(q)
     width = page_table.shape[1]
     if page_table.stride(1) != 1 and width > 1:
         page_table = page_table.contiguous()
-    seq_lens = seq_lens.contiguous()
-    lib = _lib.load()
-    out = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, h), dtype=torch.float32, device=q.device) if return_lse else None
-    with guard:
-        nbytes = lib.nsq_kv_attention_workspace_size(b, h, desc.kv_heads, d, desc.page_size, width)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        rc = lib.nsq_kv_attention_decode(ctypes.byref(desc), q.data_ptr(), code, _strides(q, 2), b, h,
-                                         page_table.data_ptr(), page_table.stride(0) if b > 1 else 0, width,
-                                         seq_lens.data_ptr(),
-                                         d ** -0.5 if softmax_scale is None else softmax_scale, out.data_ptr(),
-                                         _ptr(lse), _ptr(work), nbytes, _stream(q))
-    _lib.check(rc, "nsq_kv_attention_decode")
+    if not seq_lens.is_contiguous():
+        seq_lens = seq_lens.contiguous()
+    out = q.new_empty(shape)
+    lse = q.new_empty((b, h), dtype=torch.float32) if return_lse else None
+    if dev == _current_device():
+        nbytes = _lib.load().nsq_kv_attention_workspace_size(b, h, heads, dim, page, width)
+    else:
+        with torch.cuda.device(dev):
+            nbytes = _lib.load().nsq_kv_attention_workspace_size(b, h, heads, dim, page, width)
+    work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call(dev, "nsq_kv_attention_decode", desc, q.data_ptr(), code, qs, qh, b, h, page_table.data_ptr(),
+          page_table.stride(0) if b > 1 else 0, width, seq_lens.data_ptr(),
+          dim ** -0.5 if softmax_scale is None else softmax_scale, out.data_ptr(),
+          None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), nbytes, _stream_on(dev))
     return (out, lse) if return_lse else out
 
 
@@ -572,7 +589,6 @@ def _unwrap(mod):
 
 
 def _ptr_array(vals, ctype=None):
-    import ctypes
     arr = (ctypes.c_void_p * len(vals))(*vals) if ctype is None else (ctype * len(vals))(*vals)
     return arr
 
@@ -582,7 +598,6 @@ def linear_multi(x: torch.Tensor, mods) -> Optional[list]:
     same x, e.g. q/k/v. Returns their outputs as views of one [M, sum N]
     buffer, or None when the fused kernel does not apply (M > 32, mixed
     formats, bias dtypes that differ, group sizes that differ)."""
-    import ctypes
     mods = [_unwrap(m) for m in mods]
     kinds = {type(m).__name__ for m in mods}
     if len(kinds) != 1 or x.dtype not in _ACT_CODES:

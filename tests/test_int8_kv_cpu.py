@@ -1,8 +1,6 @@
 """Host-side checks of the int8 linear and the 8-bit key/value cache that need
 no GPU: every refusal comes before any device access."""
 
-import ctypes
-
 import pytest
 import torch
 
@@ -36,47 +34,43 @@ def test_int8_linear_refusals():
 
 
 def _desc(**kw):
-    s3 = ctypes.c_int64 * 3
     d = dict(k=FAKE, v=FAKE, k_scale=FAKE, v_scale=FAKE, num_pages=8, page_size=16, kv_heads=2, head_dim=64,
-             k_stride=s3(2048, 128, 64), v_stride=s3(2048, 128, 64), k_scale_stride=s3(32, 2, 1),
-             v_scale_stride=s3(32, 2, 1), codes=0)
+             k_stride=(2048, 128, 64), v_stride=(2048, 128, 64), k_scale_stride=(32, 2, 1),
+             v_scale_stride=(32, 2, 1), codes=0)
     d.update(kw)
-    out = _lib.KvCacheDesc()
-    for name, value in d.items():
-        setattr(out, name, value)
-    return out
+    flat = [x for v in d.values() for x in (v if isinstance(v, tuple) else (v,))]
+    return _lib.KV_CACHE.pack(*flat)
 
 
 @pytest.mark.parametrize("change,expect", [
-    ({"codes": 2}, _lib.EINVAL), ({"k": None}, _lib.EINVAL), ({"num_pages": 0}, _lib.EINVAL),
+    ({"codes": 2}, _lib.EINVAL), ({"k": 0}, _lib.EINVAL), ({"num_pages": 0}, _lib.EINVAL),
     ({"head_dim": 72}, _lib.ENOTSUP), ({"head_dim": 272}, _lib.ENOTSUP), ({"num_pages": 1 << 28}, _lib.ENOTSUP),
-    ({"v": FAKE + 8}, _lib.EALIGN), ({"k_stride": (ctypes.c_int64 * 3)(2048, 136, 64)}, _lib.EALIGN),
-    ({"v_scale_stride": (ctypes.c_int64 * 3)(-1, 1, 1)}, _lib.EINVAL)])
+    ({"v": FAKE + 8}, _lib.EALIGN), ({"k_stride": (2048, 136, 64)}, _lib.EALIGN),
+    ({"k_stride": (1 << 32, 128, 64)}, _lib.ENOTSUP), ({"v_scale_stride": (-1, 1, 1)}, _lib.EINVAL)])
 def test_cache_descriptor_refusals(change, expect):
     lib = _lib.load()
-    s2 = (ctypes.c_int64 * 2)(128, 64)
     d = _desc(**change)
-    assert lib.nsq_kv_cache_write(ctypes.byref(d), FAKE, FAKE, 1, s2, s2, 4, FAKE, None) == expect
-    assert lib.nsq_kv_cache_read(ctypes.byref(d), FAKE, 4, FAKE, FAKE, 1, None) == expect
-    assert lib.nsq_kv_attention_decode(ctypes.byref(d), FAKE, 1, s2, 2, 4, FAKE, 4, 4, FAKE, 0.125, FAKE, None, FAKE,
-                                       1 << 30, None) == expect
+    assert lib.nsq_kv_cache_write(d, FAKE, FAKE, 1, 128, 64, 128, 64, 4, FAKE, None) == expect
+    assert lib.nsq_kv_cache_read(d, FAKE, 4, FAKE, FAKE, 1, None) == expect
+    assert lib.nsq_kv_attention_decode(d, FAKE, 1, 128, 64, 2, 4, FAKE, 4, 4, FAKE, 0.125, FAKE, None, FAKE, 1 << 30,
+                                       None) == expect
 
 
 def test_cache_call_refusals():
     lib = _lib.load()
-    ok = (ctypes.c_int64 * 2)(128, 64)
-    odd = (ctypes.c_int64 * 2)(132, 64)
-    d = ctypes.byref(_desc())
-    write = lambda k=FAKE, xd=1, st=ok, t=4, sl=FAKE: lib.nsq_kv_cache_write(d, k, FAKE, xd, st, ok, t, sl, None)  # noqa: E731
+    d = _desc()
+    write = lambda k=FAKE, xd=1, st=128, t=4, sl=FAKE: lib.nsq_kv_cache_write(  # noqa: E731
+        d, k, FAKE, xd, st, 64, 128, 64, t, sl, None)
     assert write(xd=2) == _lib.EINVAL
     assert write(k=FAKE + 2) == _lib.EALIGN
-    assert write(st=odd) == _lib.EALIGN
+    assert write(st=132) == _lib.EALIGN
+    assert write(st=-128) == _lib.EINVAL
     assert write(t=-1) == _lib.EINVAL
     assert write(sl=None) == _lib.EINVAL
     assert write(t=1 << 31) == _lib.ENOTSUP
     assert write(t=0) == _lib.OK
     att = lambda q=FAKE, b=2, h=4, w=4, sc=0.125, ws=FAKE, nb=1 << 30: lib.nsq_kv_attention_decode(  # noqa: E731
-        d, q, 1, ok, b, h, FAKE, w, w, FAKE, sc, FAKE, None, ws, nb, None)
+        d, q, 1, 128, 64, b, h, FAKE, w, w, FAKE, sc, FAKE, None, ws, nb, None)
     assert att(h=3) == _lib.EINVAL  # not a multiple of kv_heads
     assert att(sc=float("nan")) == _lib.EINVAL
     assert att(sc=float("inf")) == _lib.EINVAL
