@@ -651,7 +651,7 @@ static int int8_check(int64_t M, int64_t K, int64_t N, const void* x, const int8
 }
 
 static int int8_product(const Int8Args& a, cudaStream_t stream) {
-  return a.M <= 64 ? run_int8_rows(a, stream) : run_int8_gemm(a, stream);
+  return a.M <= 64 && (int64_t)a.K * a.N < ((int64_t)1 << 24) ? run_int8_rows(a, stream) : run_int8_gemm(a, stream);
 }
 
 int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N, const int8_t* weight_int8,

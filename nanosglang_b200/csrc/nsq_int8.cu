@@ -118,6 +118,10 @@ __device__ __forceinline__ uint4 ldg_w(const int8_t* p) {
   return v;
 }
 
+__device__ __forceinline__ void dsmem_add(uint32_t cluster_addr, int v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
 struct RowsParams {
   const int8_t* x;
   const float* xscale;
@@ -128,46 +132,84 @@ struct RowsParams {
   void* y;
   int M, K, N;
   int pdl_x;  // x and xscale come from the kernel ahead
+  int split;  // CTAs of a cluster, along K
 };
 
-// 16 weight rows x 8 * MT tokens per CTA; its warps take 64-column chunks in
-// turn and add their int32 sums in shared memory (exact, so the order is free).
+// 16 weight rows x 8 * MT tokens per cluster of `split` CTAs along K. The warps
+// of all of them take 64-column chunks in turn and add their int32 sums in the
+// first CTA's shared memory (exact, so the order is free).
 template <int MT, bool BF16>
 __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParams p) {
-  __shared__ int acc_s[16][8 * MT + 1];
+  constexpr int kLd = 8 * MT + 1;
+  __shared__ int acc_s[16][kLd];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (8 * MT);
-  for (int i = threadIdx.x; i < 16 * (8 * MT + 1); i += kRWarps * 32) (&acc_s[0][0])[i] = 0;
-  if (p.pdl_x) pdl_wait_prior_grids();
+  const int rank = blockIdx.x % p.split;  // the cluster's rank along x
+  const int n0 = blockIdx.x / p.split * 16, m0 = blockIdx.y * (8 * MT);
+  for (int i = threadIdx.x; i < 16 * kLd; i += kRWarps * 32) (&acc_s[0][0])[i] = 0;
+  bool waiting = p.pdl_x;
   const int8_t* w0 = p.w + (int64_t)(n0 + g) * p.K;
   const int8_t* w1 = w0 + (int64_t)8 * p.K;
   const bool r0 = n0 + g < p.N, r1 = n0 + g + 8 < p.N;
   int d[MT][4];
 #pragma unroll
   for (int i = 0; i < MT; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0;
-#pragma unroll 2
-  for (int k = warp * 64 + t * 16; k - t * 16 < p.K; k += kRWarps * 64) {
-    const bool in = k < p.K;
+  // kAhead chunks' weights are loaded before their products: with the other
+  // warps of the SM, 64 KB and more in flight
+  constexpr int kAhead = MT <= 2 ? 4 : 2;
+  const int step = p.split * kRWarps * 64;
+  for (int k0 = (rank * kRWarps + warp) * 64; k0 < p.K; k0 += kAhead * step) {
+    uint4 a[kAhead], c[kAhead];
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    const uint4 a = in && r0 ? ldg_w(w0 + k) : zero, c = in && r1 ? ldg_w(w1 + k) : zero;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int m = m0 + 8 * i + g;
-      const uint4 b = in && m < p.M ? *reinterpret_cast<const uint4*>(p.x + (int64_t)m * p.K + k) : zero;
-      mma_16832_s8(d[i], a.x, c.x, a.y, c.y, b.x, b.y);
-      mma_16832_s8(d[i], a.z, c.z, a.w, c.w, b.z, b.w);
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = k0 + j * step + t * 16;
+      a[j] = k < p.K && r0 ? ldg_w(w0 + k) : zero;
+      c[j] = k < p.K && r1 ? ldg_w(w1 + k) : zero;
+    }
+    if (waiting) {  // the first weights are on their way while the codes of x are made
+      pdl_wait_prior_grids();
+      waiting = false;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = k0 + j * step + t * 16;
+      if (j > 0 && k0 + j * step >= p.K) break;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int m = m0 + 8 * i + g;
+        const uint4 b = k < p.K && m < p.M ? *reinterpret_cast<const uint4*>(p.x + (int64_t)m * p.K + k) : zero;
+        mma_16832_s8(d[i], a[j].x, c[j].x, a[j].y, c[j].y, b.x, b.y);
+        mma_16832_s8(d[i], a[j].z, c[j].z, a[j].w, c[j].w, b.z, b.w);
+      }
     }
   }
-  __syncthreads();
+  if (waiting) pdl_wait_prior_grids();
+  const uint32_t acc0 = smem_u32(acc_s);
+  if (p.split > 1) {
+    cluster_sync_all();  // the first CTA's sums are zero
+    const uint32_t first = dsmem_map(acc0, 0);
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    atomicAdd(&acc_s[g][8 * i + 2 * t], d[i][0]);
-    atomicAdd(&acc_s[g][8 * i + 2 * t + 1], d[i][1]);
-    atomicAdd(&acc_s[g + 8][8 * i + 2 * t], d[i][2]);
-    atomicAdd(&acc_s[g + 8][8 * i + 2 * t + 1], d[i][3]);
+    for (int i = 0; i < MT; ++i) {
+      const uint32_t at = first + (g * kLd + 8 * i + 2 * t) * 4;
+      dsmem_add(at, d[i][0]);
+      dsmem_add(at + 4, d[i][1]);
+      dsmem_add(at + 8 * kLd * 4, d[i][2]);
+      dsmem_add(at + 8 * kLd * 4 + 4, d[i][3]);
+    }
+    cluster_sync_all();  // and complete
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      atomicAdd(&acc_s[g][8 * i + 2 * t], d[i][0]);
+      atomicAdd(&acc_s[g][8 * i + 2 * t + 1], d[i][1]);
+      atomicAdd(&acc_s[g + 8][8 * i + 2 * t], d[i][2]);
+      atomicAdd(&acc_s[g + 8][8 * i + 2 * t + 1], d[i][3]);
+    }
+    __syncthreads();
   }
-  __syncthreads();
   for (int i = threadIdx.x; i < 16 * 8 * MT; i += kRWarps * 32) {
     const int n = n0 + (i & 15), m = m0 + (i >> 4);
     if (n < p.N && m < p.M) {
@@ -179,16 +221,26 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
 }
 
 template <typename F, typename... A>
-cudaError_t launch(F kern, dim3 grid, int threads, cudaStream_t stream, bool pdl, A... args) {
+cudaError_t launch(F kern, dim3 grid, int threads, int cluster, cudaStream_t stream, bool pdl, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
@@ -200,25 +252,31 @@ cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t
   const dim3 grid((unsigned)rows);
   const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 8 * 8 * kQThreads &&
                    ((reinterpret_cast<uintptr_t>(x) & 15) | (reinterpret_cast<uintptr_t>(codes) & 7)) == 0;
-  if (!vec) return launch(int8_quantize_any_kernel, grid, kQThreads, stream, pdl, x, dtype, K, codes, scale, (int)pdl);
+  if (!vec) return launch(int8_quantize_any_kernel, grid, kQThreads, 1, stream, pdl, x, dtype, K, codes, scale, (int)pdl);
   const uint16_t* x16 = static_cast<const uint16_t*>(x);
   const int per = (int)((K / 8 + kQThreads - 1) / kQThreads);
 #define NSQ_Q(NV)                                                                                             \
   (dtype == NSQ_DTYPE_BF16                                                                                    \
-       ? launch(int8_quantize_kernel<NV, true>, grid, kQThreads, stream, pdl, x16, (int)K, codes, scale, (int)pdl) \
-       : launch(int8_quantize_kernel<NV, false>, grid, kQThreads, stream, pdl, x16, (int)K, codes, scale, (int)pdl))
+       ? launch(int8_quantize_kernel<NV, true>, grid, kQThreads, 1, stream, pdl, x16, (int)K, codes, scale, (int)pdl) \
+       : launch(int8_quantize_kernel<NV, false>, grid, kQThreads, 1, stream, pdl, x16, (int)K, codes, scale, (int)pdl))
   return per <= 1 ? NSQ_Q(1) : per <= 2 ? NSQ_Q(2) : per <= 4 ? NSQ_Q(4) : NSQ_Q(8);
 #undef NSQ_Q
 }
 
 int run_int8_rows(const Int8Args& a, cudaStream_t stream) {
-  const RowsParams p{a.x, a.xscale, a.w, a.wscale, a.bias, a.bias ? a.bias_dtype : NSQ_DTYPE_NONE, a.y, a.M, a.K, a.N,
-                     a.after_quantize || pdl_enabled()};
+  RowsParams p{a.x, a.xscale, a.w, a.wscale, a.bias, a.bias ? a.bias_dtype : NSQ_DTYPE_NONE, a.y, a.M, a.K, a.N,
+               a.after_quantize || pdl_enabled(), 1};
   const int mt = a.M <= 8 ? 1 : a.M <= 16 ? 2 : a.M <= 32 ? 4 : 8;
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 8 * mt - 1) / (8 * mt)));
+  const int64_t tiles = (int64_t)((a.N + 15) / 16) * ((a.M + 8 * mt - 1) / (8 * mt));
+  // K over a cluster while the CTAs do not fill two per SM and each has 1024
+  // columns left, at up to 8 tokens (4864 -> 896 at M = 1 8.1 -> 6.6 us); the
+  // exchange through distributed shared memory costs more with more tokens
+  // (at M = 16 10.8 -> 11.9 us)
+  while (mt == 1 && p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && a.K / (2 * p.split) >= 1024) p.split *= 2;
+  const dim3 grid((unsigned)((a.N + 15) / 16 * p.split), (unsigned)((a.M + 8 * mt - 1) / (8 * mt)));
 #define NSQ_R(MT)                                                                                      \
-  (a.y_bf16 ? launch(int8_rows_kernel<MT, true>, grid, kRWarps * 32, stream, p.pdl_x, p)               \
-            : launch(int8_rows_kernel<MT, false>, grid, kRWarps * 32, stream, p.pdl_x, p))
+  (a.y_bf16 ? launch(int8_rows_kernel<MT, true>, grid, kRWarps * 32, p.split, stream, p.pdl_x, p)      \
+            : launch(int8_rows_kernel<MT, false>, grid, kRWarps * 32, p.split, stream, p.pdl_x, p))
   const cudaError_t e = mt == 1 ? NSQ_R(1) : mt == 2 ? NSQ_R(2) : mt == 4 ? NSQ_R(4) : NSQ_R(8);
 #undef NSQ_R
   return e == cudaSuccess ? NSQ_OK : NSQ_ECUDA;

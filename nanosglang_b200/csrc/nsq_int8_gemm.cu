@@ -11,9 +11,14 @@
 // run at the same time share their weight rows and tokens (8 token tiles by as
 // many weight tiles as it takes).
 //
-// Warp roles (per CTA, 320 threads): 0 TMA producer, 1 MMA issuer (of a pair,
-// the even CTA's), 2..9 epilogue. A stage holds two 128-column k-blocks, so a
-// barrier round covers 8 MMAs. The epilogue of one tile runs under the MMAs of
+// Warp roles (per CTA, 352 threads): 0 TMA of the weight, 1 MMA issuer (of a
+// pair, the even CTA's), 2 TMA of x (one lane issues a copy in about 100 cycles,
+// so one warp for all four of a stage would set the pace), 3..10 epilogue. A stage holds two 128-column k-blocks, so a
+// barrier round covers 8 MMAs. With one token tile (decode batches) it is the
+// weight's bandwidth that counts: the rows are then dealt evenly over the SMs,
+// fewer than 128 to a tile (the MMA's other rows compute on leftovers of the
+// stage that nothing reads), and the ring keeps 150 KB or more per SM in flight.
+// The epilogue of one tile runs under the MMAs of
 // the next: s32 -> fp32, scales, bias, one rounding, a staged [token][feature]
 // tile, TMA store (plain stores where N % 8 != 0 leaves no 16-byte row pitch).
 // Every wait is bounded. No TMA multicast.
@@ -30,8 +35,8 @@ constexpr int kRows = 128;  // weight rows per CTA
 constexpr int kBK = 128;    // columns per k-block: one 128-byte swizzled row
 constexpr int kKps = 2;     // k-blocks per stage
 constexpr int kEpi = 8;     // epilogue warps
-constexpr int kGemmThreads = 32 * (2 + kEpi);
-constexpr int kGroup = 8;   // token tiles that share a pass over the weight
+constexpr int kGemmThreads = 32 * (3 + kEpi);
+constexpr int kGroup = 32;   // token tiles that share a pass over the weight
 
 // CG CTAs per tile, TOK tokens per tile.
 template <int CG, int TOK>
@@ -40,6 +45,7 @@ struct GemmShape {
   static constexpr int kWBytes = kRows * kBK, kXBytes = kXRows * kBK;
   static constexpr int kStage = kKps * (kWBytes + kXBytes);
   static constexpr int kTokRound = TOK < 128 ? TOK : 128;  // tokens of a staged y tile
+  static constexpr int kWarpTok = kTokRound < 64 ? 32 : kTokRound / 2;  // of them, an epilogue warp's
   static constexpr int kYHalf = kTokRound * 64 * 2;        // 64 features
   static constexpr int NS = (226 * 1024 - 2 * kYHalf - 1024) / kStage < 6 ? (226 * 1024 - 2 * kYHalf - 1024) / kStage : 6;
   static constexpr int kY = NS * kStage;
@@ -62,6 +68,7 @@ struct GemmParams {
   DevStatus* status;
   int M, K, N, bias_dtype;
   int num_w, num_t, num_kb, num_st;
+  int wrows;  // weight rows of a CTA's tile
   int pdl_x;  // x and its scales come from the kernel ahead on the stream
 };
 
@@ -87,31 +94,37 @@ __host__ __device__ constexpr uint32_t idesc_s8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// The MMAs of one stage, issued back to back by the elected lane of a
-// converged warp: KB k-blocks of four K = 32 steps (+32 bytes = +2 descriptor
-// units a step). Only the first takes `accumulate`.
-template <int CG, int KB>
-__device__ __forceinline__ void umma_i8_elect(uint32_t d, uint64_t a0, uint64_t b0, uint64_t a1, uint64_t b1,
-                                              uint32_t idesc, uint32_t accumulate) {
+// The four MMAs of a k-block (K = 32 each, +32 bytes = +2 descriptor units a
+// step), issued back to back by the elected lane of a converged warp. Only the
+// first takes `accumulate`.
+template <int CG>
+__device__ __forceinline__ void umma_i8_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
 #define NSQ_I8_PRE "{\n\t.reg .pred e, p, t;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\t"
 #define NSQ_I8_4(M) M "[%0], %1, %5, %9, p;\n\t" M "[%0], %2, %6, %9, t;\n\t" M "[%0], %3, %7, %9, t;\n\t" M "[%0], %4, %8, %9, t;\n\t"
-#define NSQ_I8_GO(M, acc)                                                                                          \
-  asm volatile(NSQ_I8_PRE "setp.ne.b32 p, %10, 0;\n\tsetp.eq.b32 t, %10, %10;\n\t" NSQ_I8_4(M) "}" ::"r"(d), "l"(a),    \
-               "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc), "r"(acc) \
+#define NSQ_I8_GO(M)                                                                                                   \
+  asm volatile(NSQ_I8_PRE "setp.ne.b32 p, %10, 0;\n\tsetp.eq.b32 t, %10, %10;\n\t" NSQ_I8_4(M) "}" ::"r"(d), "l"(a),   \
+               "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc),              \
+               "r"(accumulate)                                                                                         \
                : "memory")
-#pragma unroll
-  for (int i = 0; i < KB; ++i) {
-    const uint64_t a = i == 0 ? a0 : a1, b = i == 0 ? b0 : b1;
-    const uint32_t acc = i == 0 ? accumulate : 1u;
-    if constexpr (CG == 1) {
-      NSQ_I8_GO("@e tcgen05.mma.cta_group::1.kind::i8 ", acc);
-    } else {
-      NSQ_I8_GO("@e tcgen05.mma.cta_group::2.kind::i8 ", acc);
-    }
+  if constexpr (CG == 1) {
+    NSQ_I8_GO("@e tcgen05.mma.cta_group::1.kind::i8 ");
+  } else {
+    NSQ_I8_GO("@e tcgen05.mma.cta_group::2.kind::i8 ");
   }
 #undef NSQ_I8_PRE
 #undef NSQ_I8_4
 #undef NSQ_I8_GO
+}
+
+// Whether the phase is complete, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // TMA load whose bytes are counted on a barrier of the pair's even CTA.
@@ -190,61 +203,48 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
     }
   };
 
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
+  if (warp == 0 || warp == 2) {
+    // ---------------- TMA producers: the weight, x ----------------
+    const bool is_x = warp == 2;
     if (lane == 0) {
-      tma_prefetch_desc(&xmap);
-      tma_prefetch_desc(&wmap);
+      const CUtensorMap* map = is_x ? &xmap : &wmap;
+      tma_prefetch_desc(map);
       const uint32_t full0 = CG == 2 ? dsmem_map(smem_u32(&full[0]), 0) : 0;
-      auto load = [&](bool is_x, int row, int st, int s) {
-        const int kb0 = st * kKps;
-        const int nk = p.num_kb - kb0 < kKps ? p.num_kb - kb0 : kKps;
-        for (int i = 0; i < nk; ++i) {
-          uint8_t* dst = smem + s * S::kStage + (is_x ? kKps * S::kWBytes + i * S::kXBytes : i * S::kWBytes);
-          const CUtensorMap* map = is_x ? &xmap : &wmap;
-          if constexpr (CG == 2) {
-            tma_load_2d_pair(dst, map, full0 + s * 8, (kb0 + i) * kBK, row);
-          } else {
-            tma_load_2d(dst, map, &full[s], (kb0 + i) * kBK, row);
-          }
-        }
-      };
-      // the even CTA arms the barrier for the bytes of both
-      auto arm = [&](int st, int s) {
-        const int nk = p.num_kb - st * kKps < kKps ? p.num_kb - st * kKps : kKps;
-        if (leader) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * nk) * (S::kWBytes + S::kXBytes));
-      };
-      auto w_row = [&](int wt) { return (wt * CG + (int)rank) * kRows; };
-      // the weights do not depend on the kernel ahead: the first stages' are
-      // on their way before it is waited for
-      int pre = 0;
-      for (int u = cid; u < units && pre < S::NS; u += ncl) {
-        int wt, tt;
-        gemm_unit(p, u, wt, tt);
-        for (int st = 0; st < p.num_st && pre < S::NS; ++st, ++pre) {
-          arm(st, pre);
-          load(false, w_row(wt), st, pre);
-        }
-      }
-      if (p.pdl_x) pdl_wait_prior_grids();
-      int it = 0;
+      uint8_t* const place = smem + (is_x ? kKps * S::kWBytes : 0);
+      const int bytes = is_x ? S::kXBytes : S::kWBytes;
+      // The weight does not depend on the kernel ahead: its first stages are on
+      // their way while that one still runs.
+      if (is_x && p.pdl_x) pdl_wait_prior_grids();
+      int it = 0, s = 0;
+      uint32_t phase = 1;  // of done[s], one use back
       for (int u = cid; u < units && ok; u += ncl) {
         int wt, tt;
         gemm_unit(p, u, wt, tt);
-        const int x_row = tt * TOK + (int)rank * (gemm_n<TOK>(p.M, tt) / CG);
+        const int row = is_x ? tt * TOK + (int)rank * (gemm_n<TOK>(p.M, tt) / CG) : (wt * CG + (int)rank) * p.wrows;
         for (int st = 0; st < p.num_st; ++st, ++it) {
-          const int s = it % S::NS;
-          if (it >= pre) {
-            if (!(ok = mbar_wait(&done[s], ((it / S::NS) & 1) ^ 1, p.status, 210, abort_flag))) break;
-            arm(st, s);
-            load(false, w_row(wt), st, s);
+          if (!(ok = mbar_wait(&done[s], phase, p.status, is_x ? 214 : 210, abort_flag))) break;
+          const int kb0 = st * kKps;
+          const int nk = p.num_kb - kb0 < kKps ? p.num_kb - kb0 : kKps;
+          // the even CTA arms the barrier for the bytes of both
+          if (!is_x && leader) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * nk) * (uint32_t)(p.wrows * kBK + S::kXBytes));
+#pragma unroll
+          for (int i = 0; i < kKps; ++i) {
+            if (i < nk) {
+              if constexpr (CG == 2) {
+                tma_load_2d_pair(place + s * S::kStage + i * bytes, map, full0 + s * 8, (kb0 + i) * kBK, row);
+              } else {
+                tma_load_2d(place + s * S::kStage + i * bytes, map, &full[s], (kb0 + i) * kBK, row);
+              }
+            }
           }
-          load(true, x_row, st, s);
+          if (++s == S::NS) {
+            s = 0;
+            phase ^= 1;
+          }
         }
       }
-      if (!ok && leader) {  // let copies in flight land before the CTA (of a pair, both) can exit
-        const int last = it > pre ? it : pre;
-        for (int j = last > S::NS ? last - S::NS : 0; j < last; ++j) {
+      if (!ok && !is_x && leader) {  // let copies in flight land before the CTA (of a pair, both) can exit
+        for (int j = it > S::NS ? it - S::NS : 0; j < it; ++j) {
           mbar_wait(&full[j % S::NS], (j / S::NS) & 1, nullptr, 0, nullptr);
         }
       }
@@ -252,31 +252,39 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (leader) {
-      int it = 0, tc = 0;
+      // The next stage's barrier is looked at between this one's two groups of
+      // MMAs, so that the tensor pipe has work while the answer comes back.
+      const uint32_t base0 = smem_u32(smem);
+      int it = 0, tc = 0, s = 0;
+      uint32_t phase = 0;
+      bool ready = false;  // full[s] was seen complete
       for (int u = cid; u < units && ok; u += ncl, ++tc) {
         int wt, tt;
         gemm_unit(p, u, wt, tt);
         const uint32_t idesc = idesc_s8(CG * kRows, gemm_n<TOK>(p.M, tt));
         const int buf = tc & 1;
+        const uint32_t d = tmem + buf * TOK;
         ok = __all_sync(0xffffffffu, mbar_wait(&empty_acc[buf], ((tc >> 1) & 1) ^ 1, p.status, 211, abort_flag));
         if (!ok) break;
         tc_fence_after();
         for (int st = 0; st < p.num_st; ++st, ++it) {
-          const int s = it % S::NS;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / S::NS) & 1, p.status, 212, abort_flag));
-          if (!ok) break;
+          if (!ready) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, p.status, 212, abort_flag));
+            if (!ok) break;
+          }
           tc_fence_after();
-          const uint32_t base = smem_u32(smem + s * S::kStage);
-          const uint64_t a0 = sw128_kmajor_desc(base), a1 = sw128_kmajor_desc(base + S::kWBytes);
-          const uint64_t b0 = sw128_kmajor_desc(base + kKps * S::kWBytes);
-          const uint64_t b1 = sw128_kmajor_desc(base + kKps * S::kWBytes + S::kXBytes);
-          const uint32_t d = tmem + buf * TOK;
+          const uint32_t base = base0 + s * S::kStage;
+          umma_i8_elect<CG>(d, sw128_kmajor_desc(base), sw128_kmajor_desc(base + kKps * S::kWBytes), idesc, st > 0);
+          const int s1 = s + 1 == S::NS ? 0 : s + 1;
+          const uint32_t phase1 = s1 == 0 ? phase ^ 1 : phase;
+          ready = __all_sync(0xffffffffu, mbar_test(&full[s1], phase1));
           if (p.num_kb - st * kKps >= 2) {
-            umma_i8_elect<CG, 2>(d, a0, b0, a1, b1, idesc, st > 0);
-          } else {
-            umma_i8_elect<CG, 1>(d, a0, b0, a1, b1, idesc, st > 0);
+            umma_i8_elect<CG>(d, sw128_kmajor_desc(base + S::kWBytes),
+                              sw128_kmajor_desc(base + kKps * S::kWBytes + S::kXBytes), idesc, 1u);
           }
           commit(&done[s]);
+          s = s1;
+          phase = phase1;
         }
         if (!ok) break;
         commit(&full_acc[buf]);
@@ -289,8 +297,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
     // ---------------- epilogue ----------------
     if (p.pdl_x) pdl_wait_prior_grids();  // the scales of x, and y's buffer
     const int sub = warp & 3;             // tensor-memory sub-partition: 32 weight rows
-    const int half = (warp - 2) >> 2;     // half of a round's tokens
-    const int etid = threadIdx.x - 64;
+    const int half = (warp - 3) >> 2;     // half of a round's tokens
+    const int etid = threadIdx.x - 96;
     const int g = lane >> 2, t = lane & 3;
     const bool has_bias = p.bias_dtype != NSQ_DTYPE_NONE;
     const uint32_t empty0 = CG == 2 ? dsmem_map(smem_u32(&empty_acc[0]), 0) : 0;
@@ -301,14 +309,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
       int wt, tt;
       gemm_unit(p, u, wt, tt);
       const int buf = tc & 1;
-      const int f0 = (wt * CG + (int)rank) * kRows;  // first feature of this CTA
+      const int f0 = (wt * CG + (int)rank) * p.wrows;  // first feature of this CTA
+      const int f1 = f0 + p.wrows < p.N ? f0 + p.wrows : p.N;
       // fragment rows of this lane: features sub * 32 + 8 q + g
       float wsc[4], bf[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = f0 + sub * 32 + 8 * q + g;
-        wsc[q] = n < p.N ? __ldg(p.wscale + n) : 0.f;
-        bf[q] = has_bias && n < p.N ? load_bias(p.bias, p.bias_dtype, n) : 0.f;
+        wsc[q] = n < f1 ? __ldg(p.wscale + n) : 0.f;
+        bf[q] = has_bias && n < f1 ? load_bias(p.bias, p.bias_dtype, n) : 0.f;
       }
       ok = mbar_wait(&full_acc[buf], (tc >> 1) & 1, p.status, 213, abort_flag);
       if (!named_bar_all(1, kEpi * 32, ok)) {
@@ -317,7 +326,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
       }
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(sub * 32) << 16) + buf * TOK;
-      constexpr int kWarpTok = S::kTokRound / 2;
+      constexpr int kWarpTok = S::kWarpTok;
 #pragma unroll 1
       for (int rd = 0; rd < TOK / S::kTokRound; ++rd) {
         if constexpr (STAGED) {
@@ -326,7 +335,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
         }
         const int col0 = rd * S::kTokRound + half * kWarpTok;
 #pragma unroll 1
-        for (int c = 0; c < kWarpTok && tt * TOK + col0 + c < p.M; c += 32) {
+        for (int c = 0; c < kWarpTok && half * kWarpTok < S::kTokRound && tt * TOK + col0 + c < p.M; c += 32) {
           uint32_t r0[16], r1[16];
           tmem_ld_16x256b_x4(acc + col0 + c, r0);
           tmem_ld_16x256b_x4(acc + (16u << 16) + col0 + c, r1);
@@ -364,7 +373,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const int m = tt * TOK + col0 + c + 8 * j + 2 * t + e, n = f0 + sub * 32 + 8 * q + g;
-                  if (m < p.M && n < p.N) {
+                  if (m < p.M && n < f1) {
                     static_cast<uint16_t*>(p.y)[(int64_t)m * p.N + n] = float_to_elem<BF16>(v[q][e]);
                   }
                 }
@@ -387,7 +396,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
           fence_proxy_async_smem();
           named_bar_sync(1, kEpi * 32);
           if (etid == 0) {
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < p.wrows / 64; ++h) {
               const int f = f0 + h * 64, m = tt * TOK + rd * S::kTokRound;
               if (f < p.N && m < p.M) tma_store_2d(&ymap, smem + S::kY + h * S::kYHalf, f, m);
             }
@@ -444,13 +453,13 @@ cudaError_t launch_gemm(const Int8Args& a, const CUtensorMap& xmap, const CUtens
 }
 
 template <int CG, int TOK>
-int run_gemm(const Int8Args& a, cudaStream_t stream) {
+int run_gemm(const Int8Args& a, int wrows, cudaStream_t stream) {
   using S = GemmShape<CG, TOK>;
-  const bool staged = a.N % 8 == 0;
+  const bool staged = a.N % 8 == 0 && wrows % 64 == 0;
   CUtensorMap xmap, wmap, ymap;
   if (encode_tensor_map_2d(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<int8_t*>(a.x), a.K, a.M, a.K, kBK,
                            S::kXRows, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS ||
-      encode_tensor_map_2d(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<int8_t*>(a.w), a.K, a.N, a.K, kBK, kRows,
+      encode_tensor_map_2d(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<int8_t*>(a.w), a.K, a.N, a.K, kBK, wrows,
                            CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS) {
     return NSQ_ECUDA;
   }
@@ -471,7 +480,8 @@ int run_gemm(const Int8Args& a, cudaStream_t stream) {
   p.M = a.M;
   p.K = a.K;
   p.N = a.N;
-  p.num_w = (a.N + CG * kRows - 1) / (CG * kRows);
+  p.wrows = wrows;
+  p.num_w = (a.N + CG * wrows - 1) / (CG * wrows);
   p.num_t = (a.M + TOK - 1) / TOK;
   p.num_kb = (a.K + kBK - 1) / kBK;
   p.num_st = (p.num_kb + kKps - 1) / kKps;
@@ -490,18 +500,27 @@ int run_gemm(const Int8Args& a, cudaStream_t stream) {
 
 }  // namespace
 
-// Tile choice: waves of tiles times a tile's time in cycles, per k-block and
-// fixed (fill, epilogue of the last tile).
+// One token tile: rows dealt evenly over the SMs. Otherwise waves of tiles
+// times a tile's time in cycles, per k-block and fixed (fill, the last tile's
+// epilogue).
 int run_int8_gemm(const Int8Args& a, cudaStream_t stream) {
   const int64_t sms = num_sms(), kb = (a.K + kBK - 1) / kBK;
+  if (a.M <= 128) {
+    const int64_t waves = (a.N + sms * kRows - 1) / (sms * kRows);
+    const int64_t each = (a.N + sms * waves - 1) / (sms * waves);
+    const int wrows = (int)((each + 7) / 8 * 8);
+    if (a.M <= 32) return run_gemm<1, 32>(a, wrows, stream);
+    if (a.M <= 64) return run_gemm<1, 64>(a, wrows, stream);
+    return run_gemm<1, 128>(a, wrows, stream);
+  }
   auto cost = [&](int cg, int tok, int per_kb, int fixed) {
     const int64_t tiles = (int64_t)((a.N + cg * kRows - 1) / (cg * kRows)) * ((a.M + tok - 1) / tok);
     const int64_t at_once = sms / cg;
     return (tiles + at_once - 1) / at_once * (kb * per_kb) + fixed;
   };
   const int64_t c2 = cost(2, 256, 640, 6000), c1 = cost(1, 128, 320, 4000), ch = cost(1, 64, 200, 3000);
-  if (c2 <= c1 && c2 <= ch) return run_gemm<2, 256>(a, stream);
-  return c1 <= ch ? run_gemm<1, 128>(a, stream) : run_gemm<1, 64>(a, stream);
+  if (c2 <= c1 && c2 <= ch) return run_gemm<2, 256>(a, kRows, stream);
+  return c1 <= ch ? run_gemm<1, 128>(a, kRows, stream) : run_gemm<1, 64>(a, kRows, stream);
 }
 
 }  // namespace nsq
