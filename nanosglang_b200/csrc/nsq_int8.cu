@@ -7,6 +7,8 @@
 // and the order of k is free, so every lane reads 16 consecutive bytes of its
 // row and feeds them to two MMAs as they come: weights go from global memory
 // to the tensor cores without shared memory or conversion.
+#include <type_traits>
+
 #include "nsq_common.cuh"
 #include "nsq_internal.h"
 #include "nsq_rows8.cuh"
@@ -18,10 +20,12 @@ namespace {
 constexpr int kQThreads = 256;
 
 // ---------------------------------------------------------------------------
-// Row quantiser: one CTA per row. NV vectors of 16 bytes per thread are kept
-// in registers between the maximum and the codes (one pass over DRAM); NV = 0
-// takes any row length, alignment and type, element by element, and reads the
-// row twice (the second time from L2).
+// Row quantiser: TPR threads per row, NV vectors of 16 bytes each, which stay in
+// registers between the maximum and the codes (one pass over DRAM, which bounds
+// it). Few rows take 256 threads each (latency), many the fewest that hold a
+// row (no waiting for other warps). int8_quantize_any_kernel takes any row
+// length, alignment and type, element by element, and reads the row twice (the
+// second time from L2).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float load_elem(const void* p, int dtype, int64_t i) {
   if (dtype == NSQ_DTYPE_F32) return static_cast<const float*>(p)[i];
@@ -41,43 +45,44 @@ __device__ __forceinline__ float block_nan_max(float m) {
   return m;
 }
 
-template <int NV, bool BF16>
-__global__ void __launch_bounds__(kQThreads) int8_quantize_kernel(const uint16_t* __restrict__ x, int K,
+template <int TPR, int NV, bool BF16>
+__global__ void __launch_bounds__(kQThreads) int8_quantize_kernel(const uint16_t* __restrict__ x, int M, int K,
                                                                   int8_t* __restrict__ codes,
                                                                   float* __restrict__ scale, int pdl) {
   if (pdl) pdl_wait_prior_grids();
   pdl_launch_dependents();
-  const int64_t row = blockIdx.x;
+  __shared__ uint32_t red[kQThreads / 32];
+  const int lane = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * (kQThreads / TPR) + threadIdx.x / TPR;
+  const bool in = row < M;
   const uint4* src = reinterpret_cast<const uint4*>(x + row * K);
-  const int nvec = K / 8;
+  const int nvec = in ? K / 8 : 0;
   uint4 v[NV];
-  float m = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int i = j * kQThreads + threadIdx.x;
+    const int i = j * TPR + lane;
     v[j] = i < nvec ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
   }
+  uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+  for (int j = 0; j < NV; ++j) m = abs_max2(m, v[j]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = nan_max(m, fabsf(elem_to_float<BF16>((uint16_t)(w[i / 2] >> (16 * (i & 1))))));
+  for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if constexpr (TPR > 32) {
+    const int w0 = threadIdx.x / TPR * (TPR / 32);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) m = __vmaxu2(m, red[w0 + i]);
   }
-  const float s = row_scale<false>(block_nan_max(m));
-  if (threadIdx.x == 0) scale[row] = s;
+  if (!in) return;
+  const float s = row_scale<false>(abs_max_value<BF16>(m));
+  if (lane == 0) scale[row] = s;
   const RowDiv dv(s);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int i = j * kQThreads + threadIdx.x;
-    if (i >= nvec) break;
-    const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-    uint32_t c[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      c[e / 4] |= (uint32_t)row_code<false>(dv(elem_to_float<BF16>((uint16_t)(w[e / 2] >> (16 * (e & 1))))))
-                  << (8 * (e & 3));
-    }
-    reinterpret_cast<uint2*>(codes + row * K)[i] = make_uint2(c[0], c[1]);
+    const int i = j * TPR + lane;
+    if (i < nvec) reinterpret_cast<uint2*>(codes + row * K)[i] = row_codes8<false, BF16>(dv, v[j]);
   }
 }
 
@@ -246,21 +251,38 @@ cudaError_t launch(F kern, dim3 grid, int threads, int cluster, cudaStream_t str
 
 }  // namespace
 
+template <int TPR, bool BF16>
+static cudaError_t quantize_rows(const uint16_t* x, int M, int K, int8_t* codes, float* scale, cudaStream_t stream,
+                                 bool pdl) {
+  const dim3 grid((unsigned)((M + kQThreads / TPR - 1) / (kQThreads / TPR)));
+  const int per = (K / 8 + TPR - 1) / TPR;
+  auto go = [&](auto kern) { return launch(kern, grid, kQThreads, 1, stream, pdl, x, M, K, codes, scale, (int)pdl); };
+  return per <= 1   ? go(int8_quantize_kernel<TPR, 1, BF16>)
+         : per <= 2 ? go(int8_quantize_kernel<TPR, 2, BF16>)
+         : per <= 4 ? go(int8_quantize_kernel<TPR, 4, BF16>)
+                    : go(int8_quantize_kernel<TPR, 8, BF16>);
+}
+
 cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K, int8_t* codes, float* scale,
                                  cudaStream_t stream) {
   const bool pdl = pdl_enabled();
-  const dim3 grid((unsigned)rows);
   const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 8 * 8 * kQThreads &&
                    ((reinterpret_cast<uintptr_t>(x) & 15) | (reinterpret_cast<uintptr_t>(codes) & 7)) == 0;
-  if (!vec) return launch(int8_quantize_any_kernel, grid, kQThreads, 1, stream, pdl, x, dtype, K, codes, scale, (int)pdl);
+  if (!vec) {
+    return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 1, stream, pdl, x, dtype, K, codes, scale,
+                  (int)pdl);
+  }
   const uint16_t* x16 = static_cast<const uint16_t*>(x);
-  const int per = (int)((K / 8 + kQThreads - 1) / kQThreads);
-#define NSQ_Q(NV)                                                                                             \
-  (dtype == NSQ_DTYPE_BF16                                                                                    \
-       ? launch(int8_quantize_kernel<NV, true>, grid, kQThreads, 1, stream, pdl, x16, (int)K, codes, scale, (int)pdl) \
-       : launch(int8_quantize_kernel<NV, false>, grid, kQThreads, 1, stream, pdl, x16, (int)K, codes, scale, (int)pdl))
-  return per <= 1 ? NSQ_Q(1) : per <= 2 ? NSQ_Q(2) : per <= 4 ? NSQ_Q(4) : NSQ_Q(8);
-#undef NSQ_Q
+  auto go = [&](auto tpr) {
+    constexpr int T = decltype(tpr)::value;
+    return dtype == NSQ_DTYPE_BF16 ? quantize_rows<T, true>(x16, (int)rows, (int)K, codes, scale, stream, pdl)
+                                   : quantize_rows<T, false>(x16, (int)rows, (int)K, codes, scale, stream, pdl);
+  };
+  const bool few = rows < 8 * num_sms();
+  if (few || K > 128 * 64) return go(std::integral_constant<int, 256>());
+  if (K > 64 * 64) return go(std::integral_constant<int, 128>());
+  if (K > 32 * 64) return go(std::integral_constant<int, 64>());
+  return go(std::integral_constant<int, 32>());
 }
 
 int run_int8_rows(const Int8Args& a, cudaStream_t stream) {

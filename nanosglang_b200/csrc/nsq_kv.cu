@@ -58,79 +58,124 @@ __device__ __forceinline__ void report(DevStatus* st, uint32_t where) {
   }
 }
 
+// Strides are below 2^32 elements (checked on the host).
+__device__ __forceinline__ int64_t mul_wide(uint32_t a, int64_t stride) {
+  return (int64_t)((uint64_t)a * (uint32_t)stride);
+}
+
 // ---------------------------------------------------------------------------
 // Write and read
 // ---------------------------------------------------------------------------
 
-// Eight elements of a row per lane, LPR lanes per row (LPR * 8 >= head_dim):
-// one 16-byte load, a shuffle maximum, one 8-byte store. Bound by DRAM.
+// Four codes (bytes of w) -> fp16 pairs (b0, b1) and (b2, b3), exact.
+template <bool FP8>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FP8) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else {
+    // 1024 + (code + 128) in the low mantissa bits, minus 1152
+    const uint32_t u = w ^ 0x80808080u;
+    const uint32_t a = prmt(u, 0x64646464u, 0x4140), b = prmt(u, 0x64646464u, 0x4342);
+    const __half2 c = __floats2half2_rn(1152.f, 1152.f);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), c);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), c);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+
+// Sixteen elements of a row per lane, LPR lanes per row (LPR * 16 >= head_dim),
+// k and v of one place together and two places at a time: the place is worked
+// out once for 64 elements, and their loads are in flight together. DRAM bounds
+// both kernels.
+constexpr int kAtOnce = 2;
+
+struct KvPlace {
+  uint32_t page, off, tok, head;
+  bool in;  // a place of the pool
+};
+template <typename P>
+__device__ __forceinline__ KvPlace kv_place(const P& p, uint32_t row, uint32_t rows, uint32_t tag, bool tell) {
+  KvPlace a;
+  a.tok = fdiv(row, p.head_div);
+  a.head = row - a.tok * (uint32_t)p.c.kv_heads;
+  const int64_t slot = row < rows ? __ldg(p.slots + a.tok) : -1;
+  a.in = slot >= 0 && slot < (int64_t)p.c.num_pages * p.c.page_size;
+  if (!a.in && slot >= 0 && tell) report(p.status, tag);
+  a.page = a.in ? fdiv((uint32_t)slot, p.page_div) : 0;
+  a.off = a.in ? (uint32_t)slot - a.page * (uint32_t)p.c.page_size : 0;
+  return a;
+}
+__device__ __forceinline__ int64_t kv_at(const KvPlace& a, const int64_t (&stride)[3]) {
+  return mul_wide(a.page, stride[0]) + mul_wide(a.off, stride[1]) + mul_wide(a.head, stride[2]);
+}
+
 template <bool FP8, bool BF16, int LPR>
 __global__ void __launch_bounds__(256) kv_write_kernel(const KvWrite p) {
   if (p.pdl) pdl_wait_prior_grids();
   const int sub = threadIdx.x % LPR;
   const uint32_t rows = (uint32_t)p.T * (uint32_t)p.c.kv_heads;
-  const bool in_row = sub * 8 < p.c.head_dim;
-  for (uint32_t r0 = (blockIdx.x * 256 + threadIdx.x) / LPR; r0 < 2 * rows; r0 += gridDim.x * (256 / LPR)) {
-    const bool isv = r0 >= rows;
-    const uint32_t r = isv ? r0 - rows : r0;
-    const int64_t tok = fdiv(r, p.head_div);
-    const int head = (int)(r - (uint32_t)tok * (uint32_t)p.c.kv_heads);
-    const int64_t slot = __ldg(p.slots + tok);
-    if (slot < 0) continue;  // a padded token
-    if (slot >= (int64_t)p.c.num_pages * p.c.page_size) {
-      if (sub == 0) report(p.status, 200);
-      continue;
-    }
-    const int64_t page = fdiv((uint32_t)slot, p.page_div);
-    const int64_t off = slot - page * p.c.page_size;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (in_row) {
-      const uint16_t* src = static_cast<const uint16_t*>(isv ? p.v : p.k) +
-                            tok * (isv ? p.v_stride[0] : p.k_stride[0]) + head * (isv ? p.v_stride[1] : p.k_stride[1]);
-      raw = __ldg(reinterpret_cast<const uint4*>(src + sub * 8));
-    }
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[8];
-    float m = 0.f;
+  const bool in_row = sub * 16 < p.c.head_dim;
+  const uint32_t step = gridDim.x * (256 / LPR);
+  // whole warps stay in the loop: the shuffles below are all lanes'
+  for (uint32_t r0 = (blockIdx.x * 256 + (threadIdx.x & ~31u)) / LPR; r0 < rows; r0 += kAtOnce * step) {
+    KvPlace a[kAtOnce];
+    uint4 x[kAtOnce][2][2];  // [place][k, v][8 elements]
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = elem_to_float<BF16>((uint16_t)(w[i / 2] >> (16 * (i & 1))));
-      m = nan_max(m, fabsf(x[i]));
-    }
-    // the lanes of a row are converged here: whole rows leave the loop together
-    const uint32_t lanes = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << (threadIdx.x & 31 & ~(LPR - 1));
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t r = r0 + (threadIdx.x & 31) / LPR + i * step;
+      a[i] = kv_place(p, r, rows, 200, sub == 0);
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) m = nan_max(m, __shfl_xor_sync(lanes, m, o));
-    const float s = row_scale<FP8>(m);
-    const RowDiv dv(s);
-    uint32_t c0 = 0, c1 = 0;
+      for (int j = 0; j < 2; ++j) {
+        const int64_t at = j ? a[i].tok * p.v_stride[0] + a[i].head * p.v_stride[1]
+                             : a[i].tok * p.k_stride[0] + a[i].head * p.k_stride[1];
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(j ? p.v : p.k) + at + sub * 16);
+        const bool in = in_row && r < rows;
+        x[i][j][0] = in ? __ldg(src) : make_uint4(0, 0, 0, 0);
+        x[i][j][1] = in ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c0 |= (uint32_t)row_code<FP8>(dv(x[i])) << (8 * i);
-      c1 |= (uint32_t)row_code<FP8>(dv(x[i + 4])) << (8 * i);
-    }
-    if (in_row) {
-      uint8_t* dst = (isv ? p.c.v : p.c.k) +
-                     (isv ? page * p.c.v_stride[0] + off * p.c.v_stride[1] + head * p.c.v_stride[2]
-                          : page * p.c.k_stride[0] + off * p.c.k_stride[1] + head * p.c.k_stride[2]);
-      *reinterpret_cast<uint2*>(dst + sub * 8) = make_uint2(c0, c1);
-    }
-    if (sub == 0) {
-      float* sd = (isv ? p.c.vs : p.c.ks) +
-                  (isv ? page * p.c.vs_stride[0] + off * p.c.vs_stride[1] + head * p.c.vs_stride[2]
-                       : page * p.c.ks_stride[0] + off * p.c.ks_stride[1] + head * p.c.ks_stride[2]);
-      *sd = s;
+    for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t m = abs_max2(abs_max2(0, x[i][j][0]), x[i][j][1]);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!a[i].in) continue;
+        const float s = row_scale<FP8>(abs_max_value<BF16>(m));
+        const RowDiv dv(s);
+        if (in_row) {
+          const uint2 lo = row_codes8<FP8, BF16>(dv, x[i][j][0]), hi = row_codes8<FP8, BF16>(dv, x[i][j][1]);
+          uint8_t* dst = j ? p.c.v + kv_at(a[i], p.c.v_stride) : p.c.k + kv_at(a[i], p.c.k_stride);
+          *reinterpret_cast<uint4*>(dst + sub * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+        if (sub == 0) *(j ? p.c.vs + kv_at(a[i], p.c.vs_stride) : p.c.ks + kv_at(a[i], p.c.ks_stride)) = s;
+      }
     }
   }
 }
 
-template <bool FP8>
-__device__ __forceinline__ float code_value(uint8_t c) {
-  if constexpr (FP8) {
-    return static_cast<float>(*reinterpret_cast<const __nv_fp8_e4m3*>(&c));
-  } else {
-    return (float)(int8_t)c;
+// Four codes times s, as four elements.
+template <bool FP8, bool BF16>
+__device__ __forceinline__ uint2 values4(uint32_t w, float s) {
+  uint32_t h[2], o[2];
+  codes_to_f16<FP8>(w, h[0], h[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    if constexpr (BF16) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * s, f.y * s);
+      o[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      const __half2 b = __floats2half2_rn(f.x * s, f.y * s);
+      o[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
   }
+  return make_uint2(o[0], o[1]);
 }
 
 // The inverse: code * s rounded once to the output type. Rows of a negative
@@ -139,39 +184,41 @@ template <bool FP8, bool BF16, int LPR>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
   if (p.pdl) pdl_wait_prior_grids();
   const int sub = threadIdx.x % LPR;
-  if (sub * 8 >= p.c.head_dim) return;
+  if (sub * 16 >= p.c.head_dim) return;
   const uint32_t rows = (uint32_t)p.T * (uint32_t)p.c.kv_heads;
-  for (uint32_t r0 = (blockIdx.x * 256 + threadIdx.x) / LPR; r0 < 2 * rows; r0 += gridDim.x * (256 / LPR)) {
-    const bool isv = r0 >= rows;
-    const uint32_t r = isv ? r0 - rows : r0;
-    const int64_t tok = fdiv(r, p.head_div);
-    const int head = (int)(r - (uint32_t)tok * (uint32_t)p.c.kv_heads);
-    const int64_t slot = __ldg(p.slots + tok);
-    uint32_t o[4] = {0, 0, 0, 0};
-    if (slot >= 0) {
-      if (slot >= (int64_t)p.c.num_pages * p.c.page_size) {
-        if (sub == 0) report(p.status, 201);
-      } else {
-        const int64_t page = fdiv((uint32_t)slot, p.page_div);
-        const int64_t off = slot - page * p.c.page_size;
-        const uint8_t* src = (isv ? p.c.v : p.c.k) +
-                             (isv ? page * p.c.v_stride[0] + off * p.c.v_stride[1] + head * p.c.v_stride[2]
-                                  : page * p.c.k_stride[0] + off * p.c.k_stride[1] + head * p.c.k_stride[2]);
-        const float s = *((isv ? p.c.vs : p.c.ks) +
-                          (isv ? page * p.c.vs_stride[0] + off * p.c.vs_stride[1] + head * p.c.vs_stride[2]
-                               : page * p.c.ks_stride[0] + off * p.c.ks_stride[1] + head * p.c.ks_stride[2]));
-        const uint2 c = *reinterpret_cast<const uint2*>(src + sub * 8);
+  const uint32_t step = gridDim.x * (256 / LPR);
+  for (uint32_t r0 = (blockIdx.x * 256 + threadIdx.x) / LPR; r0 < rows; r0 += kAtOnce * step) {
+    KvPlace a[kAtOnce];
+    uint4 c[kAtOnce][2];
+    float s[kAtOnce][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t word = i < 2 ? c.x : c.y;
-          const float a = code_value<FP8>((uint8_t)(word >> (16 * (i & 1)))) * s;
-          const float b = code_value<FP8>((uint8_t)(word >> (16 * (i & 1) + 8))) * s;
-          o[i] = (uint32_t)float_to_elem<BF16>(a) | ((uint32_t)float_to_elem<BF16>(b) << 16);
+    for (int i = 0; i < kAtOnce; ++i) a[i] = kv_place(p, r0 + i * step, rows, 201, sub == 0);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        c[i][j] = make_uint4(0, 0, 0, 0);
+        s[i][j] = 0.f;
+        if (a[i].in) {
+          const uint8_t* src = j ? p.c.v + kv_at(a[i], p.c.v_stride) : p.c.k + kv_at(a[i], p.c.k_stride);
+          c[i][j] = *reinterpret_cast<const uint4*>(src + sub * 16);
+          s[i][j] = *(j ? p.c.vs + kv_at(a[i], p.c.vs_stride) : p.c.ks + kv_at(a[i], p.c.ks_stride));
         }
       }
     }
-    uint16_t* dst = static_cast<uint16_t*>(isv ? p.v : p.k) + (int64_t)r * p.c.head_dim + sub * 8;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t r = r0 + i * step;
+      if (r >= rows) break;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(j ? p.v : p.k) + (int64_t)r * p.c.head_dim + sub * 16);
+        const uint2 v0 = values4<FP8, BF16>(c[i][j].x, s[i][j]), v1 = values4<FP8, BF16>(c[i][j].y, s[i][j]);
+        const uint2 v2 = values4<FP8, BF16>(c[i][j].z, s[i][j]), v3 = values4<FP8, BF16>(c[i][j].w, s[i][j]);
+        dst[0] = make_uint4(v0.x, v0.y, v1.x, v1.y);
+        dst[1] = make_uint4(v2.x, v2.y, v3.x, v3.y);
+      }
+    }
   }
 }
 
@@ -248,26 +295,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Four codes (bytes of w) -> fp16 pairs (b0, b1) and (b2, b3), exact.
-template <bool FP8>
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (FP8) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-        : "=r"(lo), "=r"(hi)
-        : "r"(w));
-  } else {
-    // 1024 + (code + 128) in the low mantissa bits, minus 1152
-    const uint32_t u = w ^ 0x80808080u;
-    const uint32_t a = prmt(u, 0x64646464u, 0x4140), b = prmt(u, 0x64646464u, 0x4342);
-    const __half2 c = __floats2half2_rn(1152.f, 1152.f);
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), c);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), c);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  }
-}
-
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -302,11 +329,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
-}
-
-// Strides are below 2^32 elements (checked on the host).
-__device__ __forceinline__ int64_t mul_wide(uint32_t a, int64_t stride) {
-  return (int64_t)((uint64_t)a * (uint32_t)stride);
 }
 
 // Tokens a sequence holds: seq_lens clamped to what its page-table row can name.
@@ -1187,8 +1209,10 @@ cudaError_t run_attn_t(const KvAttn& p, const AttnPlan& a, bool fp8, bool bf16, 
 }
 
 int grid_rows(int64_t rows, int lpr) {
-  const int64_t want = (rows * lpr + 255) / 256, cap = (int64_t)num_sms() * 16;
-  return (int)(want < 1 ? 1 : want > cap ? cap : want);
+  // a row per group of lanes until every SM has its blocks, then up to kAtOnce
+  const int64_t want = (rows * lpr + 255) / 256, cap = (int64_t)num_sms() * 8;
+  const int64_t deep = (want + kAtOnce - 1) / kAtOnce;
+  return (int)(want < 1 ? 1 : want <= cap ? want : deep > cap ? deep : cap);
 }
 
 }  // namespace
@@ -1196,15 +1220,15 @@ int grid_rows(int64_t rows, int lpr) {
 cudaError_t launch_kv_write(const KvCache& c, const void* k, const int64_t* k_stride, const void* v,
                             const int64_t* v_stride, const int64_t* slots, int T, bool fp8, bool bf16,
                             cudaStream_t stream) {
-  const int lpr = c.head_dim <= 64 ? 8 : c.head_dim <= 128 ? 16 : 32;
-  const dim3 grid(grid_rows(2 * (int64_t)T * c.kv_heads, lpr));
+  const int lpr = c.head_dim <= 64 ? 4 : c.head_dim <= 128 ? 8 : 16;
+  const dim3 grid(grid_rows((int64_t)T * c.kv_heads, lpr));
   const KvWrite p{c, k, v, {k_stride[0], k_stride[1]}, {v_stride[0], v_stride[1]}, slots, T,
                   make_fastdiv((uint32_t)c.kv_heads), make_fastdiv((uint32_t)c.page_size), device_status_ptr(),
                   pdl_enabled()};
-  auto go = [&](auto k8, auto k16, auto k32) {
-    return launch(lpr == 8 ? k8 : lpr == 16 ? k16 : k32, grid, 256, 0, stream, p.pdl, p);
+  auto go = [&](auto k4, auto k8, auto k16) {
+    return launch(lpr == 4 ? k4 : lpr == 8 ? k8 : k16, grid, 256, 0, stream, p.pdl, p);
   };
-#define NSQ_KV_GO(F, B) go(kv_write_kernel<F, B, 8>, kv_write_kernel<F, B, 16>, kv_write_kernel<F, B, 32>)
+#define NSQ_KV_GO(F, B) go(kv_write_kernel<F, B, 4>, kv_write_kernel<F, B, 8>, kv_write_kernel<F, B, 16>)
   if (fp8) return bf16 ? NSQ_KV_GO(true, true) : NSQ_KV_GO(true, false);
   return bf16 ? NSQ_KV_GO(false, true) : NSQ_KV_GO(false, false);
 #undef NSQ_KV_GO
@@ -1212,14 +1236,14 @@ cudaError_t launch_kv_write(const KvCache& c, const void* k, const int64_t* k_st
 
 cudaError_t launch_kv_read(const KvCache& c, const int64_t* slots, int T, void* k, void* v, bool fp8, bool bf16,
                            cudaStream_t stream) {
-  const int lpr = c.head_dim <= 64 ? 8 : c.head_dim <= 128 ? 16 : 32;
-  const dim3 grid(grid_rows(2 * (int64_t)T * c.kv_heads, lpr));
+  const int lpr = c.head_dim <= 64 ? 4 : c.head_dim <= 128 ? 8 : 16;
+  const dim3 grid(grid_rows((int64_t)T * c.kv_heads, lpr));
   const KvRead p{c, k, v, slots, T, make_fastdiv((uint32_t)c.kv_heads), make_fastdiv((uint32_t)c.page_size),
                  device_status_ptr(), pdl_enabled()};
-  auto go = [&](auto k8, auto k16, auto k32) {
-    return launch(lpr == 8 ? k8 : lpr == 16 ? k16 : k32, grid, 256, 0, stream, p.pdl, p);
+  auto go = [&](auto k4, auto k8, auto k16) {
+    return launch(lpr == 4 ? k4 : lpr == 8 ? k8 : k16, grid, 256, 0, stream, p.pdl, p);
   };
-#define NSQ_KV_GO(F, B) go(kv_read_kernel<F, B, 8>, kv_read_kernel<F, B, 16>, kv_read_kernel<F, B, 32>)
+#define NSQ_KV_GO(F, B) go(kv_read_kernel<F, B, 4>, kv_read_kernel<F, B, 8>, kv_read_kernel<F, B, 16>)
   if (fp8) return bf16 ? NSQ_KV_GO(true, true) : NSQ_KV_GO(true, false);
   return bf16 ? NSQ_KV_GO(false, true) : NSQ_KV_GO(false, false);
 #undef NSQ_KV_GO
