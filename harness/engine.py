@@ -12,7 +12,8 @@ at once, as BASELINE config 2 describes:
   * decode: one token per active request per step, as a replay of the graph
     captured for the smallest batch bucket that holds the active requests.
     The graph embeds, runs every layer (the quantized linears, RoPE, the
-    cache write, SDPA over the static cache), takes the argmax, appends it to
+    cache write, SDPA over the static cache -- or, with ``kv_cache``, the 8-bit
+    cache's write and decode attention), takes the argmax, appends it to
     a token history on the device and advances the positions, so the host
     only chooses the bucket: no host synchronisation between steps.
     Requests are placed in cache slots by descending output length, so the
@@ -32,13 +33,17 @@ from typing import List, Sequence
 
 import torch
 
+from nanosglang_b200.kv_cache import QuantizedKVCache
+
 from .model import CausalLM, apply_rope
 
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128)
 
 
 class DecodeEngine:
-    def __init__(self, model: CausalLM, max_slots: int, max_len: int, max_steps: int):
+    def __init__(self, model: CausalLM, max_slots: int, max_len: int, max_steps: int, kv_cache: str = "",
+                 page_size: int = 64):
+        """kv_cache: "" for the model's dtype, "int8" or "fp8" for an 8-bit paged cache."""
         cfg = model.config
         self.model = model
         dev = model.embed_tokens.weight.device
@@ -47,9 +52,19 @@ class DecodeEngine:
         attn0 = model.layers[0].self_attn
         kvh, hd = attn0.num_kv_heads, attn0.head_dim  # per-rank heads under tensor parallelism
         self.max_slots, self.max_len, self.max_steps = max_slots, max_len, max_steps
-        self.caches = [(torch.zeros(max_slots, kvh, max_len, hd, device=dev, dtype=dt),
-                        torch.zeros(max_slots, kvh, max_len, hd, device=dev, dtype=dt))
-                       for _ in range(cfg.num_hidden_layers)]
+        self.page_table = None
+        if kv_cache:
+            # slot i owns pages [i * width, (i + 1) * width): its token at position t is place i * width * page_size + t
+            width = (max_len + page_size - 1) // page_size
+            self.slot_tokens = width * page_size
+            self.page_table = torch.arange(max_slots * width, device=dev, dtype=torch.int32).view(max_slots, width)
+            self.first_place = torch.arange(max_slots, device=dev) * self.slot_tokens
+            self.caches = [(QuantizedKVCache(max_slots * width, page_size, kvh, hd, kv_cache, dev), None)
+                           for _ in range(cfg.num_hidden_layers)]
+        else:
+            self.caches = [(torch.zeros(max_slots, kvh, max_len, hd, device=dev, dtype=dt),
+                            torch.zeros(max_slots, kvh, max_len, hd, device=dev, dtype=dt))
+                           for _ in range(cfg.num_hidden_layers)]
         self.tokens = torch.zeros(max_slots, dtype=torch.long, device=dev)
         self.positions = torch.zeros(max_slots, dtype=torch.long, device=dev)
         self.history = torch.zeros(max_steps + 1, max_slots, dtype=torch.long, device=dev)
@@ -63,8 +78,11 @@ class DecodeEngine:
     # -- one decode step over the first bs slots (captured per bucket) --------
     def _step(self, bs: int):
         pos = self.positions[:bs]
-        mask = torch.zeros(bs, 1, 1, self.max_len, device=self.device, dtype=self.dtype)
-        mask.masked_fill_(self.cols[None, None, None, :] > pos[:, None, None, None], float("-inf"))
+        if self.page_table is not None:
+            mask = (self.first_place[:bs] + pos, self.page_table[:bs], (pos + 1).to(torch.int32))
+        else:
+            mask = torch.zeros(bs, 1, 1, self.max_len, device=self.device, dtype=self.dtype)
+            mask.masked_fill_(self.cols[None, None, None, :] > pos[:, None, None, None], float("-inf"))
         logits = self.model.forward_decode(self.tokens[:bs], pos, self.caches, mask)
         nxt = logits.argmax(dim=-1)
         self.tokens[:bs].copy_(nxt)
@@ -111,6 +129,10 @@ class DecodeEngine:
         starts = [0]
         for n in lens:
             starts.append(starts[-1] + n)
+        places = None
+        if self.page_table is not None:
+            places = positions + torch.cat([torch.full((n,), i * self.slot_tokens, device=self.device)
+                                            for i, n in enumerate(lens)])
         for layer, (kc, vc) in zip(model.layers, self.caches):
             attn = layer.self_attn
             x = layer.input_layernorm(h)
@@ -120,10 +142,13 @@ class DecodeEngine:
             v = attn.v_proj(x).view(-1, nkv, hd)
             q = apply_rope(q, model.rope_cos, model.rope_sin, positions)
             k = apply_rope(k, model.rope_cos, model.rope_sin, positions)
+            if places is not None:
+                kc.write(k, v, places)
             outs = []
             for slot, (a, b) in enumerate(zip(starts[:-1], starts[1:])):
-                kc[slot, :, :b - a] = k[a:b].transpose(0, 1)
-                vc[slot, :, :b - a] = v[a:b].transpose(0, 1)
+                if places is None:
+                    kc[slot, :, :b - a] = k[a:b].transpose(0, 1)
+                    vc[slot, :, :b - a] = v[a:b].transpose(0, 1)
                 o = torch.nn.functional.scaled_dot_product_attention(
                     q[a:b].transpose(0, 1)[None], k[a:b].transpose(0, 1)[None], v[a:b].transpose(0, 1)[None],
                     is_causal=True, scale=1.0 / math.sqrt(hd), enable_gqa=nh != nkv)

@@ -16,8 +16,9 @@ restatement against the reference model itself.
 
 The decode path used for throughput (``forward_decode``) is this harness's
 own: per-request positions in one batch over a static KV cache, written for
-CUDA-graph capture. Attention there is torch's SDPA; it is outside the path
-this repository rebuilds.
+CUDA-graph capture. Attention there is torch's SDPA over a 16-bit cache, or
+the library's decode attention over an 8-bit one
+(``nanosglang_b200.kv_cache.QuantizedKVCache``).
 """
 
 from __future__ import annotations
@@ -168,7 +169,10 @@ class Attention(nn.Module):
     def forward_decode(self, hidden_states, cos, sin, positions, k_cache, v_cache, mask):
         """One token per request (rows of a static cache): hidden (bs, hidden),
         positions (bs,), caches (slots, kv_heads, max_len, dim) whose first bs
-        slots are this batch, mask (bs, 1, 1, max_len) additive."""
+        slots are this batch, mask (bs, 1, 1, max_len) additive. With an 8-bit
+        cache: k_cache a QuantizedKVCache, v_cache None, mask (slots (bs,)
+        int64, page_table (bs, W) int32, seq_lens (bs,) int32, the new token
+        included)."""
         bs = hidden_states.shape[0]
         nh, nkv = self.num_heads, self.num_kv_heads
         q, k, v = self._qkv(hidden_states)
@@ -177,6 +181,11 @@ class Attention(nn.Module):
         v = v.reshape(bs, nkv, self.head_dim)
         q = apply_rope_full(q, cos, sin, positions)
         k = apply_rope_full(k, cos, sin, positions)
+        if v_cache is None:
+            slots, page_table, seq_lens = mask
+            k_cache.write(k, v, slots)
+            out = k_cache.attend(q, page_table, seq_lens)
+            return self.o_proj(out.reshape(bs, nh * self.head_dim))
         rows = torch.arange(bs, device=hidden_states.device)
         k_cache[rows, :, positions, :] = k
         v_cache[rows, :, positions, :] = v
@@ -195,7 +204,8 @@ class Attention(nn.Module):
         return self.q_proj(h), self.k_proj(h), self.v_proj(h)
 
     def forward_prefill(self, hidden_states, cos, sin, positions, k_cache, v_cache, slot):
-        """One request's prompt (seq, hidden) into cache slot ``slot`` (causal)."""
+        """One request's prompt (seq, hidden) into cache slot ``slot`` (causal);
+        with an 8-bit cache (v_cache None), ``slot`` holds the tokens' places (seq,) int64."""
         seq = hidden_states.shape[0]
         nh, nkv = self.num_heads, self.num_kv_heads
         q = self.q_proj(hidden_states).view(seq, nh, self.head_dim)
@@ -203,8 +213,11 @@ class Attention(nn.Module):
         v = self.v_proj(hidden_states).view(seq, nkv, self.head_dim)
         q = apply_rope(q, cos, sin, positions)
         k = apply_rope(k, cos, sin, positions)
-        k_cache[slot, :, :seq, :] = k.transpose(0, 1)
-        v_cache[slot, :, :seq, :] = v.transpose(0, 1)
+        if v_cache is None:
+            k_cache.write(k, v, slot)
+        else:
+            k_cache[slot, :, :seq, :] = k.transpose(0, 1)
+            v_cache[slot, :, :seq, :] = v.transpose(0, 1)
         out = F.scaled_dot_product_attention(q.transpose(0, 1).unsqueeze(0), k.transpose(0, 1).unsqueeze(0),
                                              v.transpose(0, 1).unsqueeze(0), is_causal=True,
                                              scale=1.0 / math.sqrt(self.head_dim), enable_gqa=nh != nkv)
@@ -291,7 +304,8 @@ class CausalLM(nn.Module):
         return self._rope_full
 
     def forward_decode(self, tokens, positions, caches, mask):
-        """tokens/positions (bs,), caches [(k, v)] per layer -> logits (bs, vocab)."""
+        """tokens/positions (bs,), caches [(k, v)] per layer, or [(QuantizedKVCache,
+        None)] with mask as in Attention.forward_decode -> logits (bs, vocab)."""
         h = self.embed_tokens(tokens)
         cos_full, sin_full = self.rope_tables(h.dtype)
         for layer, (kc, vc) in zip(self.layers, caches):

@@ -595,13 +595,16 @@ def _ptr_array(vals, ctype=None):
 
 def linear_multi(x: torch.Tensor, mods) -> Optional[list]:
     """One launch for 1..3 AWQLinear (or 1..3 FP8Linear) layers that read the
-    same x, e.g. q/k/v. Returns their outputs as views of one [M, sum N]
+    same x, e.g. q/k/v; Int8Linear layers share one quantisation of x (any M). Returns their outputs as views of one [M, sum N]
     buffer, or None when the fused kernel does not apply (M > 32, mixed
     formats, bias dtypes that differ, group sizes that differ)."""
     mods = [_unwrap(m) for m in mods]
     kinds = {type(m).__name__ for m in mods}
     if len(kinds) != 1 or x.dtype not in _ACT_CODES:
         return None
+    if kinds == {"Int8Linear"}:  # one quantisation of x for all, at any batch size
+        codes, scale = int8_quantize(x)
+        return [int8_linear_quantized(codes, scale, mm.weight_int8, mm.weight_scale, mm.bias, x.dtype) for mm in mods]
     k = x.shape[-1]
     lead = x.shape[:-1]
     x2 = _aligned(x.reshape(-1, k))
@@ -657,10 +660,14 @@ def linear_multi(x: torch.Tensor, mods) -> Optional[list]:
 def gate_up_silu(x: torch.Tensor, gate, up) -> Optional[torch.Tensor]:
     """SiLU(gate(x)) * up(x) in one launch (MLP.forward's inner expression,
     causal_lm.py:482) for AWQ or FP8 gate/up layers without bias; None when
-    the fused kernel does not apply (M > 32, bias, mismatched layers)."""
+    the fused kernel does not apply (M > 32, bias, mismatched layers). Int8Linear
+    layers share one quantisation of x and run as two products."""
     gate, up = _unwrap(gate), _unwrap(up)
     if type(gate) is not type(up) or x.dtype not in _ACT_CODES or gate.bias is not None or up.bias is not None:
         return None
+    if type(gate).__name__ == "Int8Linear":
+        g, u = linear_multi(x, (gate, up))
+        return torch.nn.functional.silu(g) * u
     k = x.shape[-1]
     lead = x.shape[:-1]
     x2 = _aligned(x.reshape(-1, k))

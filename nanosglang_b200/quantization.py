@@ -32,7 +32,7 @@ import torch.nn as nn
 
 from . import ops
 
-__all__ = ["FP8Linear", "AWQLinear", "quantize_model", "load_autoawq_state_dict", "FusedProjections", "GateUpSiLU"]
+__all__ = ["FP8Linear", "AWQLinear", "Int8Linear", "quantize_model", "load_autoawq_state_dict", "FusedProjections", "GateUpSiLU"]
 
 
 class FP8Linear(nn.Module):
@@ -128,9 +128,52 @@ class AWQLinear(nn.Module):
         return awq
 
 
+class Int8Linear(nn.Module):
+    """Linear layer in 8-bit integers on both sides (W8A8).
+
+    No counterpart in the reference; it takes the place of its quantised
+    linears. Buffers: ``weight_int8`` int8 [N, K], ``weight_scale`` float32 [N]
+    (one per output channel). ``forward`` quantises x per token, multiplies the
+    codes exactly in int32 and scales the sums: see ``ops.int8_linear``. As a
+    row-parallel shard, each rank quantises its own slice of x (a scale of its
+    own, so at least as fine as one over the whole row).
+    """
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False):
+        super().__init__()
+        self.in_features = in_features
+        self.out_features = out_features
+        self.register_buffer("weight_int8", torch.zeros(out_features, in_features, dtype=torch.int8))
+        self.register_buffer("weight_scale", torch.ones(out_features))
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(out_features))
+        else:
+            self.bias = None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return ops.int8_linear(x, self.weight_int8, self.weight_scale, self.bias)
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """``weight_int8 * weight_scale``, rounded once to dtype."""
+        return (self.weight_int8.float() * self.weight_scale[:, None]).to(dtype)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
+        """Quantise a Linear per output channel: scale = max|row| / 127 (1 if
+        the row is all zero), codes = rint(row / scale)."""
+        has_bias = linear.bias is not None
+        with torch.device(linear.weight.device):
+            out = cls(linear.in_features, linear.out_features, bias=has_bias)
+        out.weight_int8, out.weight_scale = ops.int8_quantize(linear.weight.data)
+        if has_bias:
+            out.bias = nn.Parameter(linear.bias.data.clone())
+        return out
+
+
 class FusedProjections(nn.Module):
     """Projections that read the same x (q/k/v), run as one launch for decode
-    batches (M <= 32) and as the separate layers otherwise.
+    batches (M <= 32) and as the separate layers otherwise; int8 layers share
+    one quantisation of x at any batch size.
 
     The layers stay where they are (``attn.q_proj`` etc.): this module keeps
     plain references, so the model's state_dict is unchanged. The reference
@@ -152,8 +195,9 @@ class FusedProjections(nn.Module):
 class GateUpSiLU(nn.Module):
     """``F.silu(gate_proj(x)) * up_proj(x)`` (causal_lm.py:482) as one launch
     for decode batches (M <= 32; the activation is applied in fp32 and
-    rounded once), the separate layers otherwise. Keeps plain references to
-    the two layers (the state_dict is unchanged)."""
+    rounded once), the separate layers otherwise; int8 layers share one
+    quantisation of x at any batch size. Keeps plain references to the two
+    layers (the state_dict is unchanged)."""
 
     def __init__(self, gate_proj: nn.Module, up_proj: nn.Module):
         super().__init__()
@@ -210,8 +254,12 @@ def _quantize_awq(child: nn.Linear, group_size: int) -> nn.Module:
     return AWQLinear.from_linear(child, group_size)
 
 
+def _quantize_int8(child: nn.Linear, group_size: int) -> nn.Module:
+    return Int8Linear.from_linear(child)
+
+
 # method name -> converter; the walk below is the reference's
-_QUANTIZERS = {"fp8": _quantize_fp8, "awq": _quantize_awq}
+_QUANTIZERS = {"fp8": _quantize_fp8, "awq": _quantize_awq, "int8": _quantize_int8}
 
 
 def quantize_model(
@@ -225,7 +273,8 @@ def quantize_model(
     Same walk as the reference (quantization.py:202-243): every child
     ``nn.Linear`` whose owning module name and full name contain none of
     ``skip_modules`` (default ``["embed_tokens", "lm_head", "norm"]``) is
-    replaced by its quantised form via ``setattr``.
+    replaced by its quantised form via ``setattr``. ``method``: the
+    reference's "fp8" and "awq" (16-bit activations), or "int8" (W8A8).
     """
     if skip_modules is None:
         skip_modules = ["embed_tokens", "lm_head", "norm"]

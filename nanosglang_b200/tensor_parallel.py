@@ -32,7 +32,7 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 
-from .quantization import AWQLinear, FP8Linear
+from .quantization import AWQLinear, FP8Linear, Int8Linear
 
 __all__ = [
     "init_distributed", "ColumnParallelLinear", "RowParallelLinear", "TPAttention", "TPMLP",
@@ -63,7 +63,7 @@ def init_distributed(rank: Optional[int] = None, world_size: Optional[int] = Non
 
 
 # ---------------------------------------------------------------------------
-# Sharding of one linear (dense, AWQ or FP8)
+# Sharding of one linear (dense, AWQ, FP8 or int8)
 # ---------------------------------------------------------------------------
 
 
@@ -75,7 +75,7 @@ def _span(total: int, world_size: int, rank: int, what: str):
 
 
 def shard_linear_rows(module: nn.Module, world_size: int, rank: int) -> nn.Module:
-    """Output-dim (column-parallel) shard of a dense / AWQ / FP8 linear."""
+    """Output-dim (column-parallel) shard of a dense / AWQ / FP8 / int8 linear."""
     if isinstance(module, AWQLinear):
         r0, r1 = _span(module.out_features, world_size, rank, "out_features")
         dev = module.qweight.device
@@ -93,6 +93,15 @@ def shard_linear_rows(module: nn.Module, world_size: int, rank: int) -> nn.Modul
             out = FP8Linear(module.in_features, r1 - r0, bias=module.bias is not None)
         out.weight_fp8 = module.weight_fp8[r0:r1].contiguous()
         out.weight_scale = module.weight_scale.clone()
+        if module.bias is not None:
+            out.bias = nn.Parameter(module.bias.data[r0:r1].clone())
+        return out
+    if isinstance(module, Int8Linear):
+        r0, r1 = _span(module.out_features, world_size, rank, "out_features")
+        with torch.device(module.weight_int8.device):
+            out = Int8Linear(module.in_features, r1 - r0, bias=module.bias is not None)
+        out.weight_int8 = module.weight_int8[r0:r1].contiguous()
+        out.weight_scale = module.weight_scale[r0:r1].clone()
         if module.bias is not None:
             out.bias = nn.Parameter(module.bias.data[r0:r1].clone())
         return out
@@ -130,6 +139,15 @@ def shard_linear_cols(module: nn.Module, world_size: int, rank: int, keep_bias: 
         with torch.device(module.weight_fp8.device):
             out = FP8Linear(c1 - c0, module.out_features, bias=has_bias)
         out.weight_fp8 = module.weight_fp8[:, c0:c1].contiguous()
+        out.weight_scale = module.weight_scale.clone()
+        if has_bias:
+            out.bias = nn.Parameter(module.bias.data.clone())
+        return out
+    if isinstance(module, Int8Linear):
+        c0, c1 = _span(module.in_features, world_size, rank, "in_features")
+        with torch.device(module.weight_int8.device):
+            out = Int8Linear(c1 - c0, module.out_features, bias=has_bias)
+        out.weight_int8 = module.weight_int8[:, c0:c1].contiguous()
         out.weight_scale = module.weight_scale.clone()
         if has_bias:
             out.bias = nn.Parameter(module.bias.data.clone())
@@ -378,7 +396,7 @@ class TPMLP(nn.Module):
 def tensor_parallel_model(model, world_size: int, rank: int):
     """Shard every decoder layer's projections in place (tensor_parallel.py:236-301).
 
-    Works for dense, AWQ and FP8 projections (quantize before or after), keeps
+    Works for dense, AWQ, FP8 and int8 projections (quantize before or after), keeps
     each shard on the layer's device and dtype, shards q/k/v biases with their
     rows, and updates the attention head counts for this rank.
     """
