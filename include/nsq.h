@@ -214,7 +214,8 @@ int nsq_fp8_quantize_noalloc(const void* w, int w_dtype, int64_t N, int64_t K, u
  * + bias, summed in int32 (exact), scaled in fp32 and rounded once; x_dtype is
  * F16 or BF16, y has the same. It launches the row quantiser into the
  * workspace (nsq_int8_linear_workspace_size(M, K) bytes, 16-byte aligned,
- * stream-ordered like y), then the product. A token with a NaN or an infinity
+ * stream-ordered like y), then the product; up to 8 tokens with few elements
+ * are one launch and need no workspace (size 0, may be NULL). A token with a NaN or an infinity
  * gives a row of NaN.
  *
  * nsq_int8_linear_quantized: the product alone, of codes the caller keeps

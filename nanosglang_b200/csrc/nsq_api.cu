@@ -630,11 +630,17 @@ int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* 
 
 constexpr int64_t kInt8MaxK = 131072;  // 128 * 127 * 131072 < 2^31
 
+// Few enough elements of x that every CTA of the rows kernel quantises them
+// all sooner than a kernel of its own would (full call, us, one launch vs two:
+// 1 x 896 -> 4864 3.7 vs 3.9, 1 x 4096 -> 4096 7.0 vs 7.6; but 8 x 896 -> 4864
+// 5.2 vs 4.0, 1 x 8192 -> 8192 20.4 vs 16.0).
+static bool int8_fused(int64_t M, int64_t K) { return M <= 8 && M * K <= 4096; }
+
 // Workspace: the codes, then (16-byte aligned) the scales.
 static size_t int8_codes_bytes(int64_t M, int64_t K) { return ((size_t)M * (size_t)K + 15) & ~(size_t)15; }
 
 size_t nsq_int8_linear_workspace_size(int64_t M, int64_t K) {
-  if (M <= 0 || K <= 0 || M > kIntMax || K > kInt8MaxK) return 0;
+  if (M <= 0 || K <= 0 || M > kIntMax || K > kInt8MaxK || int8_fused(M, K)) return 0;
   return int8_codes_bytes(M, K) + (size_t)M * sizeof(float);
 }
 
@@ -650,8 +656,22 @@ static int int8_check(int64_t M, int64_t K, int64_t N, const void* x, const int8
   return check_device();
 }
 
+// Decode batches: the weight rows through mma.sync, or tcgen05 tiles. Measured
+// on B200, CUDA-graph chains of distinct weights, us of the product (rows vs
+// tiles): M <= 8 rows throughout (4096 -> 4096 6.7 vs 11.2, 4096 -> 14336 13.5
+// vs 14.5; 16.2 vs 18.3 for 8192 -> 8192); M = 16 tiles from 48 rows per SM on
+// (4096 -> 14336 18.3 vs 13.9, 4096 -> 4096 7.4 vs 11.4, 14336 -> 4096 19.8 vs
+// 22.4); M = 32 tiles from K = 2048 on (4864 -> 896 16.7 vs 12.3, 896 -> 4864
+// 5.0 vs 6.6); above, rows only for the smallest (896 -> 896 at M = 64 4.6 vs 5.8).
+static bool int8_by_rows(int64_t M, int64_t K, int64_t N) {
+  if (M <= 8) return true;
+  if (M <= 16) return N < 48 * (int64_t)num_sms();
+  if (M <= 32) return K < 2048;
+  return M <= 64 && K * N <= ((int64_t)1 << 20);
+}
+
 static int int8_product(const Int8Args& a, cudaStream_t stream) {
-  return a.M <= 64 && (int64_t)a.K * a.N < ((int64_t)1 << 24) ? run_int8_rows(a, stream) : run_int8_gemm(a, stream);
+  return int8_by_rows(a.M, a.K, a.N) ? run_int8_rows(a, stream) : run_int8_gemm(a, stream);
 }
 
 int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N, const int8_t* weight_int8,
@@ -659,6 +679,11 @@ int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N,
                     size_t workspace_bytes, void* stream) {
   int rc = int8_check(M, K, N, x, weight_int8, weight_scale, bias, bias_dtype, y, x_dtype);
   if (rc != NSQ_OK || M == 0) return rc;
+  if (int8_fused(M, K)) {
+    return run_int8_rows(Int8Args{nullptr, nullptr, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
+                                  x_dtype == NSQ_DTYPE_BF16, y, false, x},
+                         static_cast<cudaStream_t>(stream));
+  }
   if (!workspace || workspace_bytes < nsq_int8_linear_workspace_size(M, K)) return NSQ_EWORKSPACE;
   if (!aligned16(workspace)) return NSQ_EALIGN;
   int8_t* codes = static_cast<int8_t*>(workspace);
@@ -666,7 +691,7 @@ int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (launch_int8_quantize(x, x_dtype, M, K, codes, scale, s) != cudaSuccess) return NSQ_ECUDA;
   return int8_product(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
-                               x_dtype == NSQ_DTYPE_BF16, y, true},
+                               x_dtype == NSQ_DTYPE_BF16, y, true, nullptr},
                       s);
 }
 
@@ -677,7 +702,7 @@ int nsq_int8_linear_quantized(const int8_t* codes, const float* scale, int64_t M
   if (rc != NSQ_OK || M == 0) return rc;
   if (!scale) return NSQ_EINVAL;
   return int8_product(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
-                               y_dtype == NSQ_DTYPE_BF16, y, false},
+                               y_dtype == NSQ_DTYPE_BF16, y, false, nullptr},
                       static_cast<cudaStream_t>(stream));
 }
 

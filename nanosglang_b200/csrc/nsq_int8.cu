@@ -129,6 +129,7 @@ __device__ __forceinline__ void dsmem_add(uint32_t cluster_addr, int v) {
 
 struct RowsParams {
   const int8_t* x;
+  const uint16_t* x16;  // FUSED: x itself
   const float* xscale;
   const int8_t* w;
   const float* wscale;
@@ -140,10 +141,42 @@ struct RowsParams {
   int split;  // CTAs of a cluster, along K
 };
 
+// The block's part of FUSED: token m's row by kRWarps / tokens warps (tokens
+// rounded up to a power of two), its maximum, then its codes (the second read
+// hits L1). Called by every thread once.
+template <bool BF16>
+__device__ __forceinline__ void rows_quantize(const RowsParams& p, int8_t* xs, int ldx, uint32_t* xmax_s,
+                                              float* xscale_s) {
+  if (p.pdl_x) pdl_wait_prior_grids();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = p.M == 1 ? 8 : p.M == 2 ? 4 : p.M <= 4 ? 2 : 1;  // warps per token
+  const int m = warp / per;
+  const bool in = m < p.M;
+  const uint4* src = reinterpret_cast<const uint4*>(p.x16 + (int64_t)(in ? m : 0) * p.K);
+  const int nvec = in ? p.K / 8 : 0, first = (warp % per) * 32 + lane;
+  uint32_t mx = 0;
+  for (int i = first; i < nvec; i += per * 32) mx = abs_max2(mx, __ldg(src + i));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) xmax_s[warp] = mx;
+  __syncthreads();
+  for (int i = 0; i < per; ++i) mx = __vmaxu2(mx, xmax_s[m * per + i]);
+  const float s = row_scale<false>(abs_max_value<BF16>(mx));
+  if (in && first == 0) xscale_s[m] = s;
+  const RowDiv dv(s);
+  for (int i = first; i < nvec; i += per * 32) {
+    *reinterpret_cast<uint2*>(xs + m * ldx + i * 8) = row_codes8<false, BF16>(dv, __ldg(src + i));
+  }
+  __syncthreads();
+}
+
 // 16 weight rows x 8 * MT tokens per cluster of `split` CTAs along K. The warps
 // of all of them take 64-column chunks in turn and add their int32 sums in the
 // first CTA's shared memory (exact, so the order is free).
-template <int MT, bool BF16>
+// FUSED (up to 8 tokens, few elements): x is 16-bit; every CTA quantises all of
+// it into its shared memory while its first weights are on their way, which
+// takes less time than a launch of the row quantiser and its round trip.
+template <int MT, bool BF16, bool FUSED>
 __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParams p) {
   constexpr int kLd = 8 * MT + 1;
   __shared__ int acc_s[16][kLd];
@@ -152,7 +185,12 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
   const int rank = blockIdx.x % p.split;  // the cluster's rank along x
   const int n0 = blockIdx.x / p.split * 16, m0 = blockIdx.y * (8 * MT);
   for (int i = threadIdx.x; i < 16 * kLd; i += kRWarps * 32) (&acc_s[0][0])[i] = 0;
-  bool waiting = p.pdl_x;
+  extern __shared__ uint4 xs_raw[];  // FUSED: codes [M][ldx]; rows 64 bytes apart modulo 128: no bank conflicts
+  int8_t* const xs = reinterpret_cast<int8_t*>(xs_raw);
+  const int ldx = (p.K + 127) / 128 * 128 + 64;
+  __shared__ uint32_t xmax_s[kRWarps];
+  __shared__ float xscale_s[8];
+  bool waiting = FUSED || p.pdl_x;
   const int8_t* w0 = p.w + (int64_t)(n0 + g) * p.K;
   const int8_t* w1 = w0 + (int64_t)8 * p.K;
   const bool r0 = n0 + g < p.N, r1 = n0 + g + 8 < p.N;
@@ -163,6 +201,7 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
   // warps of the SM, 64 KB and more in flight
   constexpr int kAhead = MT <= 2 ? 4 : 2;
   const int step = p.split * kRWarps * 64;
+  // FUSED: every warp goes once round at least, for the block's quantisation
   for (int k0 = (rank * kRWarps + warp) * 64; k0 < p.K; k0 += kAhead * step) {
     uint4 a[kAhead], c[kAhead];
     const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -172,7 +211,10 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
       a[j] = k < p.K && r0 ? ldg_w(w0 + k) : zero;
       c[j] = k < p.K && r1 ? ldg_w(w1 + k) : zero;
     }
-    if (waiting) {  // the first weights are on their way while the codes of x are made
+    if constexpr (FUSED) {
+      if (waiting) rows_quantize<BF16>(p, xs, ldx, xmax_s, xscale_s);
+      waiting = false;
+    } else if (waiting) {  // the first weights are on their way while the codes of x are made
       pdl_wait_prior_grids();
       waiting = false;
     }
@@ -183,13 +225,23 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int m = m0 + 8 * i + g;
-        const uint4 b = k < p.K && m < p.M ? *reinterpret_cast<const uint4*>(p.x + (int64_t)m * p.K + k) : zero;
+        uint4 b = zero;
+        if (k < p.K && m < p.M) {
+          b = FUSED ? *reinterpret_cast<const uint4*>(xs + m * ldx + k)
+                    : *reinterpret_cast<const uint4*>(p.x + (int64_t)m * p.K + k);
+        }
         mma_16832_s8(d[i], a[j].x, c[j].x, a[j].y, c[j].y, b.x, b.y);
         mma_16832_s8(d[i], a[j].z, c[j].z, a[j].w, c[j].w, b.z, b.w);
       }
     }
   }
-  if (waiting) pdl_wait_prior_grids();
+  if (waiting) {
+    if constexpr (FUSED) {
+      rows_quantize<BF16>(p, xs, ldx, xmax_s, xscale_s);
+    } else {
+      pdl_wait_prior_grids();
+    }
+  }
   const uint32_t acc0 = smem_u32(acc_s);
   if (p.split > 1) {
     cluster_sync_all();  // the first CTA's sums are zero
@@ -218,7 +270,7 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
   for (int i = threadIdx.x; i < 16 * 8 * MT; i += kRWarps * 32) {
     const int n = n0 + (i & 15), m = m0 + (i >> 4);
     if (n < p.N && m < p.M) {
-      const float y = (float)acc_s[i & 15][i >> 4] * p.xscale[m] * __ldg(p.wscale + n);
+      const float y = (float)acc_s[i & 15][i >> 4] * (FUSED ? xscale_s[m] : p.xscale[m]) * __ldg(p.wscale + n);
       const float bn = load_bias(p.bias, p.bias_dtype, n);
       static_cast<uint16_t*>(p.y)[(int64_t)m * p.N + n] = float_to_elem<BF16>(p.bias ? y + bn : y);
     }
@@ -226,10 +278,11 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
 }
 
 template <typename F, typename... A>
-cudaError_t launch(F kern, dim3 grid, int threads, int cluster, cudaStream_t stream, bool pdl, A... args) {
+cudaError_t launch(F kern, dim3 grid, int threads, int smem, int cluster, cudaStream_t stream, bool pdl, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   int n = 0;
@@ -256,7 +309,7 @@ static cudaError_t quantize_rows(const uint16_t* x, int M, int K, int8_t* codes,
                                  bool pdl) {
   const dim3 grid((unsigned)((M + kQThreads / TPR - 1) / (kQThreads / TPR)));
   const int per = (K / 8 + TPR - 1) / TPR;
-  auto go = [&](auto kern) { return launch(kern, grid, kQThreads, 1, stream, pdl, x, M, K, codes, scale, (int)pdl); };
+  auto go = [&](auto kern) { return launch(kern, grid, kQThreads, 0, 1, stream, pdl, x, M, K, codes, scale, (int)pdl); };
   return per <= 1   ? go(int8_quantize_kernel<TPR, 1, BF16>)
          : per <= 2 ? go(int8_quantize_kernel<TPR, 2, BF16>)
          : per <= 4 ? go(int8_quantize_kernel<TPR, 4, BF16>)
@@ -269,7 +322,7 @@ cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t
   const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 8 * 8 * kQThreads &&
                    ((reinterpret_cast<uintptr_t>(x) & 15) | (reinterpret_cast<uintptr_t>(codes) & 7)) == 0;
   if (!vec) {
-    return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 1, stream, pdl, x, dtype, K, codes, scale,
+    return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 0, 1, stream, pdl, x, dtype, K, codes, scale,
                   (int)pdl);
   }
   const uint16_t* x16 = static_cast<const uint16_t*>(x);
@@ -286,8 +339,9 @@ cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t
 }
 
 int run_int8_rows(const Int8Args& a, cudaStream_t stream) {
-  RowsParams p{a.x, a.xscale, a.w, a.wscale, a.bias, a.bias ? a.bias_dtype : NSQ_DTYPE_NONE, a.y, a.M, a.K, a.N,
-               a.after_quantize || pdl_enabled(), 1};
+  const bool fused = a.x16 != nullptr;
+  RowsParams p{a.x, static_cast<const uint16_t*>(a.x16), a.xscale, a.w, a.wscale, a.bias,
+               a.bias ? a.bias_dtype : NSQ_DTYPE_NONE, a.y, a.M, a.K, a.N, a.after_quantize || pdl_enabled(), 1};
   const int mt = a.M <= 8 ? 1 : a.M <= 16 ? 2 : a.M <= 32 ? 4 : 8;
   const int64_t tiles = (int64_t)((a.N + 15) / 16) * ((a.M + 8 * mt - 1) / (8 * mt));
   // K over a cluster while the CTAs do not fill two per SM and each has 1024
@@ -296,10 +350,15 @@ int run_int8_rows(const Int8Args& a, cudaStream_t stream) {
   // (at M = 16 10.8 -> 11.9 us)
   while (mt == 1 && p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && a.K / (2 * p.split) >= 1024) p.split *= 2;
   const dim3 grid((unsigned)((a.N + 15) / 16 * p.split), (unsigned)((a.M + 8 * mt - 1) / (8 * mt)));
-#define NSQ_R(MT)                                                                                      \
-  (a.y_bf16 ? launch(int8_rows_kernel<MT, true>, grid, kRWarps * 32, p.split, stream, p.pdl_x, p)      \
-            : launch(int8_rows_kernel<MT, false>, grid, kRWarps * 32, p.split, stream, p.pdl_x, p))
-  const cudaError_t e = mt == 1 ? NSQ_R(1) : mt == 2 ? NSQ_R(2) : mt == 4 ? NSQ_R(4) : NSQ_R(8);
+  const int smem = fused ? a.M * ((a.K + 127) / 128 * 128 + 64) : 0;
+#define NSQ_R(MT, F)                                                                                              \
+  (a.y_bf16 ? launch(int8_rows_kernel<MT, true, F>, grid, kRWarps * 32, smem, p.split, stream, p.pdl_x, p)        \
+            : launch(int8_rows_kernel<MT, false, F>, grid, kRWarps * 32, smem, p.split, stream, p.pdl_x, p))
+  const cudaError_t e = fused     ? NSQ_R(1, true)
+                        : mt == 1 ? NSQ_R(1, false)
+                        : mt == 2 ? NSQ_R(2, false)
+                        : mt == 4 ? NSQ_R(4, false)
+                                  : NSQ_R(8, false);
 #undef NSQ_R
   return e == cudaSuccess ? NSQ_OK : NSQ_ECUDA;
 }

@@ -62,6 +62,7 @@ struct Int8Args {
   int y_bf16;
   void* y;  // [M, N]
   bool after_quantize;  // the kernel ahead on the stream is launch_int8_quantize's, writing x and xscale
+  const void* x16;      // run_int8_rows, up to 8 tokens: x itself (16-bit, of y's type) instead of x and xscale
 };
 int run_int8_rows(const Int8Args& a, cudaStream_t stream);  // mma.sync, weight rows streamed: decode batches
 int run_int8_gemm(const Int8Args& a, cudaStream_t stream);  // tcgen05 tiles: larger ones

@@ -395,10 +395,11 @@ def int8_linear(x: torch.Tensor, weight_int8: torch.Tensor, weight_scale: torch.
         x2 = _aligned(x2)
     m = x2.shape[0]
     y = x2.new_empty((m, n))
-    nbytes = (m * k + 15 & ~15) + 4 * m  # nsq_int8_linear_workspace_size
-    work = x2.new_empty(nbytes, dtype=torch.uint8)
+    nbytes = _lib.load().nsq_int8_linear_workspace_size(m, k)
+    work = x2.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _call(dev, "nsq_int8_linear", x2.data_ptr(), code, m, k, n, w.data_ptr(), ws.data_ptr(),
-          None if b is None else b.data_ptr(), bcode, y.data_ptr(), work.data_ptr(), nbytes, _stream_on(dev))
+          None if b is None else b.data_ptr(), bcode, y.data_ptr(), None if work is None else work.data_ptr(), nbytes,
+          _stream_on(dev))
     return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
 
 

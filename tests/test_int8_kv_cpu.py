@@ -24,8 +24,9 @@ def test_int8_linear_refusals():
     assert _int8(w=FAKE + 8) == _lib.EALIGN
     assert _int8(m=0) == _lib.OK  # nothing to do, needs no device
     lib = _lib.load()
-    need = lib.nsq_int8_linear_workspace_size(5, 48)
-    assert need == 5 * 48 + 5 * 4
+    assert lib.nsq_int8_linear_workspace_size(9, 48) == 9 * 48 + 9 * 4
+    assert lib.nsq_int8_linear_workspace_size(8, 528) == 8 * 528 + 8 * 4
+    assert lib.nsq_int8_linear_workspace_size(8, 512) == 0  # one launch
     assert lib.nsq_int8_linear_workspace_size(0, 48) == 0
     assert lib.nsq_int8_quantize(FAKE, 7, 1, 8, FAKE, FAKE, None) == _lib.EINVAL
     assert lib.nsq_int8_quantize(FAKE, 1, 1, 0, FAKE, FAKE, None) == _lib.EINVAL
