@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
       if (r >= rows) break;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(j ? p.v : p.k) + (int64_t)r * p.c.head_dim + sub * 16);
+        uint16_t* out = static_cast<uint16_t*>(j ? p.v : p.k) + (int64_t)r * p.c.head_dim + sub * 16;
+        uint4* dst = reinterpret_cast<uint4*>(out);
         const uint2 v0 = values4<FP8, BF16>(c[i][j].x, s[i][j]), v1 = values4<FP8, BF16>(c[i][j].y, s[i][j]);
         const uint2 v2 = values4<FP8, BF16>(c[i][j].z, s[i][j]), v3 = values4<FP8, BF16>(c[i][j].w, s[i][j]);
         dst[0] = make_uint4(v0.x, v0.y, v1.x, v1.y);
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 constexpr int kAttnWarps = 4;
 constexpr int kTile = 32;  // tokens of a stage
 constexpr int kWhole = 4;  // stages of an item that is not cut
+constexpr int kHeads = 8;  // query heads of an item: the columns of an MMA
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -349,19 +351,18 @@ __device__ __forceinline__ int item_units(const KvAttn& p, int n) {
 // HALVES x 16 rows of RB bytes (swizzled in RB-byte rows as TMA does), the 64
 // scales and a mask of the tokens to attend to.
 constexpr int kScaleBytes = 272;
-template <int DP, int NT>
+template <int DP>
 struct AttnShape {
   static constexpr int RB = DP < 128 ? DP : 128;  // bytes of a tile row
   static constexpr int HALVES = DP / RB;
   static constexpr int kTileBytes = 16 * DP;
   static constexpr int kStage = 4 * kTileBytes;
   static constexpr int kStages = DP == 64 ? 4 : 2;
-  static constexpr int HEADS = 8 * NT;
   static constexpr int kScale = kAttnWarps * kStages * kStage;
   static constexpr int kBar = kScale + kAttnWarps * kStages * kScaleBytes;
   static constexpr int kAlloc = kBar + kAttnWarps * kStages * 8 + 1024;
   static constexpr int kCtas = 227 * 1024 / (kAlloc + 1024);
-  static constexpr int kPerSm = DP * NT <= 128 ? (kCtas < 3 ? kCtas : 3) : (kCtas < 2 ? kCtas : 2);
+  static constexpr int kPerSm = kCtas < 3 ? kCtas : 3;
 };
 
 // A worker's place: stage s (of 32 tokens) of item (b, kh), in the segment of
@@ -401,15 +402,14 @@ __device__ __forceinline__ int row_token(int i) {
   return RB == 128 ? i : (i & 12) | ((i & 1) << 1) | ((i >> 1) & 1);
 }
 
-template <int DP, int NT, bool FP8, bool BF16, bool TMA>
-__global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv_attn_kernel(
+template <int DP, bool FP8, bool BF16, bool TMA>
+__global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_attn_kernel(
     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const KvAttn p) {
-  using S = AttnShape<DP, NT>;
+  using S = AttnShape<DP>;
   constexpr int RB = S::RB, HALVES = S::HALVES;
   constexpr int KCH = RB / 16;     // 16-byte chunks of a tile row
   constexpr int MT = DP / 16;      // 16-dim tiles of the output
   constexpr int VW = RB / 32;      // words of a v row per lane and half
-  constexpr int HEADS = S::HEADS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ long long s_scan[kAttnWarps];
@@ -420,7 +420,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar) + warp * S::kStages;
   const uint32_t ring = smem_u32(smem) + warp * S::kStages * S::kStage;
   const uint32_t ring_sc = smem_u32(smem) + S::kScale + warp * S::kStages * kScaleBytes;  // scales, mask
-  if (lane < S::kStages) mbar_init(&full[lane], 33);  // the lanes' copies, and one arrival of lane 0 (TMA: with the bytes)
+  // a phase: the lanes' copies, and one arrival of lane 0 (TMA: with the bytes)
+  if (lane < S::kStages) mbar_init(&full[lane], 33);
   fence_barrier_init();
   if (p.pdl) pdl_wait_prior_grids();
   pdl_launch_dependents();  // the join's blocks may queue up behind this grid's; they wait for its end
@@ -595,9 +596,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
           const int d = half * RB + 16 * c;
           const bool ok = pr >= 0 && d < p.c.head_dim;
           const uint32_t at = dst + h * S::kTileBytes + half * 16 * RB + tile_at<RB>(row, c);
-          cp_async16(at, ok ? kb + mul_wide(pr, p.c.k_stride[0]) + mul_wide(orow, p.c.k_stride[1]) + d : p.c.k, ok ? 16 : 0);
-          cp_async16(at + 2 * S::kTileBytes,
-                     ok ? vb + mul_wide(pr, p.c.v_stride[0]) + mul_wide(orow, p.c.v_stride[1]) + d : p.c.v, ok ? 16 : 0);
+          const int64_t ko = mul_wide(pr, p.c.k_stride[0]) + mul_wide(orow, p.c.k_stride[1]) + d;
+          const int64_t vo = mul_wide(pr, p.c.v_stride[0]) + mul_wide(orow, p.c.v_stride[1]) + d;
+          cp_async16(at, ok ? kb + ko : p.c.k, ok ? 16 : 0);
+          cp_async16(at + 2 * S::kTileBytes, ok ? vb + vo : p.c.v, ok ? 16 : 0);
         }
       }
     }
@@ -645,66 +647,60 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
     // ---- one segment of item (b, kh) ----
     const int b = cur.b;
     const int head = cur.kh / p.head_blocks;
-    const int hb0 = (cur.kh - head * p.head_blocks) * HEADS;  // first query head of this block within the group
+    const int hb0 = (cur.kh - head * p.head_blocks) * kHeads;  // first query head of this block within the group
     // q as the B operand: lane (g, t) holds head g, dims 16 j + 4 t + 0..3 of every j
-    uint32_t qf[NT][MT][2];
-    float sc[NT][2];  // score scale of heads 2t, 2t + 1
+    uint32_t qf[MT][2];
+    float sc[2];  // score scale of heads 2t, 2t + 1
+    const int hl = hb0 + g;
+    const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
+                           (int64_t)(head * p.group + (hl < p.group ? hl : 0)) * p.q_stride[1];
+    float m = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int hl = hb0 + nt * 8 + g;
-      const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
-                             (int64_t)(head * p.group + (hl < p.group ? hl : 0)) * p.q_stride[1];
-      float m = 0.f;
+    for (int j = 0; j < MT; ++j) {
+      const int d = 16 * j + 4 * t;
+      uint2 x = make_uint2(0, 0);
+      if (hl < p.group && d < p.c.head_dim) x = __ldg(reinterpret_cast<const uint2*>(qrow + d));
+      qf[j][0] = x.x;
+      qf[j][1] = x.y;
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int d = 16 * j + 4 * t;
-        const uint2 x = hl < p.group && d < p.c.head_dim ? __ldg(reinterpret_cast<const uint2*>(qrow + d)) : make_uint2(0, 0);
-        qf[nt][j][0] = x.x;
-        qf[nt][j][1] = x.y;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)qf[nt][j][i])));
-          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)(qf[nt][j][i] >> 16))));
-        }
+      for (int i = 0; i < 2; ++i) {
+        m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)qf[j][i])));
+        m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)(qf[j][i] >> 16))));
       }
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      // the largest lands in [1, 2): e = its exponent, applied in two steps so
-      // that neither factor leaves fp32's range
-      const int e = m > 0.f && m <= 3.4e38f ? ilogbf(m) : 0;
-      const float f1 = exp2f((float)(-e / 2)), f2 = exp2f((float)(-e - (-e / 2)));
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          qf[nt][j][i] = pack_f16(elem_to_float<BF16>((uint16_t)qf[nt][j][i]) * f1 * f2,
-                                  elem_to_float<BF16>((uint16_t)(qf[nt][j][i] >> 16)) * f1 * f2);
-        }
-      }
-      const float s = p.scale_log2 / f1 / f2;
-      sc[nt][0] = __shfl_sync(0xffffffffu, s, (2 * t) * 4);
-      sc[nt][1] = __shfl_sync(0xffffffffu, s, (2 * t + 1) * 4);
     }
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    // the largest lands in [1, 2): e = its exponent, applied in two steps so
+    // that neither factor leaves fp32's range
+    const int e = m > 0.f && m <= 3.4e38f ? ilogbf(m) : 0;
+    const float f1 = exp2f((float)(-e / 2)), f2 = exp2f((float)(-e - (-e / 2)));
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        qf[j][i] = pack_f16(elem_to_float<BF16>((uint16_t)qf[j][i]) * f1 * f2,
+                            elem_to_float<BF16>((uint16_t)(qf[j][i] >> 16)) * f1 * f2);
+      }
+    }
+    const float s = p.scale_log2 / f1 / f2;
+    sc[0] = __shfl_sync(0xffffffffu, s, (2 * t) * 4);
+    sc[1] = __shfl_sync(0xffffffffu, s, (2 * t + 1) * 4);
 
-    float o[MT][NT][4];
+    float o[MT][4];
     // references m and m' (kNoMax: no term yet), 2^(m - m'), denominators (this lane's tokens)
-    float mx[NT][2], mv[NT][2], vf[NT][2], l[NT][2];
+    float mx[2], mv[2], vf[2], l[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int j = 0; j < MT; ++j) o[j][nt][0] = o[j][nt][1] = o[j][nt][2] = o[j][nt][3] = 0.f;
-      mx[nt][0] = mx[nt][1] = mv[nt][0] = mv[nt][1] = kNoMax;
-      vf[nt][0] = vf[nt][1] = l[nt][0] = l[nt][1] = 0.f;
-    }
+    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    mx[0] = mx[1] = mv[0] = mv[1] = kNoMax;
+    vf[0] = vf[1] = l[0] = l[1] = 0.f;
 
     auto step = [&](int slot) {
       const uint32_t kt = ring + slot * S::kStage, vt = kt + 2 * S::kTileBytes, st = ring_sc + slot * kScaleBytes;
-      float s[2][NT][4];
+      float s[2][4];
       const uint32_t there = __float_as_uint(lds_f32(st + 256));  // the tokens to attend to
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[h][nt][0] = s[h][nt][1] = s[h][nt][2] = s[h][nt][3] = 0.f;
+        s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
 #pragma unroll
         for (int half = 0; half < HALVES; ++half) {
 #pragma unroll
@@ -715,10 +711,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
             for (int j = 0; j < 2; ++j) {
               codes_to_f16<FP8>(r[2 * j], a[0], a[2]);
               codes_to_f16<FP8>(r[2 * j + 1], a[1], a[3]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_16816<false>(s[h][nt], a, qf[nt][half * KCH + c + j][0], qf[nt][half * KCH + c + j][1]);
-              }
+              mma_16816<false>(s[h], a, qf[half * KCH + c + j][0], qf[half * KCH + c + j][1]);
             }
           }
         }
@@ -734,10 +727,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
           const float ks = lds_f32(st + h * 128 + tok * 4);
           vs[h][r] = lds_f32(st + h * 128 + 64 + tok * 4);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) s[h][nt][2 * r + e] *= ks * sc[nt][e];
-          }
+          for (int e = 0; e < 2; ++e) s[h][2 * r + e] *= ks * sc[e];
         }
       }
       if (there != 0xffffffffu) {
@@ -746,94 +736,78 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             if ((there >> (16 * h + row_token<RB>(g) + 8 * r)) & 1) continue;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[h][nt][2 * r] = s[h][nt][2 * r + 1] = -INFINITY;
+            s[h][2 * r] = s[h][2 * r + 1] = -INFINITY;
           }
         }
       }
-      float top[NT][2];
+      float top[2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e]));
-          over |= top[nt][e] > mx[nt][e] + 8.f;
-        }
+      for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(fmaxf(s[0][e], s[0][2 + e]), fmaxf(s[1][e], s[1][2 + e]));
+        over |= top[e] > mx[e] + 8.f;
       }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int e = 0; e < 2; ++e) {
+          float a = top[e];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float a = top[nt][e];
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-            if (a > mx[nt][e]) {
-              l[nt][e] *= ex2(mx[nt][e] - a);
-              mx[nt][e] = a;
-              vf[nt][e] = weight_factor(a, mv[nt][e]);
-            }
+          for (int d = 4; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+          if (a > mx[e]) {
+            l[e] *= ex2(mx[e] - a);
+            mx[e] = a;
+            vf[e] = weight_factor(a, mv[e]);
           }
         }
       }
-      float wt[2][NT][4];
+      float wt[2][4];
       over = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int e = 0; e < 2; ++e) {
+        float big = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float x = ex2(s[h][2 * r + e] - mx[e]);
+            l[e] += x;
+            wt[h][2 * r + e] = x * (vs[h][r] * vf[e]);
+            big = fmaxf(big, wt[h][2 * r + e]);
+          }
+        }
+        over |= big > 4096.f || mv[e] == kNoMax;
+      }
+      if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float big = 0.f;
+          float v = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) v = fmaxf(v, s[h][2 * r + e] + lg2(vs[h][r]));
+          }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+          if (v > mv[e]) {
+            const float f = ex2(mv[e] - v);
+            mv[e] = v;
+            vf[e] = weight_factor(mx[e], v);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) o[j][e] *= f, o[j][2 + e] *= f;
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const float x = ex2(s[h][nt][2 * r + e] - mx[nt][e]);
-              l[nt][e] += x;
-              wt[h][nt][2 * r + e] = x * (vs[h][r] * vf[nt][e]);
-              big = fmaxf(big, wt[h][nt][2 * r + e]);
-            }
-          }
-          over |= big > 4096.f || mv[nt][e] == kNoMax;
-        }
-      }
-      if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-              for (int r = 0; r < 2; ++r) v = fmaxf(v, s[h][nt][2 * r + e] + lg2(vs[h][r]));
-            }
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-            if (v > mv[nt][e]) {
-              const float f = ex2(mv[nt][e] - v);
-              mv[nt][e] = v;
-              vf[nt][e] = weight_factor(mx[nt][e], v);
-#pragma unroll
-              for (int j = 0; j < MT; ++j) o[j][nt][e] *= f, o[j][nt][2 + e] *= f;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                wt[h][nt][2 * r + e] = ex2(s[h][nt][2 * r + e] - mx[nt][e]) * (vs[h][r] * vf[nt][e]);
-              }
+              wt[h][2 * r + e] = ex2(s[h][2 * r + e] - mx[e]) * (vs[h][r] * vf[e]);
             }
           }
         }
       }
-      uint32_t pb[2][NT][2];
+      uint32_t pb[2][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) pb[h][nt][r] = movmatrix_trans(pack_f16(wt[h][nt][2 * r], wt[h][nt][2 * r + 1]));
-        }
+        for (int r = 0; r < 2; ++r) pb[h][r] = movmatrix_trans(pack_f16(wt[h][2 * r], wt[h][2 * r + 1]));
       }
       // dims 2j, 2j + 1 of this lane's 16 (or 8) are rows g, g + 8 of output tile j
 #pragma unroll
@@ -870,11 +844,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
             codes_to_f16<FP8>(prmt(v[2][j], v[3][j], 0x5140), a[2], a[3]);
             codes_to_f16<FP8>(prmt(v[0][j], v[1][j], 0x7362), c[0], c[1]);
             codes_to_f16<FP8>(prmt(v[2][j], v[3][j], 0x7362), c[2], c[3]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_16816<false>(o[half * (RB / 16) + 2 * j][nt], a, pb[h][nt][0], pb[h][nt][1]);
-              mma_16816<false>(o[half * (RB / 16) + 2 * j + 1][nt], c, pb[h][nt][0], pb[h][nt][1]);
-            }
+            mma_16816<false>(o[half * (RB / 16) + 2 * j], a, pb[h][0], pb[h][1]);
+            mma_16816<false>(o[half * (RB / 16) + 2 * j + 1], c, pb[h][0], pb[h][1]);
           }
         }
       }
@@ -902,49 +873,46 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
     const bool whole = opens && closes;
     const long long slot = 2 * me + (first ? 0 : 1);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
-        const int h = nt * 8 + 2 * t + e;
-        if (hb0 + h >= p.group) continue;
-        const float m = mx[nt][e], mm = mv[nt][e], sum = l[nt][e];
-        const int64_t row = (int64_t)b * p.H + head * p.group + hb0 + h;
-        float* ws = whole ? nullptr : p.partial + (slot * p.slot_heads + h) * (DP + 4);
-        if (g == 0) {
-          if (whole) {
-            if (p.lse != nullptr) p.lse[row] = head_lse(sum, m);
-          } else {
-            *reinterpret_cast<float4*>(ws) = make_float4(m, mm, sum, 0.f);
-          }
+      for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+      const int h = 2 * t + e;
+      if (hb0 + h >= p.group) continue;
+      const float m = mx[e], mm = mv[e], sum = l[e];
+      const int64_t row = (int64_t)b * p.H + head * p.group + hb0 + h;
+      float* ws = whole ? nullptr : p.partial + (slot * p.slot_heads + h) * (DP + 4);
+      if (g == 0) {
+        if (whole) {
+          if (p.lse != nullptr) p.lse[row] = head_lse(sum, m);
+        } else {
+          *reinterpret_cast<float4*>(ws) = make_float4(m, mm, sum, 0.f);
         }
+      }
 #pragma unroll
-        for (int half = 0; half < HALVES; ++half) {
-          const int d0 = half * RB + g * (RB / 8);
+      for (int half = 0; half < HALVES; ++half) {
+        const int d0 = half * RB + g * (RB / 8);
 #pragma unroll
-          for (int c = 0; c < RB / 64; ++c) {  // 8 dims at a time
-            float y[8];
+        for (int c = 0; c < RB / 64; ++c) {  // 8 dims at a time
+          float y[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              y[2 * j] = o[half * (RB / 16) + 4 * c + j][nt][e];
-              y[2 * j + 1] = o[half * (RB / 16) + 4 * c + j][nt][2 + e];
-            }
-            if (whole) {
-              if (d0 + 8 * c < p.c.head_dim) {
-                uint32_t w[4];
+          for (int j = 0; j < 4; ++j) {
+            y[2 * j] = o[half * (RB / 16) + 4 * c + j][e];
+            y[2 * j + 1] = o[half * (RB / 16) + 4 * c + j][2 + e];
+          }
+          if (whole) {
+            if (d0 + 8 * c < p.c.head_dim) {
+              uint32_t w[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  w[j] = (uint32_t)float_to_elem<BF16>(finish(y[2 * j], sum, mm, m)) |
-                         ((uint32_t)float_to_elem<BF16>(finish(y[2 * j + 1], sum, mm, m)) << 16);
-                }
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.c.head_dim + d0 + 8 * c) =
-                    make_uint4(w[0], w[1], w[2], w[3]);
+              for (int j = 0; j < 4; ++j) {
+                w[j] = (uint32_t)float_to_elem<BF16>(finish(y[2 * j], sum, mm, m)) |
+                       ((uint32_t)float_to_elem<BF16>(finish(y[2 * j + 1], sum, mm, m)) << 16);
               }
-            } else {
-              *reinterpret_cast<float4*>(ws + 4 + d0 + 8 * c) = make_float4(y[0], y[1], y[2], y[3]);
-              *reinterpret_cast<float4*>(ws + 8 + d0 + 8 * c) = make_float4(y[4], y[5], y[6], y[7]);
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.c.head_dim + d0 + 8 * c) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
             }
+          } else {
+            *reinterpret_cast<float4*>(ws + 4 + d0 + 8 * c) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4*>(ws + 8 + d0 + 8 * c) = make_float4(y[4], y[5], y[6], y[7]);
           }
         }
       }
@@ -969,10 +937,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP, NT>::kPerSm) kv
 // 1 (few pairs) a block has 32 dims of one pair. Consecutive pairs are different items,
 // so one long item is spread over blocks.
 constexpr int kJoinWarp = 16;
-template <int DP, int NT, bool BF16, int PAIRS>
+template <int DP, bool BF16, int PAIRS>
 __global__ void __launch_bounds__(PAIRS == 1 ? 256 : 32 * PAIRS) kv_attn_join_kernel(const KvAttn p, int items) {
   constexpr int kJoinThreads = PAIRS == 1 ? 256 : 32 * PAIRS;
-  constexpr int LANES = PAIRS == 1 ? 8 : DP / 4;  // threads that share a partial's row (or 32 dims of it), four dims each
+  // threads that share a partial's row (or 32 dims of it), four dims each
+  constexpr int LANES = PAIRS == 1 ? 8 : DP / 4;
   constexpr int KG = kJoinThreads / LANES;        // partials read side by side
   constexpr int V4 = DP > 128 ? DP / 128 : 1;     // four-dim pieces of a row per lane, in the one-warp form
   constexpr int64_t kRow = DP + 4;
@@ -986,14 +955,14 @@ __global__ void __launch_bounds__(PAIRS == 1 ? 256 : 32 * PAIRS) kv_attn_join_ke
   auto look = [&](int pair, int& item, int& h, int4& me) -> int {
     h = pair / items;
     item = pair - h * items;
-    if (h >= p.slot_heads || ((item % kh_n) % p.head_blocks) * (8 * NT) + h >= p.group) return 0;
+    if (h >= p.slot_heads || ((item % kh_n) % p.head_blocks) * kHeads + h >= p.group) return 0;
     me = __ldg(p.meta + item);
     return me.x < 0 ? 0 : me.x;
   };
   auto store = [&](int item, int h, int d4, float4 acc, float sum, float mm, float m) {
     const int b = item / kh_n, kh = item - b * kh_n;
     const int head = kh / p.head_blocks;
-    const int64_t row = (int64_t)b * p.H + head * p.group + (kh - head * p.head_blocks) * (8 * NT) + h;
+    const int64_t row = (int64_t)b * p.H + head * p.group + (kh - head * p.head_blocks) * kHeads + h;
     if (4 * d4 < p.c.head_dim) {
       const uint32_t lo = (uint32_t)float_to_elem<BF16>(finish(acc.x, sum, mm, m)) |
                           ((uint32_t)float_to_elem<BF16>(finish(acc.y, sum, mm, m)) << 16);
@@ -1008,8 +977,11 @@ __global__ void __launch_bounds__(PAIRS == 1 ? 256 : 32 * PAIRS) kv_attn_join_ke
   int4 me;
   const int count = look(blockIdx.x * PAIRS + (PAIRS == 1 ? 0 : warp), item, h, me);
   if (PAIRS > 1 && count > 0 && count <= kJoinWarp) {
-    auto part = [&](int k) { return p.partial + (k == 0 ? (int64_t)me.y : 2 * ((int64_t)me.z + k)) * slot_row + h * kRow; };
-    const float4 x0 = lane < count ? *reinterpret_cast<const float4*>(part(lane)) : make_float4(kNoMax, kNoMax, 0.f, 0.f);
+    auto part = [&](int k) {
+      return p.partial + (k == 0 ? (int64_t)me.y : 2 * ((int64_t)me.z + k)) * slot_row + h * kRow;
+    };
+    float4 x0 = make_float4(kNoMax, kNoMax, 0.f, 0.f);
+    if (lane < count) x0 = *reinterpret_cast<const float4*>(part(lane));
     float4 x[kJoinWarp][V4];  // all in flight at once
 #pragma unroll
     for (int k = 0; k < kJoinWarp; ++k) {
@@ -1060,7 +1032,9 @@ __global__ void __launch_bounds__(PAIRS == 1 ? 256 : 32 * PAIRS) kv_attn_join_ke
     int4 me;
     const int count = look(blockIdx.x * PAIRS + i, item, h, me);
     if (count == 0 || (PAIRS > 1 && count <= kJoinWarp)) continue;
-    auto part = [&](int k) { return p.partial + (k == 0 ? (int64_t)me.y : 2 * ((int64_t)me.z + k)) * slot_row + h * kRow; };
+    auto part = [&](int k) {
+      return p.partial + (k == 0 ? (int64_t)me.y : 2 * ((int64_t)me.z + k)) * slot_row + h * kRow;
+    };
     // the maxima over all partials
     float m = kNoMax, mm = kNoMax;
     for (int k = tid; k < count; k += kJoinThreads) {
@@ -1142,24 +1116,26 @@ cudaError_t launch(F kern, dim3 grid, int threads, int smem, cudaStream_t stream
 }
 
 struct AttnPlan {
-  int dp, nt, head_blocks, ctas, slot_heads;
-  bool cut;  // an item can span workers: the join kernel and its workspace are needed
+  int dp, head_blocks, ctas, slot_heads;
+  int64_t units;  // of the longest item
+  bool cut;       // an item can span workers: the join kernel and its workspace are needed
 };
 
 AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t capacity) {
   AttnPlan a{};
   a.dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-  a.nt = group <= 8 || a.dp == 256 ? 1 : 2;
-  a.head_blocks = (group + 8 * a.nt - 1) / (8 * a.nt);
-  const int per_sm = a.dp == 64    ? (a.nt == 1 ? AttnShape<64, 1>::kPerSm : AttnShape<64, 2>::kPerSm)
-                     : a.dp == 128 ? (a.nt == 1 ? AttnShape<128, 1>::kPerSm : AttnShape<128, 2>::kPerSm)
-                                   : AttnShape<256, 1>::kPerSm;
+  // more than 8 query heads of a kv head are several items, which read the same
+  // codes at about the same time (16 columns in one item took 44 us where two
+  // items take 34: 16 x 4096, 4 kv heads of 96, 12 query heads each)
+  a.head_blocks = (group + kHeads - 1) / kHeads;
+  const int per_sm = a.dp == 64 ? AttnShape<64>::kPerSm : a.dp == 128 ? AttnShape<128>::kPerSm : AttnShape<256>::kPerSm;
   const int64_t units = capacity <= kWhole * kTile ? 1 : (capacity + kTile - 1) / kTile;
   const int64_t items = B * kv_heads * a.head_blocks;
   const int64_t most = (int64_t)num_sms() * per_sm;
   a.ctas = (int)(items > most / units ? most : items * units);
   a.cut = units > 1;
-  a.slot_heads = group < 8 * a.nt ? group : 8 * a.nt;
+  a.units = units;
+  a.slot_heads = group < kHeads ? group : kHeads;
   return a;
 }
 
@@ -1178,9 +1154,9 @@ bool encode_pool(CUtensorMap* map, const KvCache& c, uint8_t* base, const int64_
                               rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B) == CUDA_SUCCESS;
 }
 
-template <int DP, int NT, bool FP8, bool BF16>
+template <int DP, bool FP8, bool BF16>
 cudaError_t run_attn(KvAttn p, const AttnPlan& a, cudaStream_t stream) {
-  using S = AttnShape<DP, NT>;
+  using S = AttnShape<DP>;
   CUtensorMap kmap{}, vmap{};
   // whole 16-token tiles per page, and strides the tensor map can hold (else the copies of 16 bytes)
   const bool tma = p.c.page_size % 16 == 0 && encode_pool(&kmap, p.c, p.c.k, p.c.k_stride, &p.k_swap) &&
@@ -1192,20 +1168,21 @@ cudaError_t run_attn(KvAttn p, const AttnPlan& a, cudaStream_t stream) {
                : launch(kern, dim3(a.ctas), kAttnWarps * 32, S::kAlloc, stream, p.pdl, kmap, vmap, p);
   };
   const cudaError_t e =
-      tma ? go(kv_attn_kernel<DP, NT, FP8, BF16, true>) : go(kv_attn_kernel<DP, NT, FP8, BF16, false>);
+      tma ? go(kv_attn_kernel<DP, FP8, BF16, true>) : go(kv_attn_kernel<DP, FP8, BF16, false>);
   if (e != cudaSuccess || !a.cut) return e;
   const int items = p.B * p.c.kv_heads * p.head_blocks;
   const int64_t pairs = (int64_t)items * p.slot_heads;
-  // more than 16 partials an item on average: blocks for 32 dims of a pair
-  if ((int64_t)items * 16 < (int64_t)a.ctas * kAttnWarps) return launch(kv_attn_join_kernel<DP, NT, BF16, 1>, dim3(pairs, DP / 32), 256, 0,
-                                                                        stream, true, p, items);
-  return launch(kv_attn_join_kernel<DP, NT, BF16, 4>, dim3((pairs + 3) / 4), 128, 0, stream, true, p, items);
+  // more partials an item than a warp takes, on average: blocks for 32 dims of a pair
+  if ((int64_t)items * kJoinWarp < (int64_t)a.ctas * kAttnWarps && a.units > 2 * kJoinWarp) {
+    return launch(kv_attn_join_kernel<DP, BF16, 1>, dim3(pairs, DP / 32), 256, 0, stream, true, p, items);
+  }
+  return launch(kv_attn_join_kernel<DP, BF16, 4>, dim3((pairs + 3) / 4), 128, 0, stream, true, p, items);
 }
 
-template <int DP, int NT>
+template <int DP>
 cudaError_t run_attn_t(const KvAttn& p, const AttnPlan& a, bool fp8, bool bf16, cudaStream_t stream) {
-  if (fp8) return bf16 ? run_attn<DP, NT, true, true>(p, a, stream) : run_attn<DP, NT, true, false>(p, a, stream);
-  return bf16 ? run_attn<DP, NT, false, true>(p, a, stream) : run_attn<DP, NT, false, false>(p, a, stream);
+  if (fp8) return bf16 ? run_attn<DP, true, true>(p, a, stream) : run_attn<DP, true, false>(p, a, stream);
+  return bf16 ? run_attn<DP, false, true>(p, a, stream) : run_attn<DP, false, false>(p, a, stream);
 }
 
 int grid_rows(int64_t rows, int lpr) {
@@ -1275,11 +1252,9 @@ cudaError_t launch_kv_attn(const KvAttnArgs& args, bool fp8, bool bf16, void* ws
   p.meta = a.cut ? reinterpret_cast<int4*>(static_cast<uint8_t*>(ws) + attn_slot_bytes(a)) : nullptr;
   p.status = device_status_ptr();
   p.pdl = pdl_enabled();
-  if (a.dp == 64) return a.nt == 1 ? run_attn_t<64, 1>(p, a, fp8, bf16, stream) : run_attn_t<64, 2>(p, a, fp8, bf16, stream);
-  if (a.dp == 128) {
-    return a.nt == 1 ? run_attn_t<128, 1>(p, a, fp8, bf16, stream) : run_attn_t<128, 2>(p, a, fp8, bf16, stream);
-  }
-  return run_attn_t<256, 1>(p, a, fp8, bf16, stream);
+  return a.dp == 64    ? run_attn_t<64>(p, a, fp8, bf16, stream)
+         : a.dp == 128 ? run_attn_t<128>(p, a, fp8, bf16, stream)
+                       : run_attn_t<256>(p, a, fp8, bf16, stream);
 }
 
 }  // namespace nsq
