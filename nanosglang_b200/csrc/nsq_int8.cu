@@ -313,13 +313,14 @@ static cudaError_t quantize_rows(const uint16_t* x, int M, int K, int8_t* codes,
   return per <= 1   ? go(int8_quantize_kernel<TPR, 1, BF16>)
          : per <= 2 ? go(int8_quantize_kernel<TPR, 2, BF16>)
          : per <= 4 ? go(int8_quantize_kernel<TPR, 4, BF16>)
-                    : go(int8_quantize_kernel<TPR, 8, BF16>);
+         : per <= 8 ? go(int8_quantize_kernel<TPR, 8, BF16>)
+                    : go(int8_quantize_kernel<TPR, 16, BF16>);
 }
 
 cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K, int8_t* codes, float* scale,
                                  cudaStream_t stream) {
   const bool pdl = pdl_enabled();
-  const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 8 * 8 * kQThreads &&
+  const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 16 * 8 * kQThreads &&
                    ((reinterpret_cast<uintptr_t>(x) & 15) | (reinterpret_cast<uintptr_t>(codes) & 7)) == 0;
   if (!vec) {
     return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 0, 1, stream, pdl, x, dtype, K, codes, scale,

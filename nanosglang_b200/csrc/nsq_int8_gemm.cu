@@ -8,8 +8,11 @@
 // 512 cycles of int8 tensor work, so the L2 path and the tensor pipe are near
 // balance; hence the largest tile whose accumulator still double-buffers in
 // tensor memory (2 x 256 columns), and a tile order in which the tiles that
-// run at the same time share their weight rows and tokens (8 token tiles by as
-// many weight tiles as it takes).
+// run at the same time share their weight rows and tokens (32 token tiles by as
+// many weight tiles as it takes). Measured: 8192 x 4096 x 14336 in 306 us, 3.1
+// P/s (less under the sustained power limit); with the token scales loaded
+// after the epilogue's wait instead of before 410 us, with stages of one
+// k-block 600 us, with groups of 8 token tiles 3% more.
 //
 // Warp roles (per CTA, 352 threads): 0 TMA of the weight, 1 MMA issuer (of a
 // pair, the even CTA's), 2 TMA of x (one lane issues a copy in about 100 cycles,
@@ -18,6 +21,10 @@
 // weight's bandwidth that counts: the rows are then dealt evenly over the SMs,
 // fewer than 128 to a tile (the MMA's other rows compute on leftovers of the
 // stage that nothing reads), and the ring keeps 150 KB or more per SM in flight.
+// Where tiles are few and K is long, a cluster of up to 4 CTAs shares a tile
+// along K (SPLIT): each copies its sums of every other one's slice of tokens
+// there in bulk, adds up its own slice and finishes it (integers: exact in any
+// order).
 // The epilogue of one tile runs under the MMAs of
 // the next: s32 -> fp32, scales, bias, one rounding, a staged [token][feature]
 // tile, TMA store (plain stores where N % 8 != 0 leaves no 16-byte row pitch).
@@ -50,8 +57,8 @@ struct GemmShape {
   static constexpr int NS = (226 * 1024 - 2 * kYHalf - 1024) / kStage < 6 ? (226 * 1024 - 2 * kYHalf - 1024) / kStage : 6;
   static constexpr int kY = NS * kStage;
   static constexpr int kBar = kY + 2 * kYHalf;
-  // full[NS], done[NS], full_acc[2], empty_acc[2], drain
-  static constexpr int kBars = 2 * NS + 5;
+  // full[NS], done[NS], full_acc[2], empty_acc[2], drain, sums
+  static constexpr int kBars = 2 * NS + 6;
   static constexpr int kTmemSlot = kBar + kBars * 8;
   static constexpr int kAbort = kTmemSlot + 4;
   static constexpr int kAlloc = kAbort + 4 + 1024;
@@ -69,6 +76,7 @@ struct GemmParams {
   int M, K, N, bias_dtype;
   int num_w, num_t, num_kb, num_st;
   int wrows;  // weight rows of a CTA's tile
+  int split;  // SPLIT: CTAs of a cluster that share a tile, along K
   int pdl_x;  // x and its scales come from the kernel ahead on the stream
 };
 
@@ -142,7 +150,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return (uint32_t)float_to_elem<BF16>(a) | ((uint32_t)float_to_elem<BF16>(b) << 16);
 }
 
-template <int CG, int TOK, bool BF16, bool STAGED>
+template <int CG, int TOK, bool BF16, bool STAGED, bool SPLIT>
 __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap xmap,
                                                                     const __grid_constant__ CUtensorMap wmap,
                                                                     const __grid_constant__ CUtensorMap ymap,
@@ -155,13 +163,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
   uint64_t* full_acc = done + S::NS;                             // an accumulator is complete (both CTAs)
   uint64_t* empty_acc = full_acc + 2;                            // and read out by every epilogue warp (even CTA)
   uint64_t* drain = empty_acc + 2;
+  uint64_t* sums = drain + 1;  // SPLIT: the other CTAs' sums of this one's slice have landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kTmemSlot);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kAbort);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
   const bool leader = rank == 0;
-  const int cid = blockIdx.x / CG, ncl = gridDim.x / CG;
+  // SPLIT: one tile per cluster, and the stages [st0, st1) of it
+  const int share = SPLIT ? p.split : CG;
+  const int cid = blockIdx.x / share, ncl = gridDim.x / share;
+  const int krank = SPLIT ? (int)cluster_ctarank() : 0;
+  const int st0 = SPLIT ? p.num_st * krank / p.split : 0, st1 = SPLIT ? p.num_st * (krank + 1) / p.split : p.num_st;
+  // the sums of a token: kRows of them, a 16-byte multiple that keeps rows off one another's banks
+  constexpr uint32_t kSumBytes = (kRows + 4) * 4;
+  const int slice = SPLIT ? TOK / p.split : 0;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -174,7 +190,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
       mbar_init(&empty_acc[i], CG * kEpi);
     }
     mbar_init(drain, 1);
+    mbar_init(sums, 1);
     fence_barrier_init();
+    if (SPLIT) mbar_arrive_expect_tx(sums, (uint32_t)((p.split - 1) * slice) * kSumBytes);
   }
   if (warp == 1) {
     if constexpr (CG == 2) {
@@ -186,7 +204,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
     }
   }
   tc_fence_before();
-  if constexpr (CG == 2) {
+  if constexpr (CG == 2 || SPLIT) {
     cluster_sync_all();
   } else {
     __syncthreads();
@@ -221,7 +239,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
         int wt, tt;
         gemm_unit(p, u, wt, tt);
         const int row = is_x ? tt * TOK + (int)rank * (gemm_n<TOK>(p.M, tt) / CG) : (wt * CG + (int)rank) * p.wrows;
-        for (int st = 0; st < p.num_st; ++st, ++it) {
+        for (int st = st0; st < st1; ++st, ++it) {
           if (!(ok = mbar_wait(&done[s], phase, p.status, is_x ? 214 : 210, abort_flag))) break;
           const int kb0 = st * kKps;
           const int nk = p.num_kb - kb0 < kKps ? p.num_kb - kb0 : kKps;
@@ -267,14 +285,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
         ok = __all_sync(0xffffffffu, mbar_wait(&empty_acc[buf], ((tc >> 1) & 1) ^ 1, p.status, 211, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        for (int st = 0; st < p.num_st; ++st, ++it) {
+        for (int st = st0; st < st1; ++st, ++it) {
           if (!ready) {
             ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, p.status, 212, abort_flag));
             if (!ok) break;
           }
           tc_fence_after();
           const uint32_t base = base0 + s * S::kStage;
-          umma_i8_elect<CG>(d, sw128_kmajor_desc(base), sw128_kmajor_desc(base + kKps * S::kWBytes), idesc, st > 0);
+          umma_i8_elect<CG>(d, sw128_kmajor_desc(base), sw128_kmajor_desc(base + kKps * S::kWBytes), idesc, st > st0);
           const int s1 = s + 1 == S::NS ? 0 : s + 1;
           const uint32_t phase1 = s1 == 0 ? phase ^ 1 : phase;
           ready = __all_sync(0xffffffffu, mbar_test(&full[s1], phase1));
@@ -293,7 +311,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
       commit(drain);
       mbar_wait(drain, 0, nullptr, 0, nullptr);
     }
-  } else {
+  } else if constexpr (!SPLIT) {
     // ---------------- epilogue ----------------
     if (p.pdl_x) pdl_wait_prior_grids();  // the scales of x, and y's buffer
     const int sub = warp & 3;             // tensor-memory sub-partition: 32 weight rows
@@ -319,6 +337,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
         wsc[q] = n < f1 ? __ldg(p.wscale + n) : 0.f;
         bf[q] = has_bias && n < f1 ? load_bias(p.bias, p.bias_dtype, n) : 0.f;
       }
+      // the scales of this lane's tokens, too, come before the wait for the accumulator
+      constexpr int kWarpTok = S::kWarpTok, kRounds = TOK / S::kTokRound, kChunks = kWarpTok / 32;
+      float xs[kRounds][kChunks][8];
+#pragma unroll
+      for (int rd = 0; rd < kRounds; ++rd) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int m = tt * TOK + rd * S::kTokRound + half * kWarpTok + c * 32 + 8 * (j >> 1) + 2 * t + (j & 1);
+            xs[rd][c][j] = m < p.M ? p.xscale[m] : 0.f;
+          }
+        }
+      }
       ok = mbar_wait(&full_acc[buf], (tc >> 1) & 1, p.status, 213, abort_flag);
       if (!named_bar_all(1, kEpi * 32, ok)) {
         ok = false;
@@ -326,25 +358,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
       }
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(sub * 32) << 16) + buf * TOK;
-      constexpr int kWarpTok = S::kWarpTok;
-#pragma unroll 1
-      for (int rd = 0; rd < TOK / S::kTokRound; ++rd) {
+#pragma unroll
+      for (int rd = 0; rd < kRounds; ++rd) {
         if constexpr (STAGED) {
           if (etid == 0) bulk_wait_group_read<0>();  // the staged tile's last store has read it
           named_bar_sync(1, kEpi * 32);
         }
         const int col0 = rd * S::kTokRound + half * kWarpTok;
-#pragma unroll 1
-        for (int c = 0; c < kWarpTok && half * kWarpTok < S::kTokRound && tt * TOK + col0 + c < p.M; c += 32) {
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+          const int c = ch * 32;
+          if (half * kWarpTok >= S::kTokRound || tt * TOK + col0 + c >= p.M) break;
           uint32_t r0[16], r1[16];
           tmem_ld_16x256b_x4(acc + col0 + c, r0);
           tmem_ld_16x256b_x4(acc + (16u << 16) + col0 + c, r1);
-          float xs[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int m = tt * TOK + col0 + c + 8 * (j >> 1) + 2 * t + (j & 1);
-            xs[j] = m < p.M ? p.xscale[m] : 0.f;
-          }
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -358,7 +385,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
               v[3][e] = (float)(int)r1[4 * j + 2 + e];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                v[q][e] = v[q][e] * xs[2 * j + e] * wsc[q];
+                v[q][e] = v[q][e] * xs[rd][ch][2 * j + e] * wsc[q];
                 if (has_bias) v[q][e] += bf[q];
               }
             }
@@ -408,9 +435,65 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
     if (STAGED && etid == 0) bulk_wait_group<0>();
   }
 
+  if constexpr (SPLIT) {
+    // Every CTA's MMAs are done, so every ring is idle: here it takes this CTA's
+    // sums [TOK][kRows + 4], and behind them the others' of its slice [CTA][slice][kRows + 4].
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    int* const mine = reinterpret_cast<int*>(smem);
+    int* const theirs = mine + TOK * (kSumBytes / 4);
+    static_assert(2 * TOK * kSumBytes <= (uint32_t)S::NS * S::kStage, "both in the ring");
+    if (warp >= 3) {
+      const int sub = warp & 3, g = lane >> 2, t = lane & 3;
+      for (int c = ((warp - 3) >> 2) * 32; c < TOK; c += 64) {
+        uint32_t r0[16], r1[16];
+        const uint32_t acc = tmem + ((uint32_t)(sub * 32) << 16) + c;
+        tmem_ld_16x256b_x4(acc, r0);
+        tmem_ld_16x256b_x4(acc + (16u << 16), r1);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // token c + 8 (j / 2) + 2 t + j % 2, rows g, g + 8, g + 16, g + 24
+          int* at = mine + (c + 8 * (j >> 1) + 2 * t + (j & 1)) * (kSumBytes / 4) + sub * 32 + g;
+          const int e = 4 * (j >> 1) + (j & 1);
+          at[0] = (int)r0[e];
+          at[8] = (int)r0[e + 2];
+          at[16] = (int)r1[e];
+          at[24] = (int)r1[e + 2];
+        }
+      }
+      fence_proxy_async_smem();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < p.split; ++i) {
+        const int to = (krank + i) % p.split;  // its slot for this CTA: the others in order
+        const int at = krank < to ? krank : krank - 1;
+        bulk_copy_s2cluster(dsmem_map(smem_u32(theirs) + at * slice * kSumBytes, to),
+                            smem_u32(mine) + to * slice * kSumBytes, slice * kSumBytes, dsmem_map(smem_u32(sums), to));
+      }
+    }
+    mbar_wait(sums, 0, p.status, 215, nullptr);
+    if (p.pdl_x) pdl_wait_prior_grids();
+    int wt, tt;
+    gemm_unit(p, cid, wt, tt);
+    const int f0 = wt * p.wrows, f1 = f0 + p.wrows < p.N ? f0 + p.wrows : p.N;
+    const bool has_bias = p.bias_dtype != NSQ_DTYPE_NONE;
+    for (int i = threadIdx.x; i < slice * kRows; i += kGemmThreads) {
+      const int row = i % kRows, tok = i / kRows, n = f0 + row, m = tt * TOK + krank * slice + tok;
+      if (n >= f1 || m >= p.M) continue;
+      int sum = mine[(krank * slice + tok) * (kSumBytes / 4) + row];
+      for (int r = 0; r < p.split - 1; ++r) sum += theirs[(r * slice + tok) * (kSumBytes / 4) + row];
+      float v = (float)sum * p.xscale[m] * __ldg(p.wscale + n);
+      if (has_bias) v += load_bias(p.bias, p.bias_dtype, n);
+      static_cast<uint16_t*>(p.y)[(int64_t)m * p.N + n] = float_to_elem<BF16>(v);
+    }
+  }
+
   __syncthreads();
   tc_fence_before();
-  if constexpr (CG == 2) cluster_sync_all();
+  if constexpr (CG == 2 || SPLIT) cluster_sync_all();  // SPLIT: every copy out of this CTA has landed
   if (warp == 1) {
     tc_fence_after();
     if constexpr (CG == 2) {
@@ -421,24 +504,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
   }
 }
 
-template <int CG, int TOK, bool BF16, bool STAGED>
+template <int CG, int TOK, bool BF16, bool STAGED, bool SPLIT = false>
 cudaError_t launch_gemm(const Int8Args& a, const CUtensorMap& xmap, const CUtensorMap& wmap, const CUtensorMap& ymap,
                         const GemmParams& p, cudaStream_t stream) {
   using S = GemmShape<CG, TOK>;
-  auto kern = int8_gemm_kernel<CG, TOK, BF16, STAGED>;
+  auto kern = int8_gemm_kernel<CG, TOK, BF16, STAGED, SPLIT>;
   cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kern), S::kAlloc);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)p.num_w * p.num_t, most = num_sms() / CG;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(CG * (units < most ? units : most)));
+  cfg.gridDim = dim3((unsigned)(SPLIT ? units * p.split : CG * (units < most ? units : most)));
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = S::kAlloc;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   int n = 0;
-  if (CG == 2) {
+  if (CG == 2 || SPLIT) {
     at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = 2;
+    at[n].val.clusterDim.x = SPLIT ? p.split : 2;
     at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
     ++n;
   }
@@ -453,9 +536,9 @@ cudaError_t launch_gemm(const Int8Args& a, const CUtensorMap& xmap, const CUtens
 }
 
 template <int CG, int TOK>
-int run_gemm(const Int8Args& a, int wrows, cudaStream_t stream) {
+int run_gemm(const Int8Args& a, int wrows, int split, cudaStream_t stream) {
   using S = GemmShape<CG, TOK>;
-  const bool staged = a.N % 8 == 0 && wrows % 64 == 0;
+  const bool staged = split == 1 && a.N % 8 == 0 && wrows % 64 == 0;
   CUtensorMap xmap, wmap, ymap;
   if (encode_tensor_map_2d(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<int8_t*>(a.x), a.K, a.M, a.K, kBK,
                            S::kXRows, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS ||
@@ -481,14 +564,20 @@ int run_gemm(const Int8Args& a, int wrows, cudaStream_t stream) {
   p.K = a.K;
   p.N = a.N;
   p.wrows = wrows;
+  p.split = split;
   p.num_w = (a.N + CG * wrows - 1) / (CG * wrows);
   p.num_t = (a.M + TOK - 1) / TOK;
   p.num_kb = (a.K + kBK - 1) / kBK;
   p.num_st = (p.num_kb + kKps - 1) / kKps;
   p.pdl_x = a.after_quantize || pdl_enabled();
   if ((int64_t)p.num_w * p.num_t > 0x3FFFFFFF) return NSQ_ENOTSUP;
-  cudaError_t e;
-  if (staged) {
+  cudaError_t e = cudaSuccess;
+  if (split > 1) {
+    if constexpr (CG == 1) {
+      e = a.y_bf16 ? launch_gemm<1, TOK, true, false, true>(a, xmap, wmap, ymap, p, stream)
+                   : launch_gemm<1, TOK, false, false, true>(a, xmap, wmap, ymap, p, stream);
+    }
+  } else if (staged) {
     e = a.y_bf16 ? launch_gemm<CG, TOK, true, true>(a, xmap, wmap, ymap, p, stream)
                  : launch_gemm<CG, TOK, false, true>(a, xmap, wmap, ymap, p, stream);
   } else {
@@ -500,27 +589,50 @@ int run_gemm(const Int8Args& a, int wrows, cudaStream_t stream) {
 
 }  // namespace
 
-// One token tile: rows dealt evenly over the SMs. Otherwise waves of tiles
-// times a tile's time in cycles, per k-block and fixed (fill, the last tile's
-// epilogue).
+// The cheapest tile by an estimate in ns (measured on B200): for every wave of
+// tiles the longer of a CTA's k-blocks (32, 64 or 128 tokens: 170, 205, 265
+// each; CTA pairs of 256 x 256: 385) and its epilogue (900, 1300, 2150; 4000),
+// once more the epilogue, and 6 us for a K split (cluster launch, exchange, no
+// steady state of the ring: worth it for long K alone, 100 x 20000 -> 640 44 ->
+// 13 us). Clusters of 4 at most, and 128 CTAs in them: more are not sure to run
+// at once on 8 groups of 16 to 18 SMs. Rows of a tile: all that an even deal
+// leaves.
 int run_int8_gemm(const Int8Args& a, cudaStream_t stream) {
-  const int64_t sms = num_sms(), kb = (a.K + kBK - 1) / kBK;
-  if (a.M <= 128) {
-    const int64_t waves = (a.N + sms * kRows - 1) / (sms * kRows);
-    const int64_t each = (a.N + sms * waves - 1) / (sms * waves);
-    const int wrows = (int)((each + 7) / 8 * 8);
-    if (a.M <= 32) return run_gemm<1, 32>(a, wrows, stream);
-    if (a.M <= 64) return run_gemm<1, 64>(a, wrows, stream);
-    return run_gemm<1, 128>(a, wrows, stream);
-  }
-  auto cost = [&](int cg, int tok, int per_kb, int fixed) {
-    const int64_t tiles = (int64_t)((a.N + cg * kRows - 1) / (cg * kRows)) * ((a.M + tok - 1) / tok);
-    const int64_t at_once = sms / cg;
-    return (tiles + at_once - 1) / at_once * (kb * per_kb) + fixed;
+  const int64_t sms = num_sms(), kb = (a.K + kBK - 1) / kBK, num_st = (kb + kKps - 1) / kKps;
+  auto estimate = [](int64_t waves, int64_t blocks, int64_t ns, int64_t epilogue) {
+    return waves * (blocks * ns > epilogue ? blocks * ns : epilogue) + epilogue;
   };
-  const int64_t c2 = cost(2, 256, 640, 6000), c1 = cost(1, 128, 320, 4000), ch = cost(1, 64, 200, 3000);
-  if (c2 <= c1 && c2 <= ch) return run_gemm<2, 256>(a, kRows, stream);
-  return c1 <= ch ? run_gemm<1, 128>(a, kRows, stream) : run_gemm<1, 64>(a, kRows, stream);
+  int64_t best = INT64_MAX;
+  int tok_b = 0, rows_b = kRows, split_b = 1;
+  for (int tok = 32; tok <= 128; tok *= 2) {
+    const int64_t num_t = (a.M + tok - 1) / tok;
+    const int64_t ns = tok == 32 ? 170 : tok == 64 ? 205 : 265, epilogue = tok == 32 ? 900 : tok == 64 ? 1300 : 2150;
+    for (int split = 1; split <= 4 && split <= num_st; split *= 2) {
+      // weight tiles that run at once
+      const int64_t room = (split > 1 && sms > 128 ? 128 : sms) / (num_t * split);
+      int64_t rows = kRows;
+      if (room > 0) {
+        const int64_t waves = (a.N + room * kRows - 1) / (room * kRows);
+        rows = ((a.N + room * waves - 1) / (room * waves) + 7) / 8 * 8;
+        if (rows < 32) rows = 32;
+      }
+      const int64_t tiles = num_t * ((a.N + rows - 1) / rows);
+      if (split > 1 && (tiles * split > 128 || tiles * split > sms)) continue;
+      const int64_t cost = estimate((tiles * split + sms - 1) / sms, (kb + split - 1) / split, ns, epilogue) +
+                           (split > 1 ? 6000 : 0);
+      if (cost < best) {
+        best = cost;
+        tok_b = tok;
+        rows_b = (int)rows;
+        split_b = split;
+      }
+    }
+  }
+  const int64_t pairs = (int64_t)((a.N + 255) / 256) * ((a.M + 255) / 256);
+  if (estimate((pairs + sms / 2 - 1) / (sms / 2), kb, 385, 4000) < best) return run_gemm<2, 256>(a, kRows, 1, stream);
+  return tok_b == 32   ? run_gemm<1, 32>(a, rows_b, split_b, stream)
+         : tok_b == 64 ? run_gemm<1, 64>(a, rows_b, split_b, stream)
+                       : run_gemm<1, 128>(a, rows_b, split_b, stream);
 }
 
 }  // namespace nsq
