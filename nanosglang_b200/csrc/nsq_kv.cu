@@ -87,10 +87,12 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
-// Sixteen elements of a row per lane, LPR lanes per row (LPR * 16 >= head_dim),
-// k and v of one place together and two places at a time: the place is worked
-// out once for 64 elements, and their loads are in flight together. DRAM bounds
-// both kernels.
+// Two times eight elements of a row per lane, LPR lanes per row (LPR * 16 >=
+// head_dim; LPR * 8 elements apart, so that the lanes of a row read and write
+// whole sectors), k and v of one place together and several places at a time:
+// the place is worked out once for 32 elements a lane, and the loads are in
+// flight together. DRAM bounds both kernels, next the instructions (writing:
+// 70% of the issue slots at 5 TB/s).
 constexpr int kAtOnce = 2;
 
 struct KvPlace {
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const KvWrite p) {
   if (p.pdl) pdl_wait_prior_grids();
   const int sub = threadIdx.x % LPR;
   const uint32_t rows = (uint32_t)p.T * (uint32_t)p.c.kv_heads;
-  const bool in_row = sub * 16 < p.c.head_dim;
+  const bool in_row[2] = {sub * 8 < p.c.head_dim, (LPR + sub) * 8 < p.c.head_dim};
   const uint32_t step = gridDim.x * (256 / LPR);
   // whole warps stay in the loop: the shuffles below are all lanes'
   for (uint32_t r0 = (blockIdx.x * 256 + (threadIdx.x & ~31u)) / LPR; r0 < rows; r0 += kAtOnce * step) {
@@ -132,10 +134,9 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const KvWrite p) {
       for (int j = 0; j < 2; ++j) {
         const int64_t at = j ? a[i].tok * p.v_stride[0] + a[i].head * p.v_stride[1]
                              : a[i].tok * p.k_stride[0] + a[i].head * p.k_stride[1];
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(j ? p.v : p.k) + at + sub * 16);
-        const bool in = in_row && r < rows;
-        x[i][j][0] = in ? __ldg(src) : make_uint4(0, 0, 0, 0);
-        x[i][j][1] = in ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(j ? p.v : p.k) + at) + sub;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) x[i][j][c] = in_row[c] && r < rows ? __ldg(src + c * LPR) : make_uint4(0, 0, 0, 0);
       }
     }
 #pragma unroll
@@ -148,10 +149,10 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const KvWrite p) {
         if (!a[i].in) continue;
         const float s = row_scale<FP8>(abs_max_value<BF16>(m));
         const RowDiv dv(s);
-        if (in_row) {
-          const uint2 lo = row_codes8<FP8, BF16>(dv, x[i][j][0]), hi = row_codes8<FP8, BF16>(dv, x[i][j][1]);
-          uint8_t* dst = j ? p.c.v + kv_at(a[i], p.c.v_stride) : p.c.k + kv_at(a[i], p.c.k_stride);
-          *reinterpret_cast<uint4*>(dst + sub * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        uint8_t* dst = j ? p.c.v + kv_at(a[i], p.c.v_stride) : p.c.k + kv_at(a[i], p.c.k_stride);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (in_row[c]) reinterpret_cast<uint2*>(dst)[c * LPR + sub] = row_codes8<FP8, BF16>(dv, x[i][j][c]);
         }
         if (sub == 0) *(j ? p.c.vs + kv_at(a[i], p.c.vs_stride) : p.c.ks + kv_at(a[i], p.c.ks_stride)) = s;
       }
@@ -184,12 +185,13 @@ template <bool FP8, bool BF16, int LPR>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
   if (p.pdl) pdl_wait_prior_grids();
   const int sub = threadIdx.x % LPR;
-  if (sub * 16 >= p.c.head_dim) return;
+  const bool in_row[2] = {sub * 8 < p.c.head_dim, (LPR + sub) * 8 < p.c.head_dim};
+  if (!in_row[0]) return;
   const uint32_t rows = (uint32_t)p.T * (uint32_t)p.c.kv_heads;
   const uint32_t step = gridDim.x * (256 / LPR);
   for (uint32_t r0 = (blockIdx.x * 256 + threadIdx.x) / LPR; r0 < rows; r0 += kAtOnce * step) {
     KvPlace a[kAtOnce];
-    uint4 c[kAtOnce][2];
+    uint2 c[kAtOnce][2][2];  // [place][k, v][8 codes]
     float s[kAtOnce][2];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) a[i] = kv_place(p, r0 + i * step, rows, 201, sub == 0);
@@ -197,11 +199,12 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
     for (int i = 0; i < kAtOnce; ++i) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        c[i][j] = make_uint4(0, 0, 0, 0);
+        c[i][j][0] = c[i][j][1] = make_uint2(0, 0);
         s[i][j] = 0.f;
         if (a[i].in) {
           const uint8_t* src = j ? p.c.v + kv_at(a[i], p.c.v_stride) : p.c.k + kv_at(a[i], p.c.k_stride);
-          c[i][j] = *reinterpret_cast<const uint4*>(src + sub * 16);
+          c[i][j][0] = reinterpret_cast<const uint2*>(src)[sub];
+          if (in_row[1]) c[i][j][1] = reinterpret_cast<const uint2*>(src)[LPR + sub];
           s[i][j] = *(j ? p.c.vs + kv_at(a[i], p.c.vs_stride) : p.c.ks + kv_at(a[i], p.c.ks_stride));
         }
       }
@@ -212,12 +215,13 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
       if (r >= rows) break;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint16_t* out = static_cast<uint16_t*>(j ? p.v : p.k) + (int64_t)r * p.c.head_dim + sub * 16;
-        uint4* dst = reinterpret_cast<uint4*>(out);
-        const uint2 v0 = values4<FP8, BF16>(c[i][j].x, s[i][j]), v1 = values4<FP8, BF16>(c[i][j].y, s[i][j]);
-        const uint2 v2 = values4<FP8, BF16>(c[i][j].z, s[i][j]), v3 = values4<FP8, BF16>(c[i][j].w, s[i][j]);
-        dst[0] = make_uint4(v0.x, v0.y, v1.x, v1.y);
-        dst[1] = make_uint4(v2.x, v2.y, v3.x, v3.y);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(j ? p.v : p.k) + (int64_t)r * p.c.head_dim);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!in_row[h]) continue;
+          const uint2 lo = values4<FP8, BF16>(c[i][j][h].x, s[i][j]), hi = values4<FP8, BF16>(c[i][j][h].y, s[i][j]);
+          dst[h * LPR + sub] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
       }
     }
   }
