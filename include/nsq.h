@@ -213,7 +213,7 @@ int nsq_fp8_quantize_noalloc(const void* w, int w_dtype, int64_t N, int64_t K, u
  * nsq_int8_linear: y = (codes(x) . weight_int8^T) * scale(x) * weight_scale
  * + bias, summed in int32 (exact), scaled in fp32 and rounded once; x_dtype is
  * F16 or BF16, y has the same. It launches the row quantiser into the
- * workspace (nsq_int8_linear_workspace_size(M, K) bytes, 16-byte aligned,
+ * workspace (nsq_int8_linear_workspace_size(M, K, N) bytes, 16-byte aligned,
  * stream-ordered like y), then the product; up to 8 tokens with few elements
  * are one launch and need no workspace (size 0, may be NULL). A token with a NaN or an infinity
  * gives a row of NaN.
@@ -225,7 +225,7 @@ int nsq_fp8_quantize_noalloc(const void* w, int w_dtype, int64_t N, int64_t K, u
  * 16-byte aligned.
  */
 int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* codes, float* scale, void* stream);
-size_t nsq_int8_linear_workspace_size(int64_t M, int64_t K);
+size_t nsq_int8_linear_workspace_size(int64_t M, int64_t K, int64_t N);
 int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N, const int8_t* weight_int8,
                     const float* weight_scale, const void* bias, int bias_dtype, void* y, void* workspace,
                     size_t workspace_bytes, void* stream);

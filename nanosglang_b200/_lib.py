@@ -74,7 +74,7 @@ SIGNATURES = {
                                  c_void_p]),
     "nsq_fp8_quantize_noalloc": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "nsq_int8_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
-    "nsq_int8_linear_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "nsq_int8_linear_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "nsq_int8_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int,
                                 c_void_p, c_void_p, c_size_t, c_void_p]),
     "nsq_int8_linear_quantized": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,

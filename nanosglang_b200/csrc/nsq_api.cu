@@ -631,16 +631,19 @@ int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* 
 constexpr int64_t kInt8MaxK = 131072;  // 128 * 127 * 131072 < 2^31
 
 // Few enough elements of x that every CTA of the rows kernel quantises them
-// all sooner than a kernel of its own would (full call, us, one launch vs two:
-// 1 x 896 -> 4864 3.7 vs 3.9, 1 x 4096 -> 4096 7.0 vs 7.6; but 8 x 896 -> 4864
-// 5.2 vs 4.0, 1 x 8192 -> 8192 20.4 vs 16.0).
-static bool int8_fused(int64_t M, int64_t K) { return M <= 8 && M * K <= 4096; }
+// all, once for every 16 weight rows, sooner than a kernel of its own would
+// (full call, us, one launch vs two: 1 x 896 -> 4864 3.7 vs 3.9, 1 x 4096 ->
+// 4096 7.0 vs 7.6; but 8 x 896 -> 4864 5.2 vs 4.0, 1 x 4096 -> 14336 17.6 vs
+// 15.0, 1 x 8192 -> 8192 20.4 vs 16.0).
+static bool int8_fused(int64_t M, int64_t K, int64_t N) {
+  return M <= 8 && M * K <= 4096 && M * K * ((N + 15) / 16) <= ((int64_t)1 << 20);
+}
 
 // Workspace: the codes, then (16-byte aligned) the scales.
 static size_t int8_codes_bytes(int64_t M, int64_t K) { return ((size_t)M * (size_t)K + 15) & ~(size_t)15; }
 
-size_t nsq_int8_linear_workspace_size(int64_t M, int64_t K) {
-  if (M <= 0 || K <= 0 || M > kIntMax || K > kInt8MaxK || int8_fused(M, K)) return 0;
+size_t nsq_int8_linear_workspace_size(int64_t M, int64_t K, int64_t N) {
+  if (M <= 0 || K <= 0 || N <= 0 || M > kIntMax || K > kInt8MaxK || N > kIntMax || int8_fused(M, K, N)) return 0;
   return int8_codes_bytes(M, K) + (size_t)M * sizeof(float);
 }
 
@@ -679,12 +682,12 @@ int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N,
                     size_t workspace_bytes, void* stream) {
   int rc = int8_check(M, K, N, x, weight_int8, weight_scale, bias, bias_dtype, y, x_dtype);
   if (rc != NSQ_OK || M == 0) return rc;
-  if (int8_fused(M, K)) {
+  if (int8_fused(M, K, N)) {
     return run_int8_rows(Int8Args{nullptr, nullptr, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
                                   x_dtype == NSQ_DTYPE_BF16, y, false, x},
                          static_cast<cudaStream_t>(stream));
   }
-  if (!workspace || workspace_bytes < nsq_int8_linear_workspace_size(M, K)) return NSQ_EWORKSPACE;
+  if (!workspace || workspace_bytes < nsq_int8_linear_workspace_size(M, K, N)) return NSQ_EWORKSPACE;
   if (!aligned16(workspace)) return NSQ_EALIGN;
   int8_t* codes = static_cast<int8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(codes + int8_codes_bytes(M, K));
@@ -788,7 +791,7 @@ static int kv_attn_check(int64_t B, int64_t H, int64_t kv_heads, int64_t head_di
   if (B < 0 || H <= 0 || kv_heads <= 0 || head_dim <= 0 || page_size <= 0 || table_width < 0) return NSQ_EINVAL;
   if (H % kv_heads != 0) return NSQ_EINVAL;
   if (head_dim % 16 != 0 || head_dim > 256) return NSQ_ENOTSUP;
-  if (H > (1 << 20) || B > ((int64_t)1 << 30) / H) return NSQ_ENOTSUP;
+  if (H > (1 << 20) || B > ((int64_t)1 << 28) / H) return NSQ_ENOTSUP;  // 32-bit counts of items and heads
   if (table_width > ((int64_t)1 << 30) / page_size) return NSQ_ENOTSUP;
   return NSQ_OK;
 }

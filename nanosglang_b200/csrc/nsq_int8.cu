@@ -190,7 +190,6 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
   const int ldx = (p.K + 127) / 128 * 128 + 64;
   __shared__ uint32_t xmax_s[kRWarps];
   __shared__ float xscale_s[8];
-  bool waiting = FUSED || p.pdl_x;
   const int8_t* w0 = p.w + (int64_t)(n0 + g) * p.K;
   const int8_t* w1 = w0 + (int64_t)8 * p.K;
   const bool r0 = n0 + g < p.N, r1 = n0 + g + 8 < p.N;
@@ -201,23 +200,25 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
   // warps of the SM, 64 KB and more in flight
   constexpr int kAhead = MT <= 2 ? 4 : 2;
   const int step = p.split * kRWarps * 64;
-  // FUSED: every warp goes once round at least, for the block's quantisation
-  for (int k0 = (rank * kRWarps + warp) * 64; k0 < p.K; k0 += kAhead * step) {
-    uint4 a[kAhead], c[kAhead];
-    const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 a[kAhead], c[kAhead];
+  auto load = [&](int k0) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int k = k0 + j * step + t * 16;
       a[j] = k < p.K && r0 ? ldg_w(w0 + k) : zero;
       c[j] = k < p.K && r1 ? ldg_w(w1 + k) : zero;
     }
-    if constexpr (FUSED) {
-      if (waiting) rows_quantize<BF16>(p, xs, ldx, xmax_s, xscale_s);
-      waiting = false;
-    } else if (waiting) {  // the first weights are on their way while the codes of x are made
-      pdl_wait_prior_grids();
-      waiting = false;
-    }
+  };
+  int k0 = (rank * kRWarps + warp) * 64;
+  load(k0);
+  // the first weights are on their way while the codes of x are made
+  if constexpr (FUSED) {
+    rows_quantize<BF16>(p, xs, ldx, xmax_s, xscale_s);
+  } else if (p.pdl_x) {
+    pdl_wait_prior_grids();
+  }
+  while (k0 < p.K) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int k = k0 + j * step + t * 16;
@@ -234,13 +235,8 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
         mma_16832_s8(d[i], a[j].z, c[j].z, a[j].w, c[j].w, b.z, b.w);
       }
     }
-  }
-  if (waiting) {
-    if constexpr (FUSED) {
-      rows_quantize<BF16>(p, xs, ldx, xmax_s, xscale_s);
-    } else {
-      pdl_wait_prior_grids();
-    }
+    k0 += kAhead * step;
+    load(k0);
   }
   const uint32_t acc0 = smem_u32(acc_s);
   if (p.split > 1) {

@@ -395,7 +395,7 @@ def int8_linear(x: torch.Tensor, weight_int8: torch.Tensor, weight_scale: torch.
         x2 = _aligned(x2)
     m = x2.shape[0]
     y = x2.new_empty((m, n))
-    nbytes = _lib.load().nsq_int8_linear_workspace_size(m, k)
+    nbytes = _lib.load().nsq_int8_linear_workspace_size(m, k, n)
     work = x2.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _call(dev, "nsq_int8_linear", x2.data_ptr(), code, m, k, n, w.data_ptr(), ws.data_ptr(),
           None if b is None else b.data_ptr(), bcode, y.data_ptr(), None if work is None else work.data_ptr(), nbytes,
@@ -605,7 +605,7 @@ def linear_multi(x: torch.Tensor, mods) -> Optional[list]:
         return None
     if kinds == {"Int8Linear"}:  # one quantisation of x for all, at any batch size
         codes, scale = int8_quantize(x)
-        return [int8_linear_quantized(codes, scale, mm.weight_int8, mm.weight_scale, mm.bias, x.dtype) for mm in mods]
+        return [int8_linear_quantized(codes, scale, mm.weight_int8, mm.scale(), mm.bias, x.dtype) for mm in mods]
     k = x.shape[-1]
     lead = x.shape[:-1]
     x2 = _aligned(x.reshape(-1, k))

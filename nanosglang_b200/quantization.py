@@ -151,11 +151,15 @@ class Int8Linear(nn.Module):
             self.bias = None
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return ops.int8_linear(x, self.weight_int8, self.weight_scale, self.bias)
+        return ops.int8_linear(x, self.weight_int8, self.scale(), self.bias)
+
+    def scale(self) -> torch.Tensor:
+        """``weight_scale`` in float32 (a ``model.half()`` casts the buffer, too)."""
+        return self.weight_scale if self.weight_scale.dtype == torch.float32 else self.weight_scale.float()
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """``weight_int8 * weight_scale``, rounded once to dtype."""
-        return (self.weight_int8.float() * self.weight_scale[:, None]).to(dtype)
+        return (self.weight_int8.float() * self.scale()[:, None]).to(dtype)
 
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "Int8Linear":

@@ -158,6 +158,8 @@ def test_int8_linear_module_and_row_shards():
     assert ((m.weight_int8.double() * m.weight_scale.double()[:, None] - w).abs() <= step * (0.5 + 2.0 ** -17)).all()
     x = torch.randn(2, 5, 512, device="cuda").bfloat16()
     assert torch.equal(m(x), ops.int8_linear(x, m.weight_int8, m.weight_scale, m.bias))
+    cast = Int8Linear.from_linear(lin).bfloat16()  # casts weight_scale as well
+    assert torch.equal(cast(x), ops.int8_linear(x, m.weight_int8, m.weight_scale.bfloat16().float(), m.bias.bfloat16()))
     shards = [TP.RowParallelLinear.from_linear(m, 2, r, reduce_output=False) for r in range(2)]
     parts = [s(x[..., 256 * r:256 * (r + 1)]).double() for r, s in enumerate(shards)]
     want = [plain_linear(x[..., 256 * r:256 * (r + 1)], m.weight_int8[:, 256 * r:256 * (r + 1)], m.weight_scale,

@@ -24,10 +24,12 @@ def test_int8_linear_refusals():
     assert _int8(w=FAKE + 8) == _lib.EALIGN
     assert _int8(m=0) == _lib.OK  # nothing to do, needs no device
     lib = _lib.load()
-    assert lib.nsq_int8_linear_workspace_size(9, 48) == 9 * 48 + 9 * 4
-    assert lib.nsq_int8_linear_workspace_size(8, 528) == 8 * 528 + 8 * 4
-    assert lib.nsq_int8_linear_workspace_size(8, 512) == 0  # one launch
-    assert lib.nsq_int8_linear_workspace_size(0, 48) == 0
+    size = lib.nsq_int8_linear_workspace_size
+    assert size(9, 48, 16) == 9 * 48 + 9 * 4
+    assert size(8, 528, 16) == 8 * 528 + 8 * 4
+    assert size(8, 512, 16) == size(8, 512, 4096) == 0  # one launch
+    assert size(8, 512, 4112) == 8 * 512 + 8 * 4
+    assert size(0, 48, 16) == size(4, 48, 0) == 0
     assert lib.nsq_int8_quantize(FAKE, 7, 1, 8, FAKE, FAKE, None) == _lib.EINVAL
     assert lib.nsq_int8_quantize(FAKE, 1, 1, 0, FAKE, FAKE, None) == _lib.EINVAL
     assert lib.nsq_int8_quantize(FAKE, 1, 0, 8, FAKE, FAKE, None) == _lib.OK
@@ -77,6 +79,7 @@ def test_cache_call_refusals():
     assert att(sc=float("inf")) == _lib.EINVAL
     assert att(q=FAKE + 2) == _lib.EALIGN
     assert att(w=1 << 30) == _lib.ENOTSUP
+    assert att(b=1 << 28) == _lib.ENOTSUP
     assert att(b=0) == _lib.OK
 
 
