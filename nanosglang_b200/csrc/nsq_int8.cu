@@ -201,24 +201,24 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
   constexpr int kAhead = MT <= 2 ? 4 : 2;
   const int step = p.split * kRWarps * 64;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  uint4 a[kAhead], c[kAhead];
-  auto load = [&](int k0) {
+  int k0 = (rank * kRWarps + warp) * 64;
+  bool waiting = FUSED || p.pdl_x;
+  do {  // every warp once at least: all meet in the first round's quantisation
+    uint4 a[kAhead], c[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int k = k0 + j * step + t * 16;
       a[j] = k < p.K && r0 ? ldg_w(w0 + k) : zero;
       c[j] = k < p.K && r1 ? ldg_w(w1 + k) : zero;
     }
-  };
-  int k0 = (rank * kRWarps + warp) * 64;
-  load(k0);
-  // the first weights are on their way while the codes of x are made
-  if constexpr (FUSED) {
-    rows_quantize<BF16>(p, xs, ldx, xmax_s, xscale_s);
-  } else if (p.pdl_x) {
-    pdl_wait_prior_grids();
-  }
-  while (k0 < p.K) {
+    if (waiting) {  // the first weights are on their way while the codes of x are made
+      if constexpr (FUSED) {
+        rows_quantize<BF16>(p, xs, ldx, xmax_s, xscale_s);
+      } else {
+        pdl_wait_prior_grids();
+      }
+      waiting = false;
+    }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int k = k0 + j * step + t * 16;
@@ -236,8 +236,7 @@ __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParam
       }
     }
     k0 += kAhead * step;
-    load(k0);
-  }
+  } while (k0 < p.K);
   const uint32_t acc0 = smem_u32(acc_s);
   if (p.split > 1) {
     cluster_sync_all();  // the first CTA's sums are zero

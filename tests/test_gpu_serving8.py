@@ -167,3 +167,59 @@ def test_int8_linear_module_and_row_shards():
     eps = torch.finfo(torch.bfloat16).eps
     for a, b in zip(parts, want):
         assert ((a - b).abs() <= eps * b.abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_chain_with_programmatic_launch(captured):
+    """Projection -> cache write -> attention -> projection, step after step,
+    with programmatic dependent launch on: every kernel waits for the one it
+    reads from, so nothing changes."""
+    from nanosglang_b200 import QuantizedKVCache, _lib, ops
+    g = torch.Generator().manual_seed(15)
+    heads, kvh, dim, hidden, bs = 8, 2, 64, 512, 5
+    layers = []
+    for n, k in ((heads * dim, hidden), (kvh * dim, hidden), (kvh * dim, hidden), (hidden, heads * dim)):
+        layers.append((torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8).cuda(),
+                       (torch.rand(n, generator=g) * 1e-3).cuda()))
+    x0 = torch.randn(bs, hidden, generator=g).bfloat16().cuda()
+    table = torch.arange(bs * 20, dtype=torch.int32).view(bs, 20).cuda()
+
+    def run(steps):
+        cache = QuantizedKVCache(bs * 20, 16, kvh, dim, "fp8", "cuda")
+        lens = torch.zeros(bs, dtype=torch.int32, device="cuda")
+        places = torch.arange(bs, device="cuda") * 320
+        x = x0.clone()
+
+        def step():
+            q, k, v = (ops.int8_linear(x, w, s) for w, s in layers[:3])
+            cache.write(k.view(bs, kvh, dim), v.view(bs, kvh, dim), places)
+            lens.add_(1)
+            places.add_(1)
+            o = cache.attend(q.view(bs, heads, dim), table, lens)
+            x.copy_(torch.tanh(ops.int8_linear(o.view(bs, -1), *layers[3]) + x))
+
+        if captured:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.current_stream().wait_stream(side)
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr):
+                step()
+            for _ in range(steps - 1):
+                gr.replay()
+        else:
+            for _ in range(steps):
+                step()
+        torch.cuda.synchronize()
+        return x, cache.read(torch.arange(bs * 320, device="cuda"), torch.bfloat16)
+
+    want, want_kv = run(200)
+    prev = _lib.set_pdl(True)
+    try:
+        got, got_kv = run(200)
+    finally:
+        _lib.set_pdl(prev)
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(got_kv, want_kv))
+    assert _lib.device_status()[0] == 0
