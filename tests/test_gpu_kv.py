@@ -231,6 +231,25 @@ def test_attention_splits(lens, heads, group, dim, codes):
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("lens", [[700], [0, 513, 1, 300], [33] * 40, [129, 0, 0, 256] * 36])
+@pytest.mark.parametrize("heads,group", [(5, 1), (12, 1), (17, 9), (32, 1), (37, 1), (64, 1)])
+def test_attention_many_kv_heads(heads, group, lens):
+    """Heads that are walked side by side in every number (37: alone, 64: two
+    rows of 32, 17 x 9: 34 items of a sequence in two rows), more items than
+    workers and fewer, segments of one unit."""
+    from nanosglang_b200 import ops
+    dim, page, codes = 64, 16, torch.int8
+    pages = sum(-(-n // page) for n in lens) + 3
+    pool = make_pool(pages, page, heads, dim, codes, "nhd", seed=20)
+    table, n = tables(lens, page, pages, seed=21)
+    g = torch.Generator().manual_seed(22)
+    q = torch.randn(len(lens), heads * group, dim, generator=g).to(torch.bfloat16).cuda()
+    out, lse = ops.kv_attention_decode(q, *pool, table, n, return_lse=True)
+    check_attention(out, lse, q, pool, table, n, dim ** -0.5)
+    again = ops.kv_attention_decode(q, *pool, table, n)
+    assert torch.equal(out, again)
+
+
 @pytest.mark.parametrize("codes", CODES)
 def test_attention_ranges(codes):
     """Scales of v over thirty orders of magnitude within one sequence, peaked
