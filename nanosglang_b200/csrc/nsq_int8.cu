@@ -22,8 +22,8 @@ constexpr int kQThreads = 256;
 // ---------------------------------------------------------------------------
 // Row quantiser: TPR threads per row, NV vectors of 16 bytes each, which stay in
 // registers between the maximum and the codes (one pass over DRAM, which bounds
-// it). Few rows take 256 threads each (latency), many the fewest that hold a
-// row (no waiting for other warps). int8_quantize_any_kernel takes any row
+// it: 8192 x 4096 bf16 18.4 us, 5.5 TB/s; 16 x 4096 1.6 us). The host says
+// how many threads a row takes. int8_quantize_any_kernel takes any row
 // length, alignment and type, element by element, and reads the row twice (the
 // second time from L2).
 // ---------------------------------------------------------------------------
@@ -176,6 +176,9 @@ __device__ __forceinline__ void rows_quantize(const RowsParams& p, int8_t* xs, i
 // FUSED (up to 8 tokens, few elements): x is 16-bit; every CTA quantises all of
 // it into its shared memory while its first weights are on their way, which
 // takes less time than a launch of the row quantiser and its round trip.
+// The weight's stream bounds it, for small layers the round trips of one pass
+// (in a graph, all included: 1 x 896 -> 4864 3.8 us, 1 x 4096 -> 4096 7.0 us =
+// 2.4 TB/s, 8 x 14336 -> 4096 21 us = 2.8 TB/s).
 template <int MT, bool BF16, bool FUSED>
 __global__ void __launch_bounds__(kRWarps * 32) int8_rows_kernel(const RowsParams p) {
   constexpr int kLd = 8 * MT + 1;
@@ -304,12 +307,16 @@ static cudaError_t quantize_rows(const uint16_t* x, int M, int K, int8_t* codes,
                                  bool pdl) {
   const dim3 grid((unsigned)((M + kQThreads / TPR - 1) / (kQThreads / TPR)));
   const int per = (K / 8 + TPR - 1) / TPR;
-  auto go = [&](auto kern) { return launch(kern, grid, kQThreads, 0, 1, stream, pdl, x, M, K, codes, scale, (int)pdl); };
+  auto go = [&](auto kern) {
+    return launch(kern, grid, kQThreads, 0, 1, stream, pdl, x, M, K, codes, scale, (int)pdl);
+  };
+  if constexpr (TPR == 256) {
+    if (per > 8) return go(int8_quantize_kernel<TPR, 16, BF16>);
+  }
   return per <= 1   ? go(int8_quantize_kernel<TPR, 1, BF16>)
          : per <= 2 ? go(int8_quantize_kernel<TPR, 2, BF16>)
          : per <= 4 ? go(int8_quantize_kernel<TPR, 4, BF16>)
-         : per <= 8 ? go(int8_quantize_kernel<TPR, 8, BF16>)
-                    : go(int8_quantize_kernel<TPR, 16, BF16>);
+                    : go(int8_quantize_kernel<TPR, 8, BF16>);
 }
 
 cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K, int8_t* codes, float* scale,
@@ -318,8 +325,8 @@ cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t
   const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 16 * 8 * kQThreads &&
                    ((reinterpret_cast<uintptr_t>(x) & 15) | (reinterpret_cast<uintptr_t>(codes) & 7)) == 0;
   if (!vec) {
-    return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 0, 1, stream, pdl, x, dtype, K, codes, scale,
-                  (int)pdl);
+    return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 0, 1, stream, pdl, x, dtype, K, codes,
+                  scale, (int)pdl);
   }
   const uint16_t* x16 = static_cast<const uint16_t*>(x);
   auto go = [&](auto tpr) {
@@ -327,11 +334,14 @@ cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t
     return dtype == NSQ_DTYPE_BF16 ? quantize_rows<T, true>(x16, (int)rows, (int)K, codes, scale, stream, pdl)
                                    : quantize_rows<T, false>(x16, (int)rows, (int)K, codes, scale, stream, pdl);
   };
+  // Threads of a row, measured (us; 32, 64, 128, 256 threads): few rows want all
+  // of them (512 x 4096 5.4, 4.7, 3.7, 3.6); many rows a warp while it loads the
+  // row in few steps (16384 x 896 9.5, 11.1, 14.0, 21.2; 8192 x 1536 9.2, 9.3,
+  // 10.6, 13.4), then 128 (16384 x 2048 23.5, 23.2, 20.9, 26.7; 8192 x 4096
+  // 23.9, 23.7, 18.4, 20.8) until these need more than eight steps.
   const bool few = rows < 8 * num_sms();
   if (few || K > 128 * 64) return go(std::integral_constant<int, 256>());
-  if (K > 64 * 64) return go(std::integral_constant<int, 128>());
-  if (K > 32 * 64) return go(std::integral_constant<int, 64>());
-  return go(std::integral_constant<int, 32>());
+  return K > 1536 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 32>());
 }
 
 int run_int8_rows(const Int8Args& a, cudaStream_t stream) {

@@ -104,6 +104,29 @@ def test_linear(m, k, n, dtype):
     assert torch.equal(ops.int8_linear_quantized(codes, s, w, ws, b, dtype), y)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", [(70, 128, 4728), (200, 384, 10008), (40, 256, 16000), (500, 128, 4096),
+                                   (300, 896, 4864), (1300, 1040, 904)])
+def test_linear_uneven_tiles(m, k, n, dtype):
+    """Tiles of other than 64 or 128 rows, the last one short, 8 features to a store."""
+    from nanosglang_b200 import ops
+    x, w, ws, b = make(m, k, n, dtype, dtype, seed=n)
+    check_linear(ops.int8_linear(x, w, ws, b), x, w, ws, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1301, 8), (1301, 1016), (1190, 1536), (1185, 1544), (1200, 2048), (1187, 4104),
+                                    (1185, 8192), (1185, 8200), (20000, 136)])
+def test_quantize_many_rows(rows, k, dtype):
+    """Every number of threads and vectors a row takes when rows are many."""
+    from nanosglang_b200 import ops
+    x = torch.randn(rows, k, generator=torch.Generator().manual_seed(rows + k)).to(dtype)
+    x[rows // 2] = 0
+    codes, s = ops.int8_quantize(x.cuda())
+    rc, rs = ref_quantize(x)
+    assert torch.equal(codes.cpu(), rc) and torch.equal(s.cpu(), rs)
+
+
 def test_linear_largest_sums():
     """The longest K with every product at its largest: 127 * 128 * 131072 is just under 2^31."""
     from nanosglang_b200 import ops
