@@ -301,9 +301,9 @@ int nsq_kv_cache_read(const nsq_kv_cache* cache, const int64_t* slots, int64_t T
 size_t nsq_kv_attention_workspace_size(int64_t B, int64_t H, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                                        int64_t table_width);
 int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, int64_t q_seq_stride,
-                            int64_t q_head_stride, int64_t B, int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
-                            const int32_t* seq_lens, float softmax_scale, void* out, float* lse, void* workspace,
-                            size_t workspace_bytes, void* stream);
+                            int64_t q_head_stride, int64_t B, int64_t H, const int32_t* page_table, int64_t table_stride,
+                            int64_t table_width, const int32_t* seq_lens, float softmax_scale, void* out, float* lse,
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 /* Limit, in nanoseconds, of every bounded device-side wait that reports to the
  * status word (0 restores the default of 2 s; nsq_device_status_reset also

@@ -84,7 +84,8 @@ SIGNATURES = {
     "nsq_kv_cache_read": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
     "nsq_kv_attention_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64]),
     "nsq_kv_attention_decode": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p,
-                                        c_int64, c_int64, c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                        c_int64, c_int64, c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_size_t,
+                                        c_void_p]),
     "nsq_set_pdl": (c_int, [c_int]),
     "nsq_set_wait_limit_ns": (c_int, [ctypes.c_uint64]),
     "nsq_set_sm_reserve": (c_int, [c_int]),

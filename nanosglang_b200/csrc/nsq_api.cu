@@ -803,9 +803,9 @@ size_t nsq_kv_attention_workspace_size(int64_t B, int64_t H, int64_t kv_heads, i
 }
 
 int nsq_kv_attention_decode(const nsq_kv_cache* cache, const void* q, int q_dtype, int64_t q_seq_stride,
-                            int64_t q_head_stride, int64_t B, int64_t H, const int32_t* page_table, int64_t table_stride, int64_t table_width,
-                            const int32_t* seq_lens, float softmax_scale, void* out, float* lse, void* workspace,
-                            size_t workspace_bytes, void* stream) {
+                            int64_t q_head_stride, int64_t B, int64_t H, const int32_t* page_table, int64_t table_stride,
+                            int64_t table_width, const int32_t* seq_lens, float softmax_scale, void* out, float* lse,
+                            void* workspace, size_t workspace_bytes, void* stream) {
   KvAttnArgs a{};
   int rc = kv_check(cache, &a.c);
   if (rc != NSQ_OK) return rc;

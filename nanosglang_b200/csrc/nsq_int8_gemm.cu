@@ -16,8 +16,11 @@
 //
 // Warp roles (per CTA, 352 threads): 0 TMA of the weight, 1 MMA issuer (of a
 // pair, the even CTA's), 2 TMA of x (one lane issues a copy in about 100 cycles,
-// so one warp for all four of a stage would set the pace), 3..10 epilogue. A stage holds two 128-column k-blocks, so a
-// barrier round covers 8 MMAs. With one token tile (decode batches) it is the
+// so one warp for all four of a stage would set the pace), 3..10 epilogue. A
+// stage holds two 128-column k-blocks, so a barrier round covers 8 MMAs.
+// An MMA of one CTA takes about 62 cycles for its 128 rows and half a cycle a
+// token (with 64 rows 51), which bounds small layers at few tokens: 128 x 4096
+// -> 4096 takes 10.3 us, 5.3 of them in the MMAs. With one token tile (decode batches) it is the
 // weight's bandwidth that counts: the rows are then dealt evenly over the SMs,
 // fewer than 128 to a tile (the MMA's other rows compute on leftovers of the
 // stage that nothing reads), and the ring keeps 150 KB or more per SM in flight.
@@ -56,7 +59,7 @@ struct GemmShape {
   static constexpr int kTokRound = TOK < 128 ? TOK : 128;  // tokens of a staged y tile
   static constexpr int kWarpTok = kTokRound < 64 ? 32 : kTokRound / 2;  // of them, an epilogue warp's
   static constexpr int kYHalf = kTokRound * 64 * 2;        // 64 features
-  static constexpr int NS = (226 * 1024 - 2 * kYHalf - 1024) / kStage < 6 ? (226 * 1024 - 2 * kYHalf - 1024) / kStage : 6;
+  static constexpr int kFit = (226 * 1024 - 2 * kYHalf - 1024) / kStage, NS = kFit < 6 ? kFit : 6;
   static constexpr int kY = NS * kStage;
   static constexpr int kBar = kY + 2 * kYHalf;
   // full[NS], done[NS], full_acc[2], empty_acc[2], drain, sums
@@ -111,7 +114,9 @@ __host__ __device__ constexpr uint32_t idesc_s8(int m, int n) {
 template <int CG>
 __device__ __forceinline__ void umma_i8_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
 #define NSQ_I8_PRE "{\n\t.reg .pred e, p, t;\n\t.reg .b32 r;\n\telect.sync r|e, 0xffffffff;\n\t"
-#define NSQ_I8_4(M) M "[%0], %1, %5, %9, p;\n\t" M "[%0], %2, %6, %9, t;\n\t" M "[%0], %3, %7, %9, t;\n\t" M "[%0], %4, %8, %9, t;\n\t"
+#define NSQ_I8_4(M)                                                     \
+  M "[%0], %1, %5, %9, p;\n\t" M "[%0], %2, %6, %9, t;\n\t"              \
+  M "[%0], %3, %7, %9, t;\n\t" M "[%0], %4, %8, %9, t;\n\t"
 #define NSQ_I8_GO(M)                                                                                                   \
   asm volatile(NSQ_I8_PRE "setp.ne.b32 p, %10, 0;\n\tsetp.eq.b32 t, %10, %10;\n\t" NSQ_I8_4(M) "}" ::"r"(d), "l"(a),   \
                "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc),              \
@@ -161,7 +166,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
   using S = GemmShape<CG, TOK>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar);  // a stage's tiles landed (pair: both CTAs', even CTA's barrier)
+  // a stage's tiles landed (pair: both CTAs', even CTA's barrier)
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar);
   uint64_t* done = full + S::NS;                                 // its MMAs finished (both CTAs)
   uint64_t* full_acc = done + S::NS;                             // an accumulator is complete (both CTAs)
   uint64_t* empty_acc = full_acc + 2;                            // and read out by every epilogue warp (even CTA)
@@ -247,7 +253,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
           const int kb0 = st * kKps;
           const int nk = p.num_kb - kb0 < kKps ? p.num_kb - kb0 : kKps;
           // the even CTA arms the barrier for the bytes of both
-          if (!is_x && leader) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * nk) * (uint32_t)(p.wrows * kBK + S::kXBytes));
+          if (!is_x && leader) {
+            mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * nk) * (uint32_t)(p.wrows * kBK + S::kXBytes));
+          }
 #pragma unroll
           for (int i = 0; i < kKps; ++i) {
             if (i < nk) {

@@ -262,8 +262,15 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 //     token-major pool they read whole rows of memory between them (48 x 8192,
 //     8 kv heads of 128: 146 us, on their own 178). A warp's range covers whole
 //     items and at most two cut ones; those go to the workspace as fp32
-//     partials, and a second kernel joins them in order. Where no sequence can hold more than
-//     128 tokens an item is one unit: nothing is cut and one launch does.
+//     partials, and a second kernel joins them in order. Where no sequence can
+//     hold more than 128 tokens an item is one unit: nothing is cut and one
+//     launch does.
+// Measured (8 kv heads of 128, 4 query heads each, e4m3, bf16 q, the join
+// included): 48 x 8192 tokens 146 us, 5.7 TB/s; 64 x 2048 58 us, 4.7 TB/s;
+// 1 x 131001 60 us; 1 x 2048 10.5 us; 1 x 40 (2 kv heads of 64, int8) 7.0 us. Of
+// the 58 us 2 pass before the first copy is issued, 43 are the stream at the
+// rate of a plain copy, about 7 the last warps of an even deal (their rates
+// differ by 10%) and 4 the join with its launch.
 
 constexpr int kAttnWarps = 4;
 constexpr int kTile = 32;  // tokens of a stage

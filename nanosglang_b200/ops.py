@@ -596,9 +596,10 @@ def _ptr_array(vals, ctype=None):
 
 def linear_multi(x: torch.Tensor, mods) -> Optional[list]:
     """One launch for 1..3 AWQLinear (or 1..3 FP8Linear) layers that read the
-    same x, e.g. q/k/v; Int8Linear layers share one quantisation of x (any M). Returns their outputs as views of one [M, sum N]
-    buffer, or None when the fused kernel does not apply (M > 32, mixed
-    formats, bias dtypes that differ, group sizes that differ)."""
+    same x, e.g. q/k/v; Int8Linear layers share one quantisation of x (any M).
+    Returns their outputs as views of one [M, sum N] buffer (Int8Linear: a buffer
+    each), or None when the fused kernel does not apply (M > 32, mixed formats,
+    bias dtypes that differ, group sizes that differ)."""
     mods = [_unwrap(m) for m in mods]
     kinds = {type(m).__name__ for m in mods}
     if len(kinds) != 1 or x.dtype not in _ACT_CODES:

@@ -32,7 +32,8 @@ import torch.nn as nn
 
 from . import ops
 
-__all__ = ["FP8Linear", "AWQLinear", "Int8Linear", "quantize_model", "load_autoawq_state_dict", "FusedProjections", "GateUpSiLU"]
+__all__ = ["FP8Linear", "AWQLinear", "Int8Linear", "quantize_model", "load_autoawq_state_dict", "FusedProjections",
+           "GateUpSiLU"]
 
 
 class FP8Linear(nn.Module):
