@@ -20,10 +20,11 @@
 // stage holds two 128-column k-blocks, so a barrier round covers 8 MMAs.
 // An MMA of one CTA takes about 62 cycles for its 128 rows and half a cycle a
 // token (with 64 rows 51), which bounds small layers at few tokens: 128 x 4096
-// -> 4096 takes 10.3 us, 5.3 of them in the MMAs. With one token tile (decode batches) it is the
-// weight's bandwidth that counts: the rows are then dealt evenly over the SMs,
-// fewer than 128 to a tile (the MMA's other rows compute on leftovers of the
-// stage that nothing reads), and the ring keeps 150 KB or more per SM in flight.
+// -> 4096 takes 10.3 us, 5.3 of them in the MMAs. With one token tile (decode
+// batches) it is the weight's bandwidth that counts: the rows are then dealt
+// evenly over the SMs, fewer than 128 to a tile (the MMA's other rows compute on
+// leftovers of the stage that nothing reads), and the ring keeps 150 KB or more
+// per SM in flight.
 // Where tiles are few and K is long, a cluster of up to 4 CTAs shares a tile
 // along K (SPLIT): each copies its sums of every other one's slice of tokens
 // there in bulk, adds up its own slice and finishes it (integers: exact in any
