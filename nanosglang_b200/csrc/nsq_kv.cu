@@ -1199,11 +1199,18 @@ AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t cap
 }
 
 // The codes as a 4-D tensor (head_dim, token and head in the order of their
-// strides, page); a box is 16 tokens of one head.
+// strides, page); a box is 16 tokens of one head. False where a tensor map
+// cannot hold them: one whose pages, tokens or heads are the same memory (a
+// stride of 0, as of an expanded tensor) is among these. A stride of a dimension
+// of size 1 is 0 as well, but never used: the map gets 16 for it.
 bool encode_pool(CUtensorMap* map, const KvCache& c, uint8_t* base, const int64_t (&stride)[3], bool* swap) {
+  const int size[3] = {c.num_pages, c.page_size, c.kv_heads};
+  for (int i = 0; i < 3; ++i) {
+    if (stride[i] == 0 && size[i] > 1) return false;
+  }
   *swap = stride[2] < stride[1];
-  const uint64_t tok = (uint64_t)stride[1] ? stride[1] : 16, head = (uint64_t)stride[2] ? stride[2] : 16,
-                 page = (uint64_t)stride[0] ? stride[0] : 16;
+  const uint64_t tok = stride[1] ? (uint64_t)stride[1] : 16, head = stride[2] ? (uint64_t)stride[2] : 16,
+                 page = stride[0] ? (uint64_t)stride[0] : 16;
   const uint32_t rb = c.head_dim <= 64 ? 64 : 128;
   const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)(*swap ? c.kv_heads : c.page_size),
                             (uint64_t)(*swap ? c.page_size : c.kv_heads), (uint64_t)c.num_pages};

@@ -1,0 +1,39 @@
+"""Caches whose pages, tokens or heads share memory (expanded tensors), as the
+calls that only read them may get."""
+
+import pytest
+import torch
+
+from test_gpu_kv import CODES, check_attention, make_pool, tables
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("shared", ["heads", "pages", "tokens", "k heads only"])
+def test_attention_over_an_expanded_pool(shared, page, dim, codes):
+    """One stored head, page or token stands for all of them (stride 0): the
+    same bits as the pool written out."""
+    from nanosglang_b200 import ops
+    heads, lens = 4, [100, 0, 1, 333]
+    pages = sum(-(-n // page) for n in lens) + 1
+    dims = {"heads": 2, "pages": 0, "tokens": 1, "k heads only": 2}[shared]
+    pool = make_pool(pages, page, heads, dim, codes, seed=31)
+    view = []
+    for i, t in enumerate(pool):
+        raw = t.view(torch.uint8) if t.dtype == codes else t
+        if shared != "k heads only" or i in (0, 2):
+            raw = raw.narrow(dims, 0, 1).clone().expand(raw.shape)
+        view.append(raw.view(codes) if t.dtype == codes else raw)
+    full = [t.contiguous() for t in view]
+    table, lens_t = tables(lens, page, pages, seed=32)
+    q = torch.randn(4, 8, dim, generator=torch.Generator().manual_seed(33)).bfloat16().cuda()
+    out, lse = ops.kv_attention_decode(q, *view, table, lens_t, return_lse=True)
+    check_attention(out, lse, q, full, table, lens_t, dim ** -0.5)
+    want, want_lse = ops.kv_attention_decode(q, *full, table, lens_t, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    slots = torch.arange(pages * page).cuda()
+    for a, b in zip(ops.kv_cache_read(*view, slots, torch.half), ops.kv_cache_read(*full, slots, torch.half)):
+        assert torch.equal(a, b)
