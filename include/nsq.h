@@ -244,7 +244,8 @@ int nsq_int8_linear_quantized(const int8_t* codes, const float* scale, int64_t M
  * (scales are >= 0; a row with a NaN or an infinity reads back as NaN).
  * Strides are in elements, in the order page, token, head; head_dim is
  * contiguous, so token-major and head-major pools both fit; strides are below
- * 2^32 (one of a dimension of size 1 is not looked at). Code strides are
+ * 2^32 (one of a dimension of size 1 is not looked at; one of 0, where heads,
+ * tokens or pages share memory, is refused by the write). Code strides are
  * multiples of 16, code pointers 16-byte aligned, head_dim a multiple of 16 up
  * to 256, num_pages * page_size < 2^31.
  *

@@ -751,6 +751,13 @@ int nsq_kv_cache_write(const nsq_kv_cache* cache, const void* k, const void* v, 
   int rc = kv_check(cache, &c);
   if (rc != NSQ_OK) return rc;
   if (T < 0 || !valid_act_dtype(x_dtype)) return NSQ_EINVAL;
+  // places that share memory: the rows of several heads, tokens or pages would overwrite one another
+  const int sizes[3] = {c.num_pages, c.page_size, c.kv_heads};
+  for (int i = 0; i < 3; ++i) {
+    if (sizes[i] > 1 && (c.k_stride[i] == 0 || c.v_stride[i] == 0 || c.ks_stride[i] == 0 || c.vs_stride[i] == 0)) {
+      return NSQ_EINVAL;
+    }
+  }
   if (T > ((int64_t)1 << 30) / c.kv_heads) return NSQ_ENOTSUP;
   if (T == 0) return NSQ_OK;
   if (!k || !v || !slots) return NSQ_EINVAL;

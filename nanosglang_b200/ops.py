@@ -485,7 +485,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
 
     k_cache, v_cache: int8 or float8_e4m3fn [pages, page_size, kv_heads,
     head_dim], any strides with head_dim contiguous (token-major or head-major
-    pools); k_scale, v_scale: float32 [pages, page_size, kv_heads]. Token t
+    pools; no expanded ones, whose places share memory); k_scale, v_scale: float32 [pages, page_size, kv_heads]. Token t
     goes to place ``slots[t] = page * page_size + offset`` (int64); a negative
     slot is a padded token and is skipped, one past the pool is skipped and
     recorded in the status word. Slots are distinct: of two tokens with the

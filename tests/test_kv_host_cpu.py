@@ -1,0 +1,21 @@
+"""Host-side checks of the 8-bit cache that need no GPU."""
+
+import pytest
+
+from test_int8_kv_cpu import FAKE, _desc
+
+from nanosglang_b200 import _lib
+
+
+@pytest.mark.parametrize("what", ["k_stride", "v_stride", "k_scale_stride", "v_scale_stride"])
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_write_refuses_places_that_share_memory(what, dim):
+    """A stride of 0 in a dimension of more than one: rows would overwrite one
+    another. Of a dimension of one it is not looked at."""
+    lib = _lib.load()
+    strides = [2048, 128, 64] if "scale" not in what else [32, 2, 1]
+    strides[dim] = 0
+    write = lambda d: lib.nsq_kv_cache_write(d, FAKE, FAKE, 1, 128, 64, 128, 64, 0, FAKE, None)  # noqa: E731
+    assert write(_desc(**{what: tuple(strides)})) == _lib.EINVAL
+    one = {("num_pages", "page_size", "kv_heads")[dim]: 1}
+    assert write(_desc(**{what: tuple(strides)}, **one)) == _lib.OK
