@@ -318,8 +318,10 @@ int nsq_set_wait_limit_ns(uint64_t ns);
  * chosen, e.g. M = 16, K = 896, N = 9728) never requests the first weight box
  * of its first row group, so that group's bounded wait runs out: the kernel
  * records NSQ_EDEVICE_TIMEOUT (tag 1) in the status word, lets every copy it
- * did request land, and returns. Its output is then undefined. No counterpart
- * in the reference. Not for production use. */
+ * did request land, and returns. Its output is then undefined. Likewise the
+ * first stage of decode attention's first worker never completes (tag 204): the
+ * rows of that worker's share are then undefined, the others are right. No
+ * counterpart in the reference. Not for production use. */
 int nsq_test_withhold_weight_load(int enable);
 
 /*

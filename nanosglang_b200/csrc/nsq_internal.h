@@ -16,7 +16,7 @@ DevStatus* device_status_ptr(); // device address of this device's status word (
 bool pdl_enabled();
 // Lets `kernel` use `bytes` of dynamic shared memory on the current device (set once per kernel and device).
 cudaError_t allow_dynamic_smem(const void* kernel, int bytes);
-bool test_withhold();  // failure-path test hook: the multi-wave decode kernel skips one weight load
+bool test_withhold();  // failure-path test hook: one wait of a kernel that looks at it never completes
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (libnsq does
 // not link libcuda directly, so it also loads on machines without a driver).

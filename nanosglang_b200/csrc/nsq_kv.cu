@@ -49,6 +49,7 @@ struct KvAttn : KvAttnArgs {
   int4* meta;
   DevStatus* status;
   bool pdl;
+  bool withhold;  // failure-path test hook: the first worker's first stage never completes
 };
 
 // Records the first bad value in a device-side argument (tag 200 a written
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
   const int vpt = (p.B + kAttnWarps * 32 - 1) / (kAttnWarps * 32);  // sequences of a thread
   const int n_first = tid * vpt < p.B ? __ldg(p.seq_lens + tid * vpt) : 0;  // on its way during the set-up
   // a phase: the lanes' copies, and one arrival of lane 0 (TMA: with the bytes)
-  if (lane < S::kStages) mbar_init(&full[lane], 33);
+  if (lane < S::kStages) mbar_init(&full[lane], 33 + (p.withhold && tid == 0 && blockIdx.x == 0));
   fence_barrier_init();
   if (TMA && tid == 0) {
     tma_prefetch_desc(&kmap);
@@ -993,7 +994,11 @@ __global__ void __launch_bounds__(PAIRS == 1 ? 256 : 32 * PAIRS) kv_attn_join_ke
     item = pair - h * items;
     if (h >= p.slot_heads || ((item % kh_n) % p.head_blocks) * kHeads + h >= p.group) return 0;
     me = __ldg(p.meta + item);
-    return me.x < 0 ? 0 : me.x;
+    // a worker whose wait ran out leaves what it should have written as it was:
+    // nothing that the grid cannot have written is followed
+    const int workers = p.teams * p.abreast;
+    const bool in_grid = me.x <= p.teams && (uint32_t)me.y < 2u * (uint32_t)workers && (uint32_t)me.z < (uint32_t)workers;
+    return me.x > 0 && in_grid && me.z + (me.x - 1) * p.abreast < workers ? me.x : 0;
   };
   auto store = [&](int item, int h, int d4, float4 acc, float sum, float mm, float m) {
     const int b = item / kh_n, kh = item - b * kh_n;
@@ -1322,6 +1327,7 @@ cudaError_t launch_kv_attn(const KvAttnArgs& args, bool fp8, bool bf16, void* ws
   p.meta = a.cut ? reinterpret_cast<int4*>(static_cast<uint8_t*>(ws) + attn_slot_bytes(a)) : nullptr;
   p.status = device_status_ptr();
   p.pdl = pdl_enabled();
+  p.withhold = test_withhold();
   return a.dp == 64    ? run_attn_t<64>(p, a, fp8, bf16, stream)
          : a.dp == 128 ? run_attn_t<128>(p, a, fp8, bf16, stream)
                        : run_attn_t<256>(p, a, fp8, bf16, stream);
