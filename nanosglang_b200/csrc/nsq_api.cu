@@ -67,12 +67,16 @@ constexpr int64_t kIntMax = 0x7FFFFFFF;
 
 }  // namespace
 
-int num_sms() {
+int device_sms() {
   const int d = current_device();
   if (d < 0) return 148;
   if (g_sms[d].load(std::memory_order_acquire) == 0) check_device();
   const int sms = g_sms[d].load(std::memory_order_acquire);
-  const int all = sms > 0 ? sms : 148;
+  return sms > 0 ? sms : 148;
+}
+
+int num_sms() {
+  const int all = device_sms();
   const int use = all - g_sm_reserve.load(std::memory_order_relaxed);
   return use >= all / 2 ? use : all / 2;
 }

@@ -10,7 +10,8 @@ namespace nsq {
 
 struct DevStatus;
 
-int num_sms();                  // SM count of the current device (cached per device)
+int device_sms();               // SM count of the current device (cached per device)
+int num_sms();                  // of them, those that grids are sized for (all but nsq_set_sm_reserve's)
 int device_ready();             // NSQ_OK if the current device is sm_100, else an NSQ_E* code
 DevStatus* device_status_ptr(); // device address of this device's status word (lazily set up)
 bool pdl_enabled();

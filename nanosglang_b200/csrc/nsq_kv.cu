@@ -1182,7 +1182,7 @@ struct AttnPlan {
   bool cut;       // an item can span workers: the join kernel and its workspace are needed
 };
 
-AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t capacity) {
+AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t capacity, int sms) {
   AttnPlan a{};
   a.dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
   // more than 8 query heads of a kv head are several items, which read the same
@@ -1192,7 +1192,7 @@ AttnPlan attn_plan(int64_t B, int group, int kv_heads, int head_dim, int64_t cap
   const int per_sm = a.dp == 64 ? AttnShape<64>::kPerSm : a.dp == 128 ? AttnShape<128>::kPerSm : AttnShape<256>::kPerSm;
   const int64_t units = capacity <= kWhole * kTile ? 1 : (capacity + kTile - 1) / kTile;
   const int64_t items = B * kv_heads * a.head_blocks;
-  const int64_t most = (int64_t)num_sms() * per_sm;
+  const int64_t most = (int64_t)sms * per_sm;
   a.ctas = (int)(items > most / units ? most : items * units);
   a.cut = units > 1;
   for (int i = 1; i <= 32; ++i) {
@@ -1300,19 +1300,21 @@ cudaError_t launch_kv_read(const KvCache& c, const int64_t* slots, int T, void* 
 // Workspace: per worker two partial slots ([heads][head_dim + 4] fp32 each: two
 // references, the denominator, a pad, the accumulator), then one int4 per item:
 // its partials (-1: not cut), the first one's slot, and the worker of that slot;
-// the others are the first slots of its place in the teams after.
+// the others are the first slots of its place in the teams after. Its size is
+// for all SMs of the device: SMs kept free for others (which may change from
+// one call to the next, and during one) only make the grid of a launch smaller.
 static size_t attn_slot_bytes(const AttnPlan& a) {
   return (size_t)a.ctas * kAttnWarps * 2 * a.slot_heads * (a.dp + 4) * sizeof(float);
 }
 
 size_t kv_attn_workspace(int64_t B, int group, int kv_heads, int head_dim, int64_t capacity) {
-  const AttnPlan a = attn_plan(B, group, kv_heads, head_dim, capacity);
+  const AttnPlan a = attn_plan(B, group, kv_heads, head_dim, capacity, device_sms());
   return a.cut ? attn_slot_bytes(a) + (size_t)B * kv_heads * a.head_blocks * sizeof(int4) : 0;
 }
 
 cudaError_t launch_kv_attn(const KvAttnArgs& args, bool fp8, bool bf16, void* ws, cudaStream_t stream) {
   const int group = args.H / args.c.kv_heads;
-  const AttnPlan a = attn_plan(args.B, group, args.c.kv_heads, args.c.head_dim, args.capacity);
+  const AttnPlan a = attn_plan(args.B, group, args.c.kv_heads, args.c.head_dim, args.capacity, num_sms());
   KvAttn p{args};
   p.group = group;
   p.head_blocks = a.head_blocks;
