@@ -291,15 +291,16 @@ __device__ __forceinline__ float lg2(float x) {
 constexpr float kNoMax = -3e38f;  // below every score: exp2(x - kNoMax) is 0 for a masked x, and nothing is NaN
 
 // 2^(m - mm): what turns exp2(x - m) * vs into a weight relative to mm (0 while there is none)
-__device__ __forceinline__ float weight_factor(float m, float mm) {
-  return mm == kNoMax ? 0.f : ex2(fminf(m - mm, 126.f));
-}
-// acc * 2^(mm - m) / sum: the output of a head whose weights of v were taken
-// relative to mm and whose denominator relative to m (0 for an empty row;
-// without a scale above 0, mm is kNoMax and acc 0 or NaN).
+constexpr float kLeast = 126.f;  // mm is at least m - kLeast, so that the factor stays in fp32's range
+__device__ __forceinline__ float weight_factor(float m, float mm) { return mm == kNoMax ? 0.f : ex2(m - mm); }
+// acc / sum * 2^(mm - m): the output of a head whose weights of v were taken
+// relative to mm and whose denominator relative to m (0 for an empty row). The
+// sum of n terms goes first and the power in two steps, so that nothing on
+// the way leaves fp32's range where the output does not.
 __device__ __forceinline__ float finish(float acc, float sum, float mm, float m) {
   if (sum == 0.f) return 0.f;
-  return acc * (mm == kNoMax ? 0.f : ex2(mm - m)) / sum;
+  const float half = ex2(0.5f * (mm - m));
+  return acc / sum * half * half;
 }
 __device__ __forceinline__ float head_lse(float sum, float m) {
   return sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
@@ -809,7 +810,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
             big = fmaxf(big, wt[h][2 * r + e]);
           }
         }
-        over |= big > 4096.f || mv[e] == kNoMax;
+        over |= big > 4096.f || mx[e] - mv[e] > kLeast;  // the latter, too, while there is no reference
       }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -822,6 +823,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
           }
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+          v = fmaxf(v, mx[e] - kLeast);  // scales so small (subnormal ones are 0 to lg2) need no finer reference
           if (v > mv[e]) {
             const float f = ex2(mv[e] - v);
             mv[e] = v;
