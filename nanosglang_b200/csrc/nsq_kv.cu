@@ -250,12 +250,14 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 //     and for every bf16 within 2^-14 of the head's largest. Scores, maxima
 //     and sums are fp32;
 //   * the fp16 weights of p . v are p * vs relative to a reference m' of their
-//     own (log2 of their largest), so that they use fp16's range whatever the
-//     scales are (half-ulp 2^-12 each); the denominator is summed in fp32 from
-//     unrounded terms. At the end the accumulator is multiplied by
-//     exp2(m' - m). Both references follow lazily, when a score passes m by 8
-//     or a weight passes 2^12: rescaling and the maximum over the warp are
-//     rare, and fp16 and fp32 have the room;
+//     own, log2 of their largest less 12: the largest lies in [2^12, 2^15], so
+//     one down to 2^-26 of it keeps fp16's 11 bits (off by 2^-11 of itself at
+//     most) and smaller ones are off by 2^-37 of the largest. fp16 because the
+//     codes are exact in it and the MMA wants one type; it is what bounds the
+//     accuracy. The denominator is summed in fp32 from unrounded terms. At the
+//     end the accumulator is multiplied by exp2(m' - m). Both references follow
+//     lazily, when a score passes m by 8 or a weight passes 2^15: rescaling and
+//     the maximum over the warp are rare, and fp16 and fp32 have the room;
 //   * work is cut into units of 32 tokens of one item (sequence, kv head) and
 //     dealt evenly to the warps on the device, from seq_lens: long and ragged
 //     batches fill the machine alike. Warps are dealt to in teams of up to 32, a
@@ -291,6 +293,7 @@ __device__ __forceinline__ float lg2(float x) {
 constexpr float kNoMax = -3e38f;  // below every score: exp2(x - kNoMax) is 0 for a masked x, and nothing is NaN
 
 // 2^(m - mm): what turns exp2(x - m) * vs into a weight relative to mm (0 while there is none)
+constexpr float kLift = 12.f;    // log2 of the weight that sets a reference
 constexpr float kLeast = 126.f;  // mm is at least m - kLeast, so that the factor stays in fp32's range
 __device__ __forceinline__ float weight_factor(float m, float mm) { return mm == kNoMax ? 0.f : ex2(m - mm); }
 // acc / sum * 2^(mm - m): the output of a head whose weights of v were taken
@@ -810,7 +813,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
             big = fmaxf(big, wt[h][2 * r + e]);
           }
         }
-        over |= big > 4096.f || mx[e] - mv[e] > kLeast;  // the latter, too, while there is no reference
+        over |= big > 32768.f || mx[e] - mv[e] > kLeast;  // the latter, too, while there is no reference
       }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -823,7 +826,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
           }
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-          v = fmaxf(v, mx[e] - kLeast);  // scales so small (subnormal ones are 0 to lg2) need no finer reference
+          v = fmaxf(v - kLift, mx[e] - kLeast);  // scales so small (subnormal ones are 0 to lg2) need no finer reference
           if (v > mv[e]) {
             const float f = ex2(mv[e] - v);
             mv[e] = v;

@@ -82,3 +82,42 @@ def test_fp16_scales_and_queries(codes):
         out, lse = ops.kv_attention_decode(q, kc, vc, ks, vs, table, lens_t, softmax_scale=scale, return_lse=True)
         assert out.isfinite().all()
         check_attention(out, lse, q, (kc, vc, ks, vs), table, lens_t, scale)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("n,first", [(3000, True), (3000, False), (120, True)])
+@pytest.mark.parametrize("drop", [14, 18, 22])
+def test_small_weights_keep_their_bits(codes, n, first, drop):
+    """One token takes nearly all of the softmax, but its v is 0 in half of the
+    dims: there the output is the sum of weights ``drop`` powers of two smaller.
+
+    Each weight is off by 2^-11 of itself, and below 2^-26 of the largest by
+    2^-37 of that; the other terms as in test_gpu_kv.py."""
+    from nanosglang_b200 import ops
+    page, dim, pages = 16, 64, -(-n // 16)
+    g = torch.Generator().manual_seed(67)
+    vc = torch.randint(1, 128, (pages, page, 1, dim), generator=g, dtype=torch.int8)
+    at = 7 if first else n - 3
+    vc[at // page, at % page, 0, :32] = 0
+    if codes != torch.int8:
+        vc = vc.float().to(codes)
+    kc = torch.ones(pages, page, 1, dim).to(codes)
+    ks = torch.rand(pages, page, 1, generator=g) / dim
+    ks[at // page, at % page] = (drop + 1) / dim
+    vs = torch.full((pages, page, 1), 2.0 ** -7)
+    q = torch.ones(1, 2, dim).half()
+    ln2 = 0.6931471805599453
+    out = ops.kv_attention_decode(q.cuda(), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(),
+                                  torch.arange(pages, dtype=torch.int32)[None].cuda(),
+                                  torch.tensor([n], dtype=torch.int32).cuda(), softmax_scale=ln2)
+    score = (ks.double().view(-1)[:n] * dim) * ln2
+    p = torch.exp(score - score.max())
+    v = vc.half().double().view(-1, dim)[:n] * 2.0 ** -7
+    total = p.sum()
+    want = p @ v / total
+    size = score.max()
+    d = size * dim * 2.0 ** -23 + (size + 7 * ln2 + 16) * 8 * 2.0 ** -24
+    tol = want * (2.0 ** -11 + 2 * d + n * 2.0 ** -23) + n * 2.0 ** -37 * (p * v.amax(-1)).max() / total
+    tol = 1.05 * tol + 2.0 ** -11 * want + 2.0 ** -25
+    worst = ((out[0].cpu().double() - want).abs() / tol).max().item()
+    assert worst <= 1.0, f"worst error {worst} of the tolerance"
