@@ -246,9 +246,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 //     p . v; the query heads that share the kv head are the 8 columns. The
 //     codes are read in the swizzled tile without bank conflicts (ldmatrix for
 //     k, 16-byte reads for v) and become fp16 in registers, exactly;
-//   * q is scaled per head by a power of two into fp16's range, exact for fp16
-//     and for every bf16 within 2^-14 of the head's largest. Scores, maxima
-//     and sums are fp32;
+//   * q enters the MMA as fp16: fp16 as it is, bf16 scaled per head by a power
+//     of two that takes its largest near the end of fp16's range, exact for
+//     every element within 2^-31 of that. Scores, maxima and sums are fp32;
 //   * the fp16 weights of p . v are p * vs relative to a reference m' of their
 //     own, log2 of their largest less 12: the largest lies in [2^12, 2^15], so
 //     one down to 2^-26 of it keeps fp16's 11 bits (off by 2^-11 of itself at
@@ -693,7 +693,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
     const int hl = hb0 + g;
     const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + b * p.q_stride[0] +
                            (int64_t)(head * p.group + (hl < p.group ? hl : 0)) * p.q_stride[1];
-    float m = 0.f;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       const int d = 16 * j + 4 * t;
@@ -701,29 +700,39 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
       if (hl < p.group && d < p.c.head_dim) x = __ldg(reinterpret_cast<const uint2*>(qrow + d));
       qf[j][0] = x.x;
       qf[j][1] = x.y;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)qf[j][i])));
-        m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)(qf[j][i] >> 16))));
-      }
     }
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // the largest lands in [1, 2): e = its exponent, applied in two steps so
-    // that neither factor leaves fp32's range
-    const int e = m > 0.f && m <= 3.4e38f ? ilogbf(m) : 0;
-    const float f1 = exp2f((float)(-e / 2)), f2 = exp2f((float)(-e - (-e / 2)));
+    if constexpr (BF16) {
+      float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
+      for (int j = 0; j < MT; ++j) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        qf[j][i] = pack_f16(elem_to_float<BF16>((uint16_t)qf[j][i]) * f1 * f2,
-                            elem_to_float<BF16>((uint16_t)(qf[j][i] >> 16)) * f1 * f2);
+        for (int i = 0; i < 2; ++i) {
+          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)qf[j][i])));
+          m = fmaxf(m, fabsf(elem_to_float<BF16>((uint16_t)(qf[j][i] >> 16))));
+        }
       }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      // 2^-e takes the largest to [2^14, 2^15) (where it is below 2^-100 to [1, 2),
+      // so that the score's scale 2^e stays normal), in two steps so that
+      // neither factor leaves fp32's range
+      int e = m > 0.f && m <= 3.4e38f ? ilogbf(m) : 0;
+      if (e > -100) e -= 14;
+      const float f1 = exp2f((float)(-e / 2)), f2 = exp2f((float)(-e - (-e / 2)));
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          qf[j][i] = pack_f16(elem_to_float<BF16>((uint16_t)qf[j][i]) * f1 * f2,
+                              elem_to_float<BF16>((uint16_t)(qf[j][i] >> 16)) * f1 * f2);
+        }
+      }
+      const float s = p.scale_log2 / f1 / f2;
+      sc[0] = __shfl_sync(0xffffffffu, s, (2 * t) * 4);
+      sc[1] = __shfl_sync(0xffffffffu, s, (2 * t + 1) * 4);
+    } else {
+      sc[0] = sc[1] = p.scale_log2;
     }
-    const float s = p.scale_log2 / f1 / f2;
-    sc[0] = __shfl_sync(0xffffffffu, s, (2 * t) * 4);
-    sc[1] = __shfl_sync(0xffffffffu, s, (2 * t + 1) * 4);
 
     float o[MT][4];
     // references m and m' (kNoMax: no term yet), 2^(m - m'), denominators (this lane's tokens)

@@ -121,3 +121,26 @@ def test_small_weights_keep_their_bits(codes, n, first, drop):
     tol = 1.05 * tol + 2.0 ** -11 * want + 2.0 ** -25
     worst = ((out[0].cpu().double() - want).abs() / tol).max().item()
     assert worst <= 1.0, f"worst error {worst} of the tolerance"
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype,largest,rest", [(torch.float16, 6e4, 2.0 ** -10), (torch.float16, 6e4, 2.0 ** -20),
+                                                (torch.float16, 2.0 ** -20, 2.0 ** -21),
+                                                (torch.bfloat16, 2.0 ** 20, 2.0 ** -4),
+                                                (torch.bfloat16, 2.0 ** 100, 2.0 ** 72),
+                                                (torch.bfloat16, 2.0 ** -90, 2.0 ** -118)])
+def test_small_elements_of_q_count(codes, dtype, largest, rest):
+    """A head whose largest element meets zeros of k: its score is made of
+    elements many powers of two smaller, each of which has to be exact."""
+    from nanosglang_b200 import ops
+    lens, page, dim, pages = [300, 61], 16, 64, 30
+    kc, vc, ks, vs = make_pool(pages, page, 1, dim, codes, seed=68, spread=0.2)
+    kc.view(torch.uint8)[..., 5] = 0
+    table, lens_t = tables(lens, page, pages, seed=69)
+    g = torch.Generator().manual_seed(70)
+    q = ((1 + torch.rand(2, 4, dim, generator=g)) * rest * torch.randn(2, 4, dim, generator=g).sign()).to(dtype)
+    q[..., 5] = largest
+    scale = 0.25 / rest
+    out, lse = ops.kv_attention_decode(q.cuda(), kc, vc, ks, vs, table, lens_t, softmax_scale=scale, return_lse=True)
+    assert (lse[0] - lse[0].min() != 0).any()
+    check_attention(out, lse, q, (kc, vc, ks, vs), table, lens_t, scale)
