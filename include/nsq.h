@@ -359,7 +359,10 @@ int nsq_set_sm_reserve(int n);
 /* Opt in (1) or out (0, default) of programmatic dependent launch for the
  * linear kernels: with it on, a linear starts streaming its weights while the
  * previous kernel on the stream drains. Only valid when no kernel earlier on
- * the stream writes the weights being read. Returns the previous setting. */
+ * the stream writes the weights being read; nsq_int8_quantize may, its codes are
+ * complete before a kernel behind it starts. The row quantiser, the cache's
+ * write and read and decode attention are launched that way as well; they wait
+ * for the kernel ahead before they read anything. Returns the previous setting. */
 int nsq_set_pdl(int enable);
 
 #ifdef __cplusplus

@@ -627,7 +627,7 @@ int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* 
   if (!x || !codes || !scale) return NSQ_EINVAL;
   int rc = check_device();
   if (rc != NSQ_OK) return rc;
-  return launch_int8_quantize(x, x_dtype, M, K, codes, scale, static_cast<cudaStream_t>(stream)) == cudaSuccess
+  return launch_int8_quantize(x, x_dtype, M, K, codes, scale, static_cast<cudaStream_t>(stream), false) == cudaSuccess
              ? NSQ_OK
              : NSQ_ECUDA;
 }
@@ -696,7 +696,7 @@ int nsq_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t N,
   int8_t* codes = static_cast<int8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(codes + int8_codes_bytes(M, K));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (launch_int8_quantize(x, x_dtype, M, K, codes, scale, s) != cudaSuccess) return NSQ_ECUDA;
+  if (launch_int8_quantize(x, x_dtype, M, K, codes, scale, s, true) != cudaSuccess) return NSQ_ECUDA;
   return int8_product(Int8Args{codes, scale, (int)M, (int)K, (int)N, weight_int8, weight_scale, bias, bias_dtype,
                                x_dtype == NSQ_DTYPE_BF16, y, true, nullptr},
                       s);

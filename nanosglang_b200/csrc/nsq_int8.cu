@@ -27,6 +27,13 @@ constexpr int kQThreads = 256;
 // length, alignment and type, element by element, and reads the row twice (the
 // second time from L2).
 // ---------------------------------------------------------------------------
+// What of programmatic launch a quantiser takes part in: it waits for the kernel
+// ahead, and lets the one behind start at once. That one may be a product which
+// loads its weight before it waits, so only a quantiser launched for the
+// product's x does. One called by itself may be writing that weight: it releases
+// nothing, and its codes are visible to all before a block of it ends.
+constexpr int kPdlWait = 1, kPdlRelease = 2;
+
 __device__ __forceinline__ float load_elem(const void* p, int dtype, int64_t i) {
   if (dtype == NSQ_DTYPE_F32) return static_cast<const float*>(p)[i];
   const uint16_t u = static_cast<const uint16_t*>(p)[i];
@@ -49,8 +56,8 @@ template <int TPR, int NV, bool BF16>
 __global__ void __launch_bounds__(kQThreads) int8_quantize_kernel(const uint16_t* __restrict__ x, int M, int K,
                                                                   int8_t* __restrict__ codes,
                                                                   float* __restrict__ scale, int pdl) {
-  if (pdl) pdl_wait_prior_grids();
-  pdl_launch_dependents();
+  if (pdl & kPdlWait) pdl_wait_prior_grids();
+  if (pdl & kPdlRelease) pdl_launch_dependents();
   __shared__ uint32_t red[kQThreads / 32];
   const int lane = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * (kQThreads / TPR) + threadIdx.x / TPR;
@@ -75,7 +82,7 @@ __global__ void __launch_bounds__(kQThreads) int8_quantize_kernel(const uint16_t
 #pragma unroll
     for (int i = 0; i < TPR / 32; ++i) m = __vmaxu2(m, red[w0 + i]);
   }
-  if (!in) return;
+  if (!in) return;  // (the last block's rest: nothing to write)
   const float s = row_scale<false>(abs_max_value<BF16>(m));
   if (lane == 0) scale[row] = s;
   const RowDiv dv(s);
@@ -84,13 +91,14 @@ __global__ void __launch_bounds__(kQThreads) int8_quantize_kernel(const uint16_t
     const int i = j * TPR + lane;
     if (i < nvec) reinterpret_cast<uint2*>(codes + row * K)[i] = row_codes8<false, BF16>(dv, v[j]);
   }
+  if (pdl == kPdlWait) __threadfence();
 }
 
 __global__ void __launch_bounds__(kQThreads) int8_quantize_any_kernel(const void* __restrict__ x, int dtype, int64_t K,
                                                                       int8_t* __restrict__ codes,
                                                                       float* __restrict__ scale, int pdl) {
-  if (pdl) pdl_wait_prior_grids();
-  pdl_launch_dependents();
+  if (pdl & kPdlWait) pdl_wait_prior_grids();
+  if (pdl & kPdlRelease) pdl_launch_dependents();
   const int64_t row = blockIdx.x;
   float m = 0.f;
   for (int64_t i = threadIdx.x; i < K; i += kQThreads) m = nan_max(m, fabsf(load_elem(x, dtype, row * K + i)));
@@ -100,6 +108,7 @@ __global__ void __launch_bounds__(kQThreads) int8_quantize_any_kernel(const void
   for (int64_t i = threadIdx.x; i < K; i += kQThreads) {
     codes[row * K + i] = (int8_t)row_code<false>(dv(load_elem(x, dtype, row * K + i)));
   }
+  if (pdl == kPdlWait) __threadfence();
 }
 
 // ---------------------------------------------------------------------------
@@ -304,11 +313,11 @@ cudaError_t launch(F kern, dim3 grid, int threads, int smem, int cluster, cudaSt
 
 template <int TPR, bool BF16>
 static cudaError_t quantize_rows(const uint16_t* x, int M, int K, int8_t* codes, float* scale, cudaStream_t stream,
-                                 bool pdl) {
+                                 int pdl) {
   const dim3 grid((unsigned)((M + kQThreads / TPR - 1) / (kQThreads / TPR)));
   const int per = (K / 8 + TPR - 1) / TPR;
   auto go = [&](auto kern) {
-    return launch(kern, grid, kQThreads, 0, 1, stream, pdl, x, M, K, codes, scale, (int)pdl);
+    return launch(kern, grid, kQThreads, 0, 1, stream, (pdl & kPdlWait) != 0, x, M, K, codes, scale, pdl);
   };
   if constexpr (TPR == 256) {
     if (per > 8) return go(int8_quantize_kernel<TPR, 16, BF16>);
@@ -320,13 +329,13 @@ static cudaError_t quantize_rows(const uint16_t* x, int M, int K, int8_t* codes,
 }
 
 cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K, int8_t* codes, float* scale,
-                                 cudaStream_t stream) {
-  const bool pdl = pdl_enabled();
+                                 cudaStream_t stream, bool before_product) {
+  const int pdl = (pdl_enabled() ? kPdlWait : 0) | (before_product ? kPdlRelease : 0);
   const bool vec = dtype != NSQ_DTYPE_F32 && K % 8 == 0 && K <= 16 * 8 * kQThreads &&
                    ((reinterpret_cast<uintptr_t>(x) & 15) | (reinterpret_cast<uintptr_t>(codes) & 7)) == 0;
   if (!vec) {
-    return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 0, 1, stream, pdl, x, dtype, K, codes,
-                  scale, (int)pdl);
+    return launch(int8_quantize_any_kernel, dim3((unsigned)rows), kQThreads, 0, 1, stream, (pdl & kPdlWait) != 0, x,
+                  dtype, K, codes, scale, pdl);
   }
   const uint16_t* x16 = static_cast<const uint16_t*>(x);
   auto go = [&](auto tpr) {

@@ -50,8 +50,9 @@ cudaError_t launch_fp8_quantize(const void* w, int dtype, int64_t total, uint8_t
                                 float* scale, void* workspace, cudaStream_t stream);
 
 // int8 linear: rows quantised to int8 with one scale each, then the product.
+// before_product: the next launch on the stream is run_int8_rows or run_int8_gemm with after_quantize.
 cudaError_t launch_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K, int8_t* codes, float* scale,
-                                 cudaStream_t stream);
+                                 cudaStream_t stream, bool before_product);
 struct Int8Args {
   const int8_t* x;      // codes [M, K]
   const float* xscale;  // [M]
