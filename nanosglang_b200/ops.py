@@ -50,6 +50,17 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _weight(t: torch.Tensor) -> torch.Tensor:
+    """A weight contiguous and 16-byte aligned, as the linears take it. With
+    programmatic launch on they read weights before they wait for the kernel
+    right ahead, which must not be the copy made here: another launch, which
+    starts when the copy is complete, lies between."""
+    c = _aligned(t)
+    if c.data_ptr() != t.data_ptr():
+        torch.zeros(1, device=t.device)
+    return c
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -120,11 +131,11 @@ def awq_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
     if x.shape[-1] != k:
         raise RuntimeError(f"x has {x.shape[-1]} features, the layer expects {k}")
     if not qweight.is_contiguous() or qweight.data_ptr() & 15:
-        qweight = _aligned(qweight)
+        qweight = _weight(qweight)
     if not scales.is_contiguous():
-        scales = scales.contiguous()
+        scales = _weight(scales)
     if not zeros.is_contiguous():
-        zeros = zeros.contiguous()
+        zeros = _weight(zeros)
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     if not x2.is_contiguous() or x2.data_ptr() & 15:
         x2 = _aligned(x2)
@@ -230,7 +241,7 @@ def fp8_linear(x: torch.Tensor, weight_fp8: torch.Tensor, weight_scale: torch.Te
         raise TypeError(f"fp8 weight must be float8_e4m3fn, got {weight_fp8.dtype}")
     w = weight_fp8
     if not w.is_contiguous() or w.data_ptr() & 15:
-        w = _aligned(w)
+        w = _weight(w)
     n, k = w.shape
     if x.shape[-1] != k:
         raise RuntimeError(f"x has {x.shape[-1]} features, the layer expects {k}")
@@ -358,7 +369,7 @@ def _int8_operands(weight_int8: torch.Tensor, weight_scale: torch.Tensor, bias: 
         raise TypeError(f"weight_scale must be float32 with one value per output channel ({n}), "
                         f"got {weight_scale.dtype} {tuple(weight_scale.shape)}")
     if not weight_int8.is_contiguous() or weight_int8.data_ptr() & 15:
-        weight_int8 = _aligned(weight_int8)
+        weight_int8 = _weight(weight_int8)
     if not weight_scale.is_contiguous():
         weight_scale = weight_scale.contiguous()
     if bias is None:
@@ -632,15 +643,15 @@ def linear_multi(x: torch.Tensor, mods) -> Optional[list]:
         gs = {mm.group_size for mm in mods}
         if len(gs) != 1 or any(mm.in_features != k for mm in mods):
             return None
-        qws = [_aligned(mm.qweight) for mm in mods]
-        scs = [mm.scales.contiguous() for mm in mods]
-        zrs = [mm.zeros.contiguous() for mm in mods]
+        qws = [_weight(mm.qweight) for mm in mods]
+        scs = [_weight(mm.scales) for mm in mods]
+        zrs = [_weight(mm.zeros) for mm in mods]
         rc = lib.nsq_awq_linear_multi(_ptr(x2), _ACT_CODES[x.dtype], m, k, len(mods),
                                       _ptr_array([t.data_ptr() for t in qws]), _ptr_array([t.data_ptr() for t in scs]),
                                       _ptr_array([t.data_ptr() for t in zrs]), n_arr, gs.pop(), b_arr, bcode, _ptr(y),
                                       y.shape[1], _stream(x))
     elif kinds == {"FP8Linear"}:
-        ws = [_aligned(_u8(mm.weight_fp8)) for mm in mods]
+        ws = [_weight(_u8(mm.weight_fp8)) for mm in mods]
         if any(w.shape[1] != k for w in ws):
             return None
         scs = [_scale_arg(mm.weight_scale) for mm in mods]
@@ -682,12 +693,11 @@ def gate_up_silu(x: torch.Tensor, gate, up) -> Optional[torch.Tensor]:
     if type(gate).__name__ == "AWQLinear":
         if gate.group_size != up.group_size or gate.in_features != k or up.in_features != k:
             return None
-        rc = lib.nsq_awq_gate_up_silu(_ptr(x2), _ACT_CODES[x.dtype], m, k, n, _ptr(_aligned(gate.qweight)),
-                                      _ptr(gate.scales.contiguous()), _ptr(gate.zeros.contiguous()),
-                                      _ptr(_aligned(up.qweight)), _ptr(up.scales.contiguous()),
-                                      _ptr(up.zeros.contiguous()), gate.group_size, _ptr(y), _stream(x))
+        qg, sg, zg, qu, su, zu = (_weight(t) for mod in (gate, up) for t in (mod.qweight, mod.scales, mod.zeros))
+        rc = lib.nsq_awq_gate_up_silu(_ptr(x2), _ACT_CODES[x.dtype], m, k, n, _ptr(qg), _ptr(sg), _ptr(zg), _ptr(qu),
+                                      _ptr(su), _ptr(zu), gate.group_size, _ptr(y), _stream(x))
     elif type(gate).__name__ == "FP8Linear":
-        wg, wu = _aligned(_u8(gate.weight_fp8)), _aligned(_u8(up.weight_fp8))
+        wg, wu = _weight(_u8(gate.weight_fp8)), _weight(_u8(up.weight_fp8))
         if wg.shape[1] != k or wu.shape[1] != k:
             return None
         rc = lib.nsq_fp8_gate_up_silu(_ptr(x2), _ACT_CODES[x.dtype], m, k, n, _ptr(wg), _ptr(_scale_arg(gate.weight_scale)),

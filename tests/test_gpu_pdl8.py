@@ -111,3 +111,60 @@ def test_weight_quantised_just_ahead(m, k, n, dtype, quantized, pdl):
 
     want = runs()
     assert torch.equal(pdl(runs), want)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 512, 512), (5, 1024, 512), (100, 512, 1000)])
+def test_weight_view_copied_in_the_call(m, k, n, pdl):
+    """A weight that is not contiguous is copied within the call, right ahead of
+    the kernel that reads the copy."""
+    from nanosglang_b200 import ops
+    g = torch.Generator().manual_seed(6)
+    weights = [torch.randint(-127, 128, (k, n), generator=g, dtype=torch.int8).cuda() for _ in range(3)]
+    scale = torch.rand(n, generator=g).cuda()
+    x = torch.randn(m, k, generator=g).bfloat16().cuda()
+
+    def runs():
+        w = weights[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.int8_linear(x, w.t(), scale)
+        out = []
+        for i in range(12):
+            w.copy_(weights[i % 3])
+            graph.replay()
+            out.append(y.clone())
+        torch.cuda.synchronize()
+        return torch.stack(out)
+
+    want = runs()
+    assert torch.equal(pdl(runs), want)
+
+
+def test_a_weight_copy_is_not_right_ahead():
+    """What the call launches last before a kernel that may load the weight
+    early is not the copy of that weight."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from nanosglang_b200 import ops
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func._schema.name.split("::")[1])
+            return func(*args, **(kwargs or {}))
+
+    g = torch.Generator().manual_seed(7)
+    w = torch.randint(-127, 128, (512, 64), generator=g, dtype=torch.int8).cuda().t()
+    f8 = torch.randn(512, 64, generator=g).cuda().to(torch.float8_e4m3fn).view(torch.uint8).t()
+    qw = torch.randint(-9, 9, (64, 64), generator=g, dtype=torch.int32).cuda().t()
+    sz = [torch.rand(4, 64, generator=g).half().cuda().t() for _ in range(2)]
+    x = torch.randn(2, 512, generator=g).half().cuda()
+    codes, scale = ops.int8_quantize(x)
+    ones = torch.ones(64, device="cuda")
+    for call in (lambda: ops.int8_linear(x, w, ones), lambda: ops.int8_linear_quantized(codes, scale, w, ones),
+                 lambda: ops.fp8_linear(x, f8, ones[:1]), lambda: ops.awq_linear(x, qw, *sz, 128)):
+        seen.clear()
+        with Log():
+            call()
+        copies = [i for i, name in enumerate(seen) if name in ("clone", "copy_", "contiguous", "_to_copy")]
+        assert copies and any(name in ("zeros", "zero_", "fill_") for name in seen[copies[-1] + 1:]), seen
