@@ -50,15 +50,19 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _weight(t: torch.Tensor) -> torch.Tensor:
-    """A weight contiguous and 16-byte aligned, as the linears take it. With
-    programmatic launch on they read weights before they wait for the kernel
-    right ahead, which must not be the copy made here: another launch, which
-    starts when the copy is complete, lies between."""
-    c = _aligned(t)
+def _settled(c: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
+    """c, which is t or a copy of it just made. With programmatic launch on, the
+    linears read weights, scales and biases before they wait for the kernel
+    right ahead, which must not be that copy: another launch, which starts when
+    the copy is complete, lies between."""
     if c.data_ptr() != t.data_ptr():
         torch.zeros(1, device=t.device)
     return c
+
+
+def _weight(t: torch.Tensor) -> torch.Tensor:
+    """A weight contiguous and 16-byte aligned, as the linears take it."""
+    return _settled(_aligned(t), t)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -70,7 +74,8 @@ def _bias_arg(bias: Optional[torch.Tensor]):
         return None, _lib.DTYPE_NONE
     if bias.dtype not in _BIAS_CODES:
         raise TypeError(f"bias dtype {bias.dtype} not supported")
-    bias = bias.contiguous()
+    if not bias.is_contiguous():
+        bias = _settled(bias.contiguous(), bias)
     return bias, _BIAS_CODES[bias.dtype]
 
 
@@ -218,9 +223,7 @@ def _u8(w: torch.Tensor) -> torch.Tensor:
 def _scale_arg(weight_scale: torch.Tensor) -> torch.Tensor:
     if weight_scale.numel() != 1:
         raise RuntimeError("weight_scale must hold exactly one value (per-tensor scale)")
-    if weight_scale.dtype != torch.float32:
-        weight_scale = weight_scale.float()
-    return weight_scale.contiguous()
+    return _settled(weight_scale.float().contiguous(), weight_scale)
 
 
 _FP8_TYPES = (torch.float8_e4m3fn, torch.uint8)

@@ -160,9 +160,11 @@ def test_a_weight_copy_is_not_right_ahead():
     sz = [torch.rand(4, 64, generator=g).half().cuda().t() for _ in range(2)]
     x = torch.randn(2, 512, generator=g).half().cuda()
     codes, scale = ops.int8_quantize(x)
-    ones = torch.ones(64, device="cuda")
+    ones, wide, plain = torch.ones(64, device="cuda"), torch.ones(64, 2, device="cuda"), f8.contiguous()
     for call in (lambda: ops.int8_linear(x, w, ones), lambda: ops.int8_linear_quantized(codes, scale, w, ones),
-                 lambda: ops.fp8_linear(x, f8, ones[:1]), lambda: ops.awq_linear(x, qw, *sz, 128)):
+                 lambda: ops.fp8_linear(x, f8, ones[:1]), lambda: ops.awq_linear(x, qw, *sz, 128),
+                 lambda: ops.fp8_linear(x, plain, ones[:1].half()),
+                 lambda: ops.fp8_linear(x, plain, ones[:1], wide[:, 0])):
         seen.clear()
         with Log():
             call()
