@@ -70,6 +70,9 @@ class DecodeEngine:
         self.history = torch.zeros(max_steps + 1, max_slots, dtype=torch.long, device=dev)
         self.step = torch.zeros(1, dtype=torch.long, device=dev)
         self.cols = torch.arange(max_len, device=dev)
+        # what prefill and decode_steps have made of positions and step, for their checks on the host
+        self.held = [0] * max_slots
+        self.rows = 0
         self.graphs = {}
         self.buckets = [b for b in BUCKETS if b <= max_slots]
         if not self.buckets or self.buckets[-1] < max_slots:
@@ -120,9 +123,12 @@ class DecodeEngine:
     # -- prefill --------------------------------------------------------------
     @torch.no_grad()
     def prefill(self, prompts: List[torch.Tensor]):
-        """Packed prefill of prompts (device tensors) into slots 0..n-1."""
+        """Packed prefill of prompts (device tensors) into slots 0..n-1; the others start empty."""
         model = self.model
         lens = [int(p.shape[0]) for p in prompts]
+        if len(lens) > self.max_slots or max(lens) > self.max_len:
+            raise ValueError(f"{len(lens)} prompts of up to {max(lens)} tokens exceed {self.max_slots} slots of "
+                             f"{self.max_len}")
         tokens = torch.cat(prompts)
         positions = torch.cat([torch.arange(n, device=self.device) for n in lens])
         h = model.embed_tokens(tokens)
@@ -160,13 +166,31 @@ class DecodeEngine:
         n = len(prompts)
         first = logits.argmax(dim=-1)
         self.tokens[:n].copy_(first)
-        self.positions[:n].copy_(torch.tensor(lens, device=self.device))
+        self.held = lens + [0] * (self.max_slots - n)
+        self.positions.copy_(torch.tensor(self.held, device=self.device))
         self.history[0, :n].copy_(first)
         self.step.fill_(1)
+        self.rows = 1
 
     def decode_steps(self, active_counts: Sequence[int]):
-        for n in active_counts:
-            self.graphs[self.bucket(n)].replay()
+        """One step for each count of active requests (slots 0..count-1; the
+        bucket's other slots step along). Refuses steps that would leave a slot
+        of the cache or the history, whose places follow from prefill and the
+        steps since."""
+        buckets = [self.bucket(n) for n in active_counts]
+        if self.rows + len(buckets) > self.max_steps + 1:
+            raise ValueError(f"{len(buckets)} steps exceed the engine's max_steps of {self.max_steps}")
+        held, lo = list(self.held), 0
+        for hi in sorted(set(buckets)):  # slots lo..hi-1 take every step of a bucket of hi or more
+            steps = sum(b >= hi for b in buckets)
+            held[lo:hi] = [h + steps for h in held[lo:hi]]
+            if max(held[lo:hi]) > self.max_len:
+                raise ValueError(f"{len(buckets)} steps take a slot past the engine's max_len of {self.max_len}")
+            lo = hi
+        self.held = held
+        self.rows += len(buckets)
+        for b in buckets:
+            self.graphs[b].replay()
 
 
 def make_workload(num_requests: int, prompt_min: int, prompt_max: int, out_min: int, out_max: int, vocab: int,
