@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const KvWrite p) {
   const bool in_row[2] = {sub * 8 < p.c.head_dim, (LPR + sub) * 8 < p.c.head_dim};
   const uint32_t step = gridDim.x * (256 / LPR);
   // whole warps stay in the loop: the shuffles below are all lanes'
-  for (uint32_t r0 = (blockIdx.x * 256 + (threadIdx.x & ~31u)) / LPR; r0 < rows; r0 += kAtOnce * step) {
+  for (uint32_t r0 = blockIdx.x * (256 / LPR) + (threadIdx.x & ~31u) / LPR; r0 < rows; r0 += kAtOnce * step) {
     KvPlace a[kAtOnce];
     uint4 x[kAtOnce][2][2];  // [place][k, v][8 elements]
 #pragma unroll
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
   if (!in_row[0]) return;
   const uint32_t rows = (uint32_t)p.T * (uint32_t)p.c.kv_heads;
   const uint32_t step = gridDim.x * (256 / LPR);
-  for (uint32_t r0 = (blockIdx.x * 256 + threadIdx.x) / LPR; r0 < rows; r0 += kAtOnce * step) {
+  for (uint32_t r0 = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; r0 < rows; r0 += kAtOnce * step) {
     KvPlace a[kAtOnce];
     uint2 c[kAtOnce][2][2];  // [place][k, v][8 codes]
     float s[kAtOnce][2];

@@ -37,3 +37,18 @@ def test_attention_over_an_expanded_pool(shared, page, dim, codes):
     slots = torch.arange(pages * page).cuda()
     for a, b in zip(ops.kv_cache_read(*view, slots, torch.half), ops.kv_cache_read(*full, slots, torch.half)):
         assert torch.equal(a, b)
+
+
+def test_write_of_half_a_thousand_million_rows():
+    """More threads (16 lanes for two rows) than 32 bits count: the last tokens
+    are written, and nothing but they (one row of k and v, expanded)."""
+    from nanosglang_b200 import ops
+    n, dim = 2 ** 29 + 1000, 256
+    pool = make_pool(2, 16, 1, dim, torch.int8, seed=34)
+    want = [t.clone() for t in pool]
+    row = torch.randn(1, 1, dim, generator=torch.Generator().manual_seed(35)).bfloat16().cuda()
+    slots = torch.full((n,), -1, device="cuda")
+    slots[-3:] = torch.tensor([4, 31, 9])
+    ops.kv_cache_write(row.expand(n, 1, dim), row.expand(n, 1, dim), *pool, slots)
+    ops.kv_cache_write(row.expand(3, 1, dim), row.expand(3, 1, dim), *want, slots[-3:].clone())
+    assert all(torch.equal(a, b) for a, b in zip(pool, want))
