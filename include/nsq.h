@@ -221,7 +221,8 @@ int nsq_fp8_quantize_noalloc(const void* w, int w_dtype, int64_t N, int64_t K, u
  * nsq_int8_linear_quantized: the product alone, of codes the caller keeps
  * (quantised once, used by several layers); y_dtype is F16 or BF16.
  *
- * Requires K % 16 == 0, K <= 131072 (int32 sums), codes, weight, x and y
+ * Requires K % 16 == 0, K <= 131072 (int32 sums), M and N at most 2^31 - 1024
+ * (M of nsq_int8_quantize, too), codes, weight, x and y
  * 16-byte aligned.
  */
 int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* codes, float* scale, void* stream);

@@ -620,9 +620,13 @@ int nsq_fp8_quantize(const void* w, int w_dtype, int64_t N, int64_t K, uint8_t* 
   return e == cudaSuccess ? NSQ_OK : NSQ_ECUDA;
 }
 
+// tokens and weight rows: the kernels round them up to whole tiles in 32 bits
+constexpr int64_t kInt8MaxRows = kIntMax - 1023;
+
 int nsq_int8_quantize(const void* x, int x_dtype, int64_t M, int64_t K, int8_t* codes, float* scale, void* stream) {
   if (M < 0 || K <= 0 || M > kIntMax || K > kIntMax) return NSQ_EINVAL;
   if (!(valid_act_dtype(x_dtype) || x_dtype == NSQ_DTYPE_F32)) return NSQ_EINVAL;
+  if (M > kInt8MaxRows) return NSQ_ENOTSUP;
   if (M == 0) return NSQ_OK;
   if (!x || !codes || !scale) return NSQ_EINVAL;
   int rc = check_device();
@@ -656,7 +660,7 @@ static int int8_check(int64_t M, int64_t K, int64_t N, const void* x, const int8
   if (M < 0 || K <= 0 || N <= 0 || M > kIntMax || K > kIntMax || N > kIntMax) return NSQ_EINVAL;
   if (!valid_act_dtype(y_dtype) || !valid_bias_dtype(bias_dtype)) return NSQ_EINVAL;
   if ((bias_dtype == NSQ_DTYPE_NONE) != (bias == nullptr)) return NSQ_EINVAL;
-  if (K % 16 != 0 || K > kInt8MaxK) return NSQ_ENOTSUP;
+  if (K % 16 != 0 || K > kInt8MaxK || M > kInt8MaxRows || N > kInt8MaxRows) return NSQ_ENOTSUP;
   if (M == 0) return NSQ_OK;
   if (!x || !w || !ws || !y) return NSQ_EINVAL;
   if (!aligned16(x) || !aligned16(y) || !aligned16(w)) return NSQ_EALIGN;

@@ -1,4 +1,4 @@
-"""Host-side checks of the 8-bit cache that need no GPU."""
+"""Host-side checks of the 8-bit operators that need no GPU."""
 
 import pytest
 
@@ -19,3 +19,12 @@ def test_write_refuses_places_that_share_memory(what, dim):
     assert write(_desc(**{what: tuple(strides)})) == _lib.EINVAL
     one = {("num_pages", "page_size", "kv_heads")[dim]: 1}
     assert write(_desc(**{what: tuple(strides)}, **one)) == _lib.OK
+
+
+@pytest.mark.parametrize("much", [2 ** 31 - 1, 2 ** 31 - 1023])
+def test_int8_refuses_rows_that_tiles_would_take_past_32_bits(much):
+    lib = _lib.load()
+    linear = lambda m, n: lib.nsq_int8_linear(FAKE, 1, m, 16, n, FAKE, FAKE, None, -1, FAKE, FAKE, 1 << 40, None)  # noqa: E731
+    assert linear(1, much) == linear(much, 1) == _lib.ENOTSUP
+    assert lib.nsq_int8_linear_quantized(FAKE, FAKE, 1, 16, much, FAKE, FAKE, None, -1, FAKE, 1, None) == _lib.ENOTSUP
+    assert lib.nsq_int8_quantize(FAKE, 1, much, 8, FAKE, FAKE, None) == _lib.ENOTSUP
