@@ -79,7 +79,7 @@ struct GemmParams {
   const void* bias;
   void* y;
   DevStatus* status;
-  int M, K, N, bias_dtype;
+  int M, N, bias_dtype;
   int num_w, num_t, num_kb, num_st;
   int wrows;  // weight rows of a CTA's tile
   int split;  // SPLIT: CTAs of a cluster that share a tile, along K
@@ -528,8 +528,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
 }
 
 template <int CG, int TOK, bool BF16, bool STAGED, bool SPLIT = false>
-cudaError_t launch_gemm(const Int8Args& a, const CUtensorMap& xmap, const CUtensorMap& wmap, const CUtensorMap& ymap,
-                        const GemmParams& p, cudaStream_t stream) {
+cudaError_t launch_gemm(const CUtensorMap& xmap, const CUtensorMap& wmap, const CUtensorMap& ymap, const GemmParams& p,
+                        cudaStream_t stream) {
   using S = GemmShape<CG, TOK>;
   auto kern = int8_gemm_kernel<CG, TOK, BF16, STAGED, SPLIT>;
   cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kern), S::kAlloc);
@@ -584,7 +584,6 @@ int run_gemm(const Int8Args& a, int wrows, int split, cudaStream_t stream) {
   p.y = a.y;
   p.status = device_status_ptr();
   p.M = a.M;
-  p.K = a.K;
   p.N = a.N;
   p.wrows = wrows;
   p.tma_y = tma_y;
@@ -595,18 +594,18 @@ int run_gemm(const Int8Args& a, int wrows, int split, cudaStream_t stream) {
   p.num_st = (p.num_kb + kKps - 1) / kKps;
   p.pdl_x = a.after_quantize || pdl_enabled();
   if ((int64_t)p.num_w * p.num_t > 0x3FFFFFFF) return NSQ_ENOTSUP;
-  cudaError_t e = cudaSuccess;
+  cudaError_t e = cudaErrorInvalidValue;  // (pairs have no split form)
   if (split > 1) {
     if constexpr (CG == 1) {
-      e = a.y_bf16 ? launch_gemm<1, TOK, true, false, true>(a, xmap, wmap, ymap, p, stream)
-                   : launch_gemm<1, TOK, false, false, true>(a, xmap, wmap, ymap, p, stream);
+      e = a.y_bf16 ? launch_gemm<1, TOK, true, false, true>(xmap, wmap, ymap, p, stream)
+                   : launch_gemm<1, TOK, false, false, true>(xmap, wmap, ymap, p, stream);
     }
   } else if (staged) {
-    e = a.y_bf16 ? launch_gemm<CG, TOK, true, true>(a, xmap, wmap, ymap, p, stream)
-                 : launch_gemm<CG, TOK, false, true>(a, xmap, wmap, ymap, p, stream);
+    e = a.y_bf16 ? launch_gemm<CG, TOK, true, true>(xmap, wmap, ymap, p, stream)
+                 : launch_gemm<CG, TOK, false, true>(xmap, wmap, ymap, p, stream);
   } else {
-    e = a.y_bf16 ? launch_gemm<CG, TOK, true, false>(a, xmap, wmap, ymap, p, stream)
-                 : launch_gemm<CG, TOK, false, false>(a, xmap, wmap, ymap, p, stream);
+    e = a.y_bf16 ? launch_gemm<CG, TOK, true, false>(xmap, wmap, ymap, p, stream)
+                 : launch_gemm<CG, TOK, false, false>(xmap, wmap, ymap, p, stream);
   }
   return e == cudaSuccess ? NSQ_OK : NSQ_ECUDA;
 }

@@ -671,13 +671,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnShape<DP>::kPerSm) kv_att
   };
 
   // places in a tile: ldmatrix rows of k, and this lane's chunk of the four tokens of v
-      const int krow = row_token<RB>(lane & 15);
-      uint32_t v_at[4];
-  #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = row_token<RB>(2 * t + (i & 1) + 8 * (i >> 1));
-        v_at[i] = RB == 128 ? tile_at<RB>(r, g) : tile_at<RB>(r, g >> 1) + 8 * (g & 1);
-      }
+  const int krow = row_token<RB>(lane & 15);
+  uint32_t v_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row_token<RB>(2 * t + (i & 1) + 8 * (i >> 1));
+    v_at[i] = RB == 128 ? tile_at<RB>(r, g) : tile_at<RB>(r, g >> 1) + 8 * (g & 1);
+  }
 
   uint32_t filled = 0, done = 0;  // stages
   for (; filled < S::kStages && more; ++filled) fill(filled % S::kStages);
