@@ -321,8 +321,10 @@ int nsq_set_wait_limit_ns(uint64_t ns);
  * records NSQ_EDEVICE_TIMEOUT (tag 1) in the status word, lets every copy it
  * did request land, and returns. Its output is then undefined. Likewise the
  * first stage of decode attention's first worker never completes (tag 204): the
- * rows of that worker's share are then undefined, the others are right. No
- * counterpart in the reference. Not for production use. */
+ * rows of that worker's share are then undefined, the others are right), nor
+ * that of the int8 linear's tensor-core kernel's first CTA (tags 210 to 215, by
+ * the wait that gives up first; y is undefined). No counterpart in the
+ * reference. Not for production use. */
 int nsq_test_withhold_weight_load(int enable);
 
 /*

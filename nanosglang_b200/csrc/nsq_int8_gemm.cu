@@ -85,6 +85,7 @@ struct GemmParams {
   int split;  // SPLIT: CTAs of a cluster that share a tile, along K
   int tma_y;  // STAGED: the tile is whole blocks of 64 features, stored by TMA; else by the threads
   int pdl_x;  // x and its scales come from the kernel ahead on the stream
+  int withhold;  // failure-path test hook: the first CTA's first stage never completes
 };
 
 __device__ __forceinline__ void gemm_unit(const GemmParams& p, int u, int& wt, int& tt) {
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < S::NS; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], 1 + (p.withhold && i == 0 && blockIdx.x == 0));
       mbar_init(&done[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -593,6 +594,7 @@ int run_gemm(const Int8Args& a, int wrows, int split, cudaStream_t stream) {
   p.num_kb = (a.K + kBK - 1) / kBK;
   p.num_st = (p.num_kb + kKps - 1) / kKps;
   p.pdl_x = a.after_quantize || pdl_enabled();
+  p.withhold = test_withhold();
   if ((int64_t)p.num_w * p.num_t > 0x3FFFFFFF) return NSQ_ENOTSUP;
   cudaError_t e = cudaErrorInvalidValue;  // (pairs have no split form)
   if (split > 1) {

@@ -74,3 +74,17 @@ def test_attention_wait_runs_out(withheld, lens, heads, dim, page, word):
     assert (code, where) == (_lib.EDEVICE_TIMEOUT, ATTENTION_WAIT_TAG)
     assert torch.equal(got[0][-1], want[-1])  # far from the first worker's share
     assert torch.equal(call(), want) and _lib.device_status()[0] == 0
+
+
+# a tile of one CTA, of a pair, and one whose K is split over a cluster; with and without a staged y
+@pytest.mark.parametrize("m,k,n", [(300, 2048, 1024), (300, 2048, 1001), (1000, 2064, 2600), (200, 12304, 520)])
+def test_int8_gemm_wait_runs_out(withheld, m, k, n):
+    from nanosglang_b200 import _lib, ops
+    g = torch.Generator().manual_seed(44)
+    x = torch.randn(m, k, generator=g).bfloat16().cuda()
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8).cuda()
+    ws = torch.rand(n, generator=g).cuda()
+    want = ops.int8_linear(x, w, ws)
+    code, where, _ = withheld(lambda: ops.int8_linear(x, w, ws))
+    assert code == _lib.EDEVICE_TIMEOUT and 210 <= where <= 215
+    assert torch.equal(ops.int8_linear(x, w, ws), want) and _lib.device_status()[0] == 0
