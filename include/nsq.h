@@ -353,7 +353,7 @@ int nsq_ipc_close(void* dev_ptr);
 int nsq_peer_allreduce(void* const* workspaces, int rank, int world, int64_t max_bytes, const void* in, void* out,
                        int64_t n, int dtype, void* stream);
 
-/* Number of SMs the linear kernels leave free when they size their grids
+/* Number of SMs the kernels leave free when they size their grids
  * (default 0; at most half the SMs), so that a collective launched on
  * another stream can run beside them. Returns the previous setting. No
  * counterpart in the reference (its all-reduce is serial). */

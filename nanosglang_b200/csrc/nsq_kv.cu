@@ -270,10 +270,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRead p) {
 //     launch does.
 // Measured (8 kv heads of 128, 4 query heads each, e4m3, bf16 q, the join
 // included): 48 x 8192 tokens 146 us, 5.7 TB/s; 64 x 2048 58 us, 4.7 TB/s;
-// 1 x 131001 60 us; 1 x 2048 10.5 us; 1 x 40 (2 kv heads of 64, int8) 7.0 us. Of
-// the 58 us 2 pass before the first copy is issued, 43 are the stream at the
-// rate of a plain copy, about 7 the last warps of an even deal (their rates
-// differ by 10%) and 4 the join with its launch.
+// 1 x 131001 60 us; 1 x 2048 10.5 us; 1 x 40 (2 kv heads of 64, int8, fp16 q)
+// 6.6 us. Of the 58 us 2 pass before the first copy is issued, 43 are the
+// stream at the rate of a plain copy, about 7 the last warps of an even deal
+// (their rates differ by 10%) and 4 the join with its launch.
 
 constexpr int kAttnWarps = 4;
 constexpr int kTile = 32;  // tokens of a stage
@@ -292,9 +292,9 @@ __device__ __forceinline__ float lg2(float x) {
 }
 constexpr float kNoMax = -3e38f;  // below every score: exp2(x - kNoMax) is 0 for a masked x, and nothing is NaN
 
-// 2^(m - mm): what turns exp2(x - m) * vs into a weight relative to mm (0 while there is none)
 constexpr float kLift = 12.f;    // log2 of the weight that sets a reference
-constexpr float kLeast = 126.f;  // mm is at least m - kLeast, so that the factor stays in fp32's range
+constexpr float kLeast = 126.f;  // mm is at least m - kLeast, so that weight_factor stays in fp32's range
+// 2^(m - mm): what turns exp2(x - m) * vs into a weight relative to mm (0 while there is none)
 __device__ __forceinline__ float weight_factor(float m, float mm) { return mm == kNoMax ? 0.f : ex2(m - mm); }
 // acc / sum * 2^(mm - m): the output of a head whose weights of v were taken
 // relative to mm and whose denominator relative to m (0 for an empty row). The

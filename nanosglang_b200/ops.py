@@ -387,7 +387,8 @@ def int8_linear(x: torch.Tensor, weight_int8: torch.Tensor, weight_scale: torch.
                 bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """W8A8 linear: x is quantised per token (``int8_quantize``), the codes are
     multiplied in int32 (exact) and the sums scaled in float32:
-    ``y = (codes @ weight_int8^T) * scale * weight_scale + bias``.
+    ``y = (codes @ weight_int8^T) * scale * weight_scale + bias``, in that order
+    and rounded once to y's type.
 
     x: [..., K] float16 or bfloat16; weight_int8 int8 [N, K], weight_scale
     float32 [N]; returns [..., N] in x's dtype. K must be a multiple of 16, at
@@ -550,6 +551,8 @@ def kv_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     (grouped-query); page_table int32 [B, W]: the pages of each sequence in
     order; seq_lens int32 [B]: tokens held (0 for a padded row: its output is
     0, its log-sum-exp -inf). ``softmax_scale`` defaults to head_dim ** -0.5.
+    Scores and sums are float32, the weights of v float16 (relative to their
+    largest: 11 bits each). The caches may be expanded views.
     Returns out [B, heads, head_dim] in q's dtype, with ``return_lse`` also the
     natural log-sum-exp of the scaled scores, float32 [B, heads]. Entries of
     page_table past a sequence's last page are never read. A page outside the

@@ -135,7 +135,9 @@ class Int8Linear(nn.Module):
     No counterpart in the reference; it takes the place of its quantised
     linears. Buffers: ``weight_int8`` int8 [N, K], ``weight_scale`` float32 [N]
     (one per output channel). ``forward`` quantises x per token, multiplies the
-    codes exactly in int32 and scales the sums: see ``ops.int8_linear``. As a
+    codes exactly in int32 and scales the sums: see ``ops.int8_linear``. A
+    ``model.half()`` casts ``weight_scale`` like any buffer, to 11 bits (8 for
+    bfloat16) and a conversion in every forward: cast first, then quantise. As a
     row-parallel shard, each rank quantises its own slice of x (a scale of its
     own, so at least as fine as one over the whole row).
     """
