@@ -95,6 +95,9 @@ class DecodeEngine:
 
     @torch.no_grad()
     def capture(self, buckets: Sequence[int] = ()):
+        # each bucket's two steps ahead of the capture write behind what the slots hold
+        if max(self.held) + 2 > self.max_len or self.rows + 2 > self.max_steps + 1:
+            raise ValueError("no room for the steps ahead of a capture: capture before the prefill")
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
         for bs in (buckets or self.buckets):

@@ -75,3 +75,16 @@ def test_prompts_past_the_slot_are_refused(kv_cache):
         eng.prefill(prompts(21))
     with pytest.raises(ValueError, match="slots"):
         eng.prefill(prompts(1, 1, 1, 1, 1))
+
+
+@pytest.mark.parametrize("kv_cache", ["", "int8"])
+def test_capture_past_the_slot_is_refused(kv_cache):
+    """A capture runs two steps first; behind a slot that is nearly full they
+    would write into the next one."""
+    eng = make(kv_cache=kv_cache)
+    eng.held = [3, 19, 0, 0]
+    with pytest.raises(ValueError, match="capture"):
+        eng.capture()
+    eng.held, eng.rows = [3, 18, 0, 0], 12
+    with pytest.raises(ValueError, match="capture"):
+        eng.capture()
