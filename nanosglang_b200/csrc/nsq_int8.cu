@@ -22,7 +22,7 @@ constexpr int kQThreads = 256;
 // ---------------------------------------------------------------------------
 // Row quantiser: TPR threads per row, NV vectors of 16 bytes each, which stay in
 // registers between the maximum and the codes (one pass over DRAM, which bounds
-// it: 8192 x 4096 bf16 18.4 us, 5.5 TB/s; 16 x 4096 1.6 us). The host says
+// it: 8192 x 4096 bf16 18.9 us, 5.3 TB/s; 16 x 4096 1.6 us). The host says
 // how many threads a row takes. int8_quantize_any_kernel takes any row
 // length, alignment and type, element by element, and reads the row twice (the
 // second time from L2).

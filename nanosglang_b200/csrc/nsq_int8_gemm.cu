@@ -459,6 +459,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) int8_gemm_kernel(const __grid
     if (STAGED && etid == 0) bulk_wait_group<0>();
   }
 
+  // A wait ran out: of the copies asked for, those of stages whose barrier was
+  // never armed cannot be waited for. They land within microseconds; nobody
+  // leaves, or uses the ring, for a millisecond.
+  if (*abort_flag) {
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
+
   if constexpr (SPLIT) {
     // Every CTA's MMAs are done, so every ring is idle: here it takes this CTA's
     // sums [TOK][kRows + 4], and behind them the others' of its slice [CTA][slice][kRows + 4].
