@@ -27,6 +27,7 @@ constexpr int kQThreads = 256;
 // length, alignment and type, element by element, and reads the row twice (the
 // second time from L2).
 // ---------------------------------------------------------------------------
+
 // What of programmatic launch a quantiser takes part in: it waits for the kernel
 // ahead, and lets the one behind start at once. That one may be a product which
 // loads its weight before it waits, so only a quantiser launched for the

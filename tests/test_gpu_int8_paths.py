@@ -53,3 +53,14 @@ def test_k_split_over_a_cluster(m, k, n, dtype, bias):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows(m, k, n, dtype):
     check(m, k, n, dtype, [None, dtype, torch.float32][(m + n) % 3])
+
+
+def test_one_token_without_a_batch_dimension():
+    from nanosglang_b200 import ops
+    x, w, ws, b = make(1, 512, 70, torch.bfloat16, torch.bfloat16)
+    want = ops.int8_linear(x, w, ws, b)
+    assert torch.equal(ops.int8_linear(x[0], w, ws, b), want[0])
+    codes, s = ops.int8_quantize(x[0])
+    assert codes.shape == (512,) and s.shape == ()
+    assert torch.equal(ops.int8_linear_quantized(codes, s, w, ws, b), want[0])
+    assert torch.equal(ops.int8_linear(x.expand(9, 512), w, ws, b), want.expand(9, 70))

@@ -52,3 +52,38 @@ def test_write_of_half_a_thousand_million_rows():
     ops.kv_cache_write(row.expand(n, 1, dim), row.expand(n, 1, dim), *pool, slots)
     ops.kv_cache_write(row.expand(3, 1, dim), row.expand(3, 1, dim), *want, slots[-3:].clone())
     assert all(torch.equal(a, b) for a, b in zip(pool, want))
+
+
+def test_attention_over_expanded_queries_and_tables():
+    """One query for all heads, one page table for all sequences (stride 0), and
+    one page named many times."""
+    from nanosglang_b200 import ops
+    page, heads, dim, width = 16, 2, 64, 20
+    pool = make_pool(30, page, heads, dim, torch.int8, seed=36)
+    g = torch.Generator().manual_seed(37)
+    lens = torch.tensor([0, 1, 77, 320, 5], dtype=torch.int32).cuda()
+    table = torch.randperm(30, generator=g)[:width].int().cuda()
+    table[3:9] = table[3]
+    q = torch.randn(5, 1, dim, generator=g).half().cuda()
+    out, lse = ops.kv_attention_decode(q.expand(5, 6, dim), *pool, table.expand(5, width), lens, return_lse=True)
+    full = table.repeat(5, 1)
+    check_attention(out, lse, q.repeat(1, 6, 1), pool, full, lens, dim ** -0.5)
+    want = ops.kv_attention_decode(q.repeat(1, 6, 1), *pool, full, lens)
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("width", [3, 12])
+def test_attention_of_thousands_of_sequences(width):
+    """More sequences than a block has threads, most of them empty or short."""
+    from nanosglang_b200 import ops
+    b, page, dim = 5003, 16, 64
+    pool = make_pool(64, page, 1, dim, torch.int8, seed=38)
+    g = torch.Generator().manual_seed(39)
+    lens = torch.randint(-30, 17 * width, (b,), generator=g).clamp(0, page * width).int()
+    lens[-1] = page * width
+    table = torch.randint(0, 64, (b, width), generator=g).int()
+    q = torch.randn(b, 2, dim, generator=g).bfloat16()
+    out, lse = ops.kv_attention_decode(q.cuda(), *pool, table.cuda(), lens.cuda(), return_lse=True)
+    at = torch.cat([torch.arange(0, b, 61), torch.tensor([b - 1])])
+    check_attention(out[at.cuda()], lse[at.cuda()], q[at], pool, table[at], lens[at], dim ** -0.5)
+    assert (out[(lens == 0).cuda()] == 0).all() and out.isfinite().all()
