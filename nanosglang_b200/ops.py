@@ -65,6 +65,11 @@ def _weight(t: torch.Tensor) -> torch.Tensor:
     return _settled(_aligned(t), t)
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """The scales, zero points or bias of a linear, contiguous."""
+    return t if t.is_contiguous() else _settled(t.contiguous(), t)
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -74,8 +79,7 @@ def _bias_arg(bias: Optional[torch.Tensor]):
         return None, _lib.DTYPE_NONE
     if bias.dtype not in _BIAS_CODES:
         raise TypeError(f"bias dtype {bias.dtype} not supported")
-    if not bias.is_contiguous():
-        bias = _settled(bias.contiguous(), bias)
+    bias = _dense(bias)
     return bias, _BIAS_CODES[bias.dtype]
 
 
@@ -137,10 +141,7 @@ def awq_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zer
         raise RuntimeError(f"x has {x.shape[-1]} features, the layer expects {k}")
     if not qweight.is_contiguous() or qweight.data_ptr() & 15:
         qweight = _weight(qweight)
-    if not scales.is_contiguous():
-        scales = _weight(scales)
-    if not zeros.is_contiguous():
-        zeros = _weight(zeros)
+    scales, zeros = _dense(scales), _dense(zeros)
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     if not x2.is_contiguous() or x2.data_ptr() & 15:
         x2 = _aligned(x2)
@@ -650,8 +651,8 @@ def linear_multi(x: torch.Tensor, mods) -> Optional[list]:
         if len(gs) != 1 or any(mm.in_features != k for mm in mods):
             return None
         qws = [_weight(mm.qweight) for mm in mods]
-        scs = [_weight(mm.scales) for mm in mods]
-        zrs = [_weight(mm.zeros) for mm in mods]
+        scs = [_dense(mm.scales) for mm in mods]
+        zrs = [_dense(mm.zeros) for mm in mods]
         rc = lib.nsq_awq_linear_multi(_ptr(x2), _ACT_CODES[x.dtype], m, k, len(mods),
                                       _ptr_array([t.data_ptr() for t in qws]), _ptr_array([t.data_ptr() for t in scs]),
                                       _ptr_array([t.data_ptr() for t in zrs]), n_arr, gs.pop(), b_arr, bcode, _ptr(y),
@@ -699,7 +700,8 @@ def gate_up_silu(x: torch.Tensor, gate, up) -> Optional[torch.Tensor]:
     if type(gate).__name__ == "AWQLinear":
         if gate.group_size != up.group_size or gate.in_features != k or up.in_features != k:
             return None
-        qg, sg, zg, qu, su, zu = (_weight(t) for mod in (gate, up) for t in (mod.qweight, mod.scales, mod.zeros))
+        qg, qu = _weight(gate.qweight), _weight(up.qweight)
+        sg, zg, su, zu = (_dense(t) for mod in (gate, up) for t in (mod.scales, mod.zeros))
         rc = lib.nsq_awq_gate_up_silu(_ptr(x2), _ACT_CODES[x.dtype], m, k, n, _ptr(qg), _ptr(sg), _ptr(zg), _ptr(qu),
                                       _ptr(su), _ptr(zu), gate.group_size, _ptr(y), _stream(x))
     elif type(gate).__name__ == "FP8Linear":
